@@ -451,9 +451,114 @@ int slora_tables_compact(const int64_t* a_start, const int64_t* a_len, const int
                          int64_t* new_len, int64_t* new_loc, void* new_scaling, int64_t* scratch, int64_t* counts,
                          uint8_t* mem_state, int64_t tot_rows, int32_t* status, void* stream);
 
+/*
+ * ---- 8-bit KV cache ------------------------------------------------------------------------------------------------
+ * No counterpart in the reference, whose KV rows share the pool's 16-bit type.  A cache of pages: page p holds
+ * page_tokens tokens of every KV head, k and v as [n_pages][kv_heads][page_tokens][head_dim] 8-bit values, with one FP32
+ * scale per (page, KV head) for k and one for v (value = scale * stored).  Pages are handed out by any allocator of
+ * rows, slora_pool_alloc_rows over a map of pages among them.
+ */
+#define SLORA_KV_INT8 0 /* two's complement, -127 .. 127 */
+#define SLORA_KV_E4M3 1 /* 4 exponent and 3 mantissa bits, largest value 448 */
+
+typedef struct slora_kv8_cache { /* one layer */
+  void* k;          /* 16-byte aligned */
+  void* v;
+  float* k_scale;   /* [n_pages][kv_heads] */
+  float* v_scale;
+  float* weights;   /* [n_pages][kv_heads][page_tokens] accumulated attention weights, or NULL */
+  int64_t n_pages;
+  int page_tokens;  /* 16, 32, 64 or 128 */
+  int kv_heads;
+  int head_dim;     /* 64, 128 or 256 */
+  int kind;         /* SLORA_KV_INT8 or SLORA_KV_E4M3 */
+} slora_kv8_cache;
+
+typedef struct slora_kv8_batch { /* the sequences of a step; every table is device memory */
+  const int64_t* page_table; /* [n_seq][max_pages], rows table_stride entries apart */
+  int64_t table_stride;
+  const int32_t* kv_len;     /* [n_seq] tokens of the sequence in the cache, the step's new tokens included */
+  const int32_t* q_start;    /* [n_seq] first row of the sequence's new tokens in q, k, v */
+  const int32_t* q_len;      /* [n_seq] new tokens: the last q_len of the kv_len */
+  int32_t* status;           /* device word that collects SLORA_STATUS_* bits, or NULL */
+  int n_seq;
+  int max_pages;
+  int max_q_len;             /* no q_len is larger: sizes launches; a longer sequence is skipped (BAD_TABLE) */
+} slora_kv8_batch;
+/* A sequence with q_len < 0, q_len > max_q_len, kv_len < 0, kv_len > max_pages * page_tokens or rows outside q is skipped
+ * with SLORA_STATUS_BAD_TABLE; so is a page outside [0, n_pages).  Outputs of rows that belong to no sequence, or to a
+ * skipped one, are left as they are. */
+
+/*
+ * Rotary embedding of q [T][q_heads][head_dim] and k [T][k_heads][head_dim] (either may be NULL with 0 heads; rows
+ * *_stride elements apart, heads contiguous) into q_out / k_out (which may be q / k).  The first `rot` elements of a head
+ * are turned, the others copied.  Pair i: elements (i, i + rot / 2) with layout 0 ("half", the reference's
+ * rotary_emb_fwd, slora/models/llama/triton_kernel/rotary_emb.py:8-71), (2i, 2i + 1) with layout 1 ("interleaved").
+ *   angle = 2 pi positions[t] turns[i] (turns: rot / 2 doubles, device), (c, s) = factor * (cos, sin) of the angle,
+ *   y0 = x0 c - x1 s, y1 = x0 s + x1 c; inverse != 0 turns the other way, which is also the gradient's direction.
+ * Angles are reduced in 64 bits (far positions keep theirs), products are FP32, one rounding at the end.
+ * head_dim 64, 128 or 256; rot a multiple of 16 up to head_dim.
+ */
+int slora_rotary(void* q_out, void* k_out, const void* q, const void* k, int64_t T, int q_heads, int k_heads,
+                 int head_dim, int rot, int64_t q_out_stride, int64_t k_out_stride, int64_t q_stride, int64_t k_stride,
+                 const int64_t* positions, const double* turns, float factor, int layout, int inverse, int dtype,
+                 void* stream);
+
+/*
+ * Append the step's new tokens to the cache: k and v [T][kv_heads][head_dim] (rows k_stride / v_stride elements apart) of
+ * sequence b's rows q_start .. q_start + q_len go to positions kv_len - q_len .. kv_len of its pages.  With turns != NULL
+ * k is turned first and, when q is given, q_out = rotary(q) for q_heads heads (as slora_rotary; k itself is not written,
+ * and is not rounded between rotation and quantisation).
+ * Per touched page and KV head: s_new = max(s_old, max |x| / top) over the new values x (top 127 or 448; s_old = 0 when
+ * the page holds no older token of the sequence); new values become round(x / s_new); when s_new > s_old the page's older
+ * values q become round(q * s_old / s_new).  Rounding is to nearest, ties to even, of the exact quotient.  NaN is stored as
+ * 0 and infinities as the largest value (both leave the scale alone) with SLORA_STATUS_NONFINITE.  weights of new
+ * tokens, where the cache has them, become 0.  Positions beyond kv_len of the last page are left as they are.
+ */
+#define SLORA_STATUS_NONFINITE 16 /* a NaN or an infinity was appended to an 8-bit cache */
+int slora_kv8_append(const slora_kv8_cache* cache, const slora_kv8_batch* batch, const void* k, const void* v,
+                     int64_t k_stride, int64_t v_stride, int64_t T, const void* q, void* q_out, int q_heads,
+                     int64_t q_stride, int64_t q_out_stride, const int64_t* positions, const double* turns, int rot,
+                     float factor, int layout, int dtype, void* stream);
+
+/*
+ * Tokens first[b] .. first[b] + count - 1 (first == NULL: from 0) of each sequence as 16-bit values, k_out and v_out
+ * [n_seq][count][kv_heads][head_dim] contiguous; positions at and beyond kv_len read as zero.
+ */
+int slora_kv8_read(const slora_kv8_cache* cache, const slora_kv8_batch* batch, const int32_t* first, int64_t count,
+                   void* k_out, void* v_out, int dtype, void* stream);
+
+/*
+ * Attention of q [T][q_heads][head_dim] over the cache: query j of sequence b (row q_start + j) sees keys up to position
+ * kv_len - q_len + j, the last `window` of them when window > 0; q head h uses KV head h / (q_heads / kv_heads).
+ *   p = softmax(scale * q . k), out = sum p v, lse = log sum exp (natural; may be NULL)
+ * A query that sees no key gives 0 and lse -inf.  add_weights != 0: cache->weights += the p of every key, summed over
+ * the step's queries and over the q heads of its KV head.
+ * workspace: slora_kv8_attend_workspace_bytes(...) bytes of device memory, 16-byte aligned, contents irrelevant; calls
+ * that may overlap on the GPU need workspaces of their own.
+ */
+size_t slora_kv8_attend_workspace_bytes(const slora_kv8_cache* cache, const slora_kv8_batch* batch, int64_t T,
+                                        int q_heads, int add_weights);
+int slora_kv8_attend(const slora_kv8_cache* cache, const slora_kv8_batch* batch, const void* q, int64_t q_stride,
+                     int64_t T, int q_heads, void* out, int64_t out_stride, float* lse, float scale, int window,
+                     int add_weights, void* workspace, size_t workspace_bytes, int dtype, void* stream);
+
+/*
+ * Eviction by accumulated weight: of every sequence longer than `budget` each KV head keeps budget tokens, the first
+ * `sink`, the last `recent` and, of the others, those with the largest weights (ties: the lowest position; a NaN counts
+ * as the largest), in their order; shorter sequences keep all.  kept [n_seq][kv_heads][budget] int32 receives the kept
+ * positions (-1 behind the last).  The kept tokens move to positions 0 .. of the pages of dest_table (rows
+ * dest_stride entries apart; the batch's own page table: in place), their weights with them.  A destination page whose
+ * tokens all keep their position is copied as it is; every other gets the scale max |value| / top of its tokens
+ * and the values round(q * s_old / s_new) (as slora_kv8_append).  Destination pages must be disjoint from all source
+ * pages, or the batch's own table.  The sequences' new length is min(kv_len, budget).
+ */
+int slora_kv8_evict(const slora_kv8_cache* cache, const slora_kv8_batch* batch, int budget, int recent, int sink,
+                    int32_t* kept, const int64_t* dest_table, int64_t dest_stride, int dest_pages, void* stream);
+
 /* Kernels this process has launched through the library so far, per family:
  * out[0] simple (one CTA per work item), out[1] pipelined (persistent, warp-specialised), out[2] tensor core
- * (tcgen05, long segments), out[3] plan building and table validation.  The counters only ever grow; a caller
+ * (tcgen05, long segments), out[3] plan building, table validation, pool bookkeeping and the 8-bit cache.  The counters only ever grow; a caller
  * that wants the launches of a region subtracts two readings.  (Accounting aid: the reference has no counterpart;
  * its kernel launches are counted by the profiler.) */
 void slora_launch_counts(int64_t out[4]);

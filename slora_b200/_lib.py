@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_int, c_int32, c_int64, c_size_t, c_uint, c_void_p, c_char_p, POINTER
+from ctypes import c_float, c_int, c_int32, c_int64, c_size_t, c_uint, c_void_p, c_char_p, POINTER
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("SLORA_B200_LIB") or os.path.join(_HERE, "libslora_b200.so")   # override: a development build
@@ -24,7 +24,23 @@ def flag_resolved(max_rank: int) -> int:
     """``SLORA_FLAG_RESOLVED(max_rank)``: the plan holds resolved tiles for adapters of rank up to ``max_rank``."""
     return (((int(max_rank) + 7) >> 3) & 0x1f) << 8 if 0 < max_rank <= 128 else 0
 
-STATUS_BITS = {1: "bad adapter id", 2: "bad table entry", 4: "unsupported rank", 8: "bulk-copy wait timed out"}
+KV_INT8, KV_E4M3 = 0, 1
+
+
+class Kv8Cache(ctypes.Structure):
+    """``slora_kv8_cache``: one layer of an 8-bit cache."""
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p), ("weights", c_void_p),
+                ("n_pages", c_int64), ("page_tokens", c_int), ("kv_heads", c_int), ("head_dim", c_int), ("kind", c_int)]
+
+
+class Kv8Batch(ctypes.Structure):
+    """``slora_kv8_batch``: the sequences of a step."""
+    _fields_ = [("page_table", c_void_p), ("table_stride", c_int64), ("kv_len", c_void_p), ("q_start", c_void_p),
+                ("q_len", c_void_p), ("status", c_void_p), ("n_seq", c_int), ("max_pages", c_int), ("max_q_len", c_int)]
+
+
+STATUS_BITS = {1: "bad adapter id", 2: "bad table entry", 4: "unsupported rank", 8: "bulk-copy wait timed out",
+               16: "a NaN or an infinity was appended"}
 
 
 def _load():
@@ -97,6 +113,15 @@ _SIGS = {
     "slora_pool_free_rows": (c_int, [_P, c_int64, _P, c_int64, _P, _P]),
     "slora_tables_compact": (c_int, [_P, _P, _P, _P, _P, c_int64, c_int64, _P, _P, _P, _P, _P, _P, _P, c_int64, _P,
                                      _P]),
+    "slora_rotary": (c_int, [_P, _P, _P, _P, c_int64, c_int, c_int, c_int, c_int, c_int64, c_int64, c_int64, c_int64, _P,
+                             _P, c_float, c_int, c_int, c_int, _P]),
+    "slora_kv8_append": (c_int, [_P, _P, _P, _P, c_int64, c_int64, c_int64, _P, _P, c_int, c_int64, c_int64, _P, _P, c_int,
+                                 c_float, c_int, c_int, _P]),
+    "slora_kv8_read": (c_int, [_P, _P, _P, c_int64, _P, _P, c_int, _P]),
+    "slora_kv8_attend_workspace_bytes": (c_size_t, [_P, _P, c_int64, c_int, c_int]),
+    "slora_kv8_attend": (c_int, [_P, _P, _P, c_int64, c_int64, c_int, _P, c_int64, _P, c_float, c_int, c_int, _P, c_size_t,
+                                 c_int, _P]),
+    "slora_kv8_evict": (c_int, [_P, _P, c_int, c_int, c_int, _P, _P, c_int64, c_int, _P]),
     "slora_plan_info": (c_int, [_P, _P, _P, _P, _P]),
     "slora_plan_header": (c_int, [_P, _P, _P]),
     "slora_launch_counts": (None, [_P]),
@@ -158,3 +183,27 @@ def current_stream_ptr() -> int:
     of a B200 box, a third of a call's time in Python); the raw query behind it takes a tenth of that."""
     from torch import _C
     return _C._cuda_getCurrentRawStream(_C._cuda_getDevice())
+
+
+class _Here:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE_CTX = _Here()
+
+
+def on_device(first, *others):
+    """Context in which the device of ``first`` is the current one.  All tensors must lie on it."""
+    index = first.device.index
+    for t in others:
+        if t is not None and t.device.index != index:
+            raise RuntimeError(f"tensors of one call lie on devices {index} and {t.device.index}")
+    from torch import _C
+    if index == _C._cuda_getDevice():
+        return _HERE_CTX
+    import torch
+    return torch.cuda.device(index)

@@ -16,6 +16,8 @@ import os
 import torch
 
 from . import _lib
+from .kv_cache import KvCache8
+from .rotary import RotaryTable, _positions, rotary
 
 
 class BatchPlan:
@@ -190,12 +192,20 @@ class LoraBatchOps:
         to rows ``rows[t]`` of the KV-pool buffers ``k_out`` / ``v_out`` instead of updating ``k`` / ``v`` in place
         (``destindex_copy_kv``, ``transformer_layer_infer_template.py:50-62``).  Both happen in the expand's epilogue
         where the kernels allow (C entry ``slora_batch_lora_qkv_rope``).
+
+        ``rope=(table, positions)`` with a :class:`~slora_b200.RotaryTable` and the tokens' positions takes any of its
+        layouts and scalings; ``kv_dest=(cache, batch)`` with a :class:`~slora_b200.KvCache8` and the step's
+        :class:`~slora_b200.KvBatch` puts the new k and v into the layer's 8-bit pages (turned first when ``rope`` is
+        given).  Both run as one launch behind the expand; q, k and v hold base plus delta in place (q turned).
         """
         kb, vb, rows, stride = self._common(layer_id)
         _lib.require_cuda(x, q, k, v)
         if k.size(1) != v.size(1):
             raise RuntimeError("k and v must have the same width")
         d = self.delta
+        if isinstance(rope[0] if rope is not None else None, RotaryTable) or \
+                isinstance(kv_dest[0] if kv_dest is not None else None, KvCache8):
+            return self._lora_get_qkv_kv8(layer_id, x, q, k, v, rope, kv_dest, int(head_dim))
         if rope is not None:
             cos, sin = rope
             _lib.require_cuda(cos, sin)
@@ -234,6 +244,23 @@ class LoraBatchOps:
             self.a_loc.data_ptr(), self.a_scaling.data_ptr(), self.a_start.numel(), self.a_loc.numel(),
             d[0].data_ptr(), d[1].data_ptr(), d[2].data_ptr(), d[0].stride(0), self.max_lora_dim, x.size(0),
             _lib.dtype_code(x.dtype), self.flags, _lib.current_stream_ptr()))
+        return q
+
+    def _lora_get_qkv_kv8(self, layer_id, x, q, k, v, rope, kv_dest, head_dim):
+        if rope is not None and (not isinstance(rope[0], RotaryTable) or rope[0].head_dim != head_dim):
+            raise RuntimeError("an 8-bit cache takes rope=(RotaryTable, positions) of its head_dim")
+        if kv_dest is not None and (not isinstance(kv_dest[0], KvCache8) or kv_dest[0].head_dim != head_dim):
+            raise RuntimeError("a RotaryTable goes with kv_dest=(KvCache8, KvBatch) of its head_dim, or none")
+        heads = [t.view(t.size(0), -1, head_dim) for t in (q, k, v)]
+        if rope is not None:
+            _lib.require_cuda(rope[1])
+            _positions(rope[1], x.size(0))
+        self.lora_get_qkv(layer_id, x, q, k, v)
+        if kv_dest is None:
+            rotary(rope[0], rope[1], heads[0], heads[1])
+        else:
+            cache, batch = kv_dest
+            cache.append(layer_id, batch, heads[1], heads[2], q=heads[0] if rope is not None else None, rope=rope)
         return q
 
     def lora_get_o(self, layer_id, x, o):

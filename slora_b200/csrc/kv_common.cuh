@@ -1,0 +1,144 @@
+// 8-bit paged KV cache: argument blocks, page lookup, 8-bit conversions and the exact rounding of quotients that the
+// append, read, attention and eviction kernels share.
+//
+// A page holds `page` tokens of every KV head: values [page id][head][token][d] of one byte, one FP32 scale per (page,
+// head) for k and one for v.  One (page, head) is a contiguous run of page * d bytes, so a head's tokens stream in
+// runs of 1 to 32 KB wherever the pages lie, and the scale costs 4 bytes per run.
+#pragma once
+
+#include "lora_common.cuh"
+
+namespace slora {
+
+constexpr int kStatusNonfinite = SLORA_STATUS_NONFINITE;
+
+struct KvCache {
+  uint8_t* k;
+  uint8_t* v;
+  float* ks;
+  float* vs;
+  float* w;
+  int64_t n_pages;
+  int shift;  // log2 of the tokens of a page
+  int hkv;
+  int d;
+};
+
+struct KvBatch {
+  const int64_t* table;
+  int64_t table_stride;
+  const int32_t* kv_len;
+  const int32_t* q_start;
+  const int32_t* q_len;
+  int32_t* status;
+  int n_seq;
+  int max_q;
+  int64_t max_tokens;  // max_pages * page: no sequence may be longer
+  int64_t T;           // rows of q, k, v
+};
+
+// One sequence, checked: a bad one has no new tokens and no keys.
+struct KvSeq {
+  int kv, q, row;  // tokens in the cache, new ones among them, first row of the new ones
+  bool bad;
+};
+__device__ __forceinline__ KvSeq kv_seq(const KvBatch& b, int i) {
+  KvSeq s;
+  s.kv = b.kv_len[i];
+  s.q = b.q_len[i];
+  s.row = b.q_start[i];
+  s.bad = s.kv < 0 || s.kv > b.max_tokens || s.q < 0 || s.q > b.max_q || s.row < 0 ||
+          (s.q > 0 && static_cast<int64_t>(s.row) + s.q > b.T);
+  if (s.bad) s.kv = s.q = s.row = 0;
+  return s;
+}
+
+// Page of position `pos` of sequence i, -1 when the table's entry is no page.
+__device__ __forceinline__ int64_t kv_page(const KvCache& c, const KvBatch& b, int i, int pos) {
+  const int64_t p = b.table[i * b.table_stride + (pos >> c.shift)];
+  return p >= 0 && p < c.n_pages ? p : -1;
+}
+
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
+  return __byte_perm(a, b, sel);
+}
+
+// ---- 8-bit values ---------------------------------------------------------------------------------------------------
+// Pairs of stored bytes become pairs of f16 without a conversion instruction.  int8: the byte with its sign bit flipped
+// under the exponent byte 0x64 is 1024 + 128 + q, exact, and one packed subtraction leaves q.  e4m3: sign, exponent and
+// mantissa land in their f16 fields (a shift by one below the sign), which is the value times 2^-8; the factor goes into
+// the scale (denormals included: they become f16 denormals, which the tensor pipe multiplies exactly).
+template <int KIND>
+struct Kv8;
+template <>
+struct Kv8<SLORA_KV_INT8> {
+  static constexpr float kTop = 127.f;
+  static constexpr float kScale = 1.f;  // what a converted pair still has to be multiplied by
+  static constexpr bool kInt = true;
+  // bytes -> bytes that pair() takes
+  __device__ static __forceinline__ uint32_t prepare(uint32_t w) { return w ^ 0x80808080u; }
+  __device__ static __forceinline__ uint32_t finish(uint32_t v) {  // v = (0x64, b1, 0x64, b0)
+    uint32_t r;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(0x64806480u));
+    return r;
+  }
+  // f16x2 of bytes 0, 1 / 2, 3 of a prepared word
+  __device__ static __forceinline__ uint32_t lo(uint32_t w) { return finish(prmt(w, 0x64646464u, 0x4140)); }
+  __device__ static __forceinline__ uint32_t hi(uint32_t w) { return finish(prmt(w, 0x64646464u, 0x4342)); }
+  __device__ static __forceinline__ float value(uint8_t b) { return static_cast<float>(static_cast<int8_t>(b)); }
+};
+template <>
+struct Kv8<SLORA_KV_E4M3> {
+  static constexpr float kTop = 448.f;
+  static constexpr float kScale = 256.f;
+  static constexpr bool kInt = false;
+  __device__ static __forceinline__ uint32_t prepare(uint32_t w) { return w; }
+  __device__ static __forceinline__ uint32_t finish(uint32_t v) {  // v = (b1, 0, b0, 0)
+    return (v & 0x80008000u) | ((v >> 1) & 0x3f803f80u);
+  }
+  __device__ static __forceinline__ uint32_t lo(uint32_t w) { return finish(prmt(w, 0, 0x1404)); }
+  __device__ static __forceinline__ uint32_t hi(uint32_t w) { return finish(prmt(w, 0, 0x3424)); }
+  __device__ static __forceinline__ float value(uint8_t b) {
+    const __half_raw h = {static_cast<unsigned short>(((b & 0x80u) << 8) | ((b & 0x7fu) << 7))};
+    return __half2float(__half(h)) * 256.f;
+  }
+};
+
+// round((x + lo) / s) in the 8-bit type, to nearest, ties to even, of the exact quotient (s > 0; x + lo exact in two FP32
+// words, |lo| <= ulp(x) / 2).  The FP32 quotient is within an ulp or so of the exact one, so it decides everywhere but
+// next to a border between two 8-bit values; there the sign of x + lo - border * s does (fma: one rounding, and the
+// difference is small).  Pages that are scaled anew sit on such borders often: their ratios are small fractions.
+// Returns the stored byte.
+template <int KIND>
+__device__ __forceinline__ uint32_t kv_round(float x, float lo, float s) {
+  const float y = __fdiv_rn(x, s);
+  float m = fabsf(y);
+  float step = 1.f, inv = 1.f;
+  if (!Kv8<KIND>::kInt) {  // spacing of the type at m: three bits behind the leading one, 2^-9 below 2^-6
+    const uint32_t e = max(__float_as_uint(m) >> 23, 121u);
+    step = __uint_as_float((e - 3u) << 23);
+    inv = __uint_as_float((257u - e) << 23);  // 2^(3 - (e - 127)), e <= 254 - 3 for every value below the clamp
+    if (m > 1024.f) return (__float_as_uint(y) >> 31 << 7) | 0x7eu;
+  } else {
+    m = fminf(m, 1024.f);
+  }
+  const float k = m * inv;  // in steps, exact
+  const float f = floorf(k);
+  const float off = k - f;
+  float r = off > 0.5f || (off == 0.5f && (static_cast<int>(f) & 1)) ? f + 1.f : f;
+  if (fabsf(off - 0.5f) < 2e-4f) {
+    const float border = copysignf((f + 0.5f) * step, y);
+    const float diff = copysignf(1.f, y) * (__fmaf_rn(-border, s, x) + lo);
+    r = diff > 0.f ? f + 1.f : diff < 0.f ? f : f + static_cast<float>(static_cast<int>(f) & 1);
+  }
+  const uint32_t sign = __float_as_uint(y) >> 31;
+  if (Kv8<KIND>::kInt) {
+    const int q = static_cast<int>(fminf(r, 127.f));
+    return static_cast<uint32_t>(sign ? -q : q) & 0xffu;
+  }
+  const float v = fminf(r * step, 448.f);  // a value of the type
+  const uint32_t h = __half_as_ushort(__float2half_rn(v * (1.f / 256.f)));  // sign-less f16 fields, exact
+  return (sign << 7) | (h >> 7);
+}
+
+}  // namespace slora

@@ -1,0 +1,267 @@
+// Eviction from the 8-bit cache by accumulated attention weight: which tokens a (sequence, KV head) keeps, and their move
+// to the front pages.
+//
+// Select: the budget-th largest weight by radix selection, 8 bits at a time, on the weights mapped to ordered integers
+// (in shared memory when they fit); then one sweep in position order that places every kept position.  Ties go to the
+// lowest position because the sweep counts them in order.  What bounds it: reading the weights once, and a chain of four
+// histogram passes per (sequence, head).
+//
+// Move: the scale of a page belongs to its tokens, so a page with new neighbours gets a new scale and its values new
+// roundings: max over tokens of |q| * s in 64 bits (exact), then the exact rounding of q * s / s_new.  Kept positions
+// never move up, so in place a CTA can work through a head's pages in order, reading a round of pages before it writes
+// them; with other destination pages all rounds run at once.  Bound by bytes: kept tokens read and written once.
+#pragma once
+
+#include "kv_common.cuh"
+
+namespace slora {
+
+constexpr int kSelectThreads = 1024;
+constexpr int kSelectCopies = 8;             // histogram copies: weights share few exponents, so bins are contended
+constexpr int kMoveThreads = 256;
+constexpr int kMoveWarps = kMoveThreads / 32;
+
+struct EvictArgs {
+  KvCache c;
+  KvBatch b;
+  int budget, recent, sink;
+  int32_t* kept;  // [n_seq][hkv][budget]
+  const int64_t* dest;
+  int64_t dest_stride;
+  int in_place;
+  int cached;     // weights that fit the select kernel's shared memory
+  int chunks;     // CTAs per (sequence, head) of the move
+};
+
+__device__ __forceinline__ uint32_t weight_key(float w) {
+  if (w != w) return 0xffffffffu;
+  const uint32_t b = __float_as_uint(w == 0.f ? 0.f : w);
+  return b >> 31 ? ~b : b | 0x80000000u;
+}
+
+__global__ void __launch_bounds__(kSelectThreads) kv_select_kernel(const EvictArgs a) {
+  extern __shared__ uint32_t keys[];
+  __shared__ int hist[kSelectCopies][256];
+  __shared__ uint32_t s_prefix;
+  __shared__ int s_left;
+  __shared__ int s_count[2][32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int seq = blockIdx.x / a.c.hkv, head = blockIdx.x - seq * a.c.hkv;
+  int n = a.b.kv_len[seq];
+  if (n < 0 || n > a.b.max_tokens) {
+    if (tid == 0) set_status(a.b.status, SLORA_STATUS_BAD_TABLE);
+    n = 0;
+  }
+  int32_t* kept = a.kept + static_cast<int64_t>(blockIdx.x) * a.budget;
+  if (n <= a.budget) {
+    for (int j = tid; j < a.budget; j += kSelectThreads) kept[j] = j < n ? j : -1;
+    return;
+  }
+  const int c0 = a.sink, c1 = n - a.recent;  // candidates
+  const int want = a.budget - a.sink - a.recent;
+  auto weight_at = [&](int i) {
+    const int64_t p = kv_page(a.c, a.b, seq, i);
+    if (p < 0) {
+      set_status(a.b.status, SLORA_STATUS_BAD_TABLE);
+      return 0u;
+    }
+    return weight_key(a.c.w[((p * a.c.hkv + head) << a.c.shift) + (i & ((1 << a.c.shift) - 1))]);
+  };
+  for (int i = c0 + tid; i < c1 && i - c0 < a.cached; i += kSelectThreads) keys[i - c0] = weight_at(i);
+  auto key_at = [&](int i) { return i - c0 < a.cached ? keys[i - c0] : weight_at(i); };
+  if (tid == 0) {
+    s_prefix = 0;
+    s_left = want;
+  }
+  // the want-th largest key: after the pass at `shift` the top bits of the threshold are known and s_left of the keys
+  // that share them still have to be taken
+  for (int shift = 24; shift >= 0 && want > 0; shift -= 8) {
+    for (int i = tid; i < kSelectCopies * 256; i += kSelectThreads) hist[0][i] = 0;
+    __syncthreads();
+    const uint32_t prefix = s_prefix, mask = shift == 24 ? 0u : ~0u << (shift + 8);
+    for (int i = c0 + tid; i < c1; i += kSelectThreads) {
+      const uint32_t k = key_at(i);
+      if ((k & mask) == prefix) atomicAdd(&hist[warp % kSelectCopies][(k >> shift) & 255u], 1);
+    }
+    __syncthreads();
+    if (warp == 0) {
+      // lane l holds bins 255 - 8 l .. 248 - 8 l; counts from the top
+      int v[8], sum = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        v[e] = 0;
+#pragma unroll
+        for (int x = 0; x < kSelectCopies; ++x) v[e] += hist[x][255 - 8 * lane - e];
+        sum += v[e];
+      }
+      int incl = sum;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += y;
+      }
+      int before = incl - sum;
+      const int left = s_left;
+      __syncwarp();
+      if (before < left && left <= incl) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (before < left && left <= before + v[e]) {
+            s_prefix = prefix | static_cast<uint32_t>(255 - 8 * lane - e) << shift;
+            s_left = left - before;
+          }
+          before += v[e];
+        }
+      }
+    }
+    __syncthreads();
+  }
+  __syncthreads();
+  const uint32_t limit = want > 0 ? s_prefix : 0xffffffffu;
+  const int equal = want > 0 ? s_left : 0;  // keys equal to the limit that are kept, the first ones
+  int above = 0, ties = 0;                  // kept above the limit / equal to it, before this sweep's positions
+  int buf = 0;
+  for (int base = 0; base < n; base += kSelectThreads, buf ^= 1) {
+    const int i = base + tid;
+    bool gt = false, eq = false;
+    if (i < n) {
+      if (i < c0 || i >= c1) {
+        gt = true;
+      } else if (want > 0) {
+        const uint32_t k = key_at(i);
+        gt = k > limit;
+        eq = k == limit;
+      }
+    }
+    const uint32_t mg = __ballot_sync(0xffffffffu, gt), me = __ballot_sync(0xffffffffu, eq);
+    if (lane == 0) s_count[buf][warp] = __popc(mg) | __popc(me) << 16;
+    __syncthreads();
+    int v = s_count[buf][lane];
+    const int own = v;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, v, d);
+      if (lane >= d) v += y;
+    }
+    const int total = __shfl_sync(0xffffffffu, v, 31);
+    const int before = __shfl_sync(0xffffffffu, v - own, warp);
+    const uint32_t lower = (1u << lane) - 1u;
+    const int g = above + (before & 0xffff) + __popc(mg & lower), e = ties + (before >> 16) + __popc(me & lower);
+    if (gt || (eq && e < equal)) kept[g + min(e, equal)] = i;
+    above += total & 0xffff;
+    ties += total >> 16;
+  }
+}
+
+template <int D, int KIND>
+__global__ void __launch_bounds__(kMoveThreads) kv_move_kernel(const EvictArgs a) {
+  using V8 = Kv8<KIND>;
+  constexpr int kLanes = D / 16, kRows = 32 / kLanes, kSteps = 16 / kRows;  // a warp: 16 tokens, 16 bytes a lane
+  __shared__ double s_top[kMoveWarps];
+  __shared__ int s_same[kMoveWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % kLanes, rr = lane / kLanes;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int sh = static_cast<int>(blockIdx.x);
+  const int seq = sh / a.c.hkv, head = sh - seq * a.c.hkv;
+  int n = a.b.kv_len[seq];
+  if (n < 0 || n > a.b.max_tokens) n = 0;
+  const int m = min(n, a.budget);
+  if (a.in_place && n <= a.budget) return;
+  const int32_t* kept = a.kept + static_cast<int64_t>(sh) * a.budget;
+  const int page = 1 << a.c.shift, in_page = page - 1;
+  const int team = page / 16;              // warps of a unit: (page, k or v)
+  const int at_once = kMoveWarps / team;   // units of a round
+  const int units = 2 * ((m + page - 1) >> a.c.shift);
+  const int rounds = (units + at_once - 1) / at_once;
+  const int mine = warp / team, part = warp - mine * team;
+  for (int round = blockIdx.y; round < rounds; round += a.chunks) {
+    const int unit = round * at_once + mine;
+    const int block = unit >> 1, is_v = unit & 1;
+    const bool active = unit < units;
+    const uint8_t* src8 = is_v ? a.c.v : a.c.k;
+    const float* src_s = is_v ? a.c.vs : a.c.ks;
+    // read: this warp's 16 tokens
+    uint4 w[kSteps];
+    float s[kSteps];
+    double top = 0.0;
+    bool same = true;
+    float weight = 0.f;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      w[i] = make_uint4(0, 0, 0, 0);
+      s[i] = 0.f;
+      const int j = block * page + part * 16 + i * kRows + rr;
+      if (active && j < m) {
+        const int from = kept[j];
+        same = same && from == j;
+        const int64_t p = kv_page(a.c, a.b, seq, from);
+        if (p >= 0) {
+          const int64_t ph = p * a.c.hkv + head;
+          w[i] = *reinterpret_cast<const uint4*>(src8 + ((ph << a.c.shift) + (from & in_page)) * D + 16 * sub);
+          s[i] = src_s[ph];
+        } else {
+          set_status(a.b.status, SLORA_STATUS_BAD_TABLE);
+        }
+      }
+    }
+    const int jw = block * page + part * 16 + lane;  // lanes 0..15: the weight of a token each
+    if (active && !is_v && lane < 16 && jw < m) {
+      const int from = kept[jw];
+      const int64_t p = kv_page(a.c, a.b, seq, from);
+      if (p >= 0) weight = a.c.w[((p * a.c.hkv + head) << a.c.shift) + (from & in_page)];
+    }
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      float q = 0.f;
+      const uint8_t* b = reinterpret_cast<const uint8_t*>(&w[i]);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) q = fmaxf(q, fabsf(V8::value(b[e])));
+      top = fmax(top, static_cast<double>(q) * static_cast<double>(s[i]));
+    }
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, d));
+    same = __all_sync(0xffffffffu, same);
+    if (lane == 0) {
+      s_top[warp] = top;
+      s_same[warp] = same;
+    }
+    __syncthreads();  // every warp has read its pages
+    for (int x = 0; x < team; ++x) {
+      top = fmax(top, s_top[mine * team + x]);
+      same = same && s_same[mine * team + x];
+    }
+    if (active) {
+      const int64_t dp = a.dest[seq * a.dest_stride + block];
+      if (dp < 0 || dp >= a.c.n_pages) {
+        if (lane == 0) set_status(a.b.status, SLORA_STATUS_BAD_TABLE);
+      } else if (!(a.in_place && same)) {
+        const int64_t ph = dp * a.c.hkv + head;
+        uint8_t* dst = (is_v ? a.c.v : a.c.k) + (ph << a.c.shift) * D;
+        const float keep_s = __shfl_sync(0xffffffffu, s[0], 0);
+        const float now = static_cast<float>(top / static_cast<double>(V8::kTop));
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+          const int slot = part * 16 + i * kRows + rr;
+          if (!same) {
+            uint8_t* b = reinterpret_cast<uint8_t*>(&w[i]);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float q = V8::value(b[e]);
+              const float y = q * s[i];
+              b[e] = now > 0.f ? static_cast<uint8_t>(kv_round<KIND>(y, __fmaf_rn(q, s[i], -y), now)) : 0;
+            }
+          }
+          if (block * page + slot < m) *reinterpret_cast<uint4*>(dst + slot * D + 16 * sub) = w[i];
+        }
+        if (part == 0 && lane == 0) (is_v ? a.c.vs : a.c.ks)[ph] = same ? keep_s : now;
+        if (!is_v && lane < 16 && jw < m) a.c.w[(ph << a.c.shift) + part * 16 + lane] = weight;
+      }
+    }
+    __syncthreads();  // s_top / s_same are free, and in place the round's pages are written before the next reads
+  }
+}
+
+}  // namespace slora

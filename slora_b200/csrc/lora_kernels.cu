@@ -14,6 +14,7 @@
 #include <cstdlib>
 #include <cstring>
 
+#include "host_common.h"
 #include "lora_common.cuh"
 #include "lora_pipelined.cuh"
 #include "lora_rope.cuh"
@@ -23,6 +24,27 @@
 #include "pool_ops.cuh"
 
 using namespace slora;
+
+// ---- what the library's source files share on the host (host_common.h) ----
+namespace slora {
+static thread_local char g_err[512] = "";
+std::atomic<long long> g_launches[4];
+
+int fail(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_err, sizeof(g_err), fmt, ap);
+  va_end(ap);
+  return code;
+}
+
+int check_launch(const char* what, int kernels, int family) {
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return fail(SLORA_ERR_LAUNCH, "%s: %s", what, cudaGetErrorString(e));
+  g_launches[family].fetch_add(kernels, std::memory_order_relaxed);
+  return SLORA_OK;
+}
+}  // namespace slora
 
 namespace {
 
@@ -245,32 +267,10 @@ __global__ void zero_report_kernel(int32_t* report) {
 // ------------------------------------------------------------------------------------------------------------
 // host side
 // ------------------------------------------------------------------------------------------------------------
-thread_local char g_err[512] = "";
-
-int fail(int code, const char* fmt, ...) {
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(g_err, sizeof(g_err), fmt, ap);
-  va_end(ap);
-  return code;
-}
-
-inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
 int pow2_divisor(int64_t v, int cap) {
   int p = 1;
   while (p * 2 <= cap && v % (p * 2) == 0) p *= 2;
   return p;
-}
-
-// Kernels launched so far by this process, per family: 0 simple, 1 pipelined, 2 tensor core, 3 plan / tables.
-std::atomic<long long> g_launches[4];
-
-int check_launch(const char* what, int kernels) {
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return fail(SLORA_ERR_LAUNCH, "%s: %s", what, cudaGetErrorString(e));
-  g_launches[3].fetch_add(kernels, std::memory_order_relaxed);
-  return SLORA_OK;
 }
 
 int max_tiles_for(int64_t T, int64_t n_adapters) {
