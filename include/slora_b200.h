@@ -487,7 +487,7 @@ typedef struct slora_kv8_batch { /* the sequences of a step; every table is devi
 } slora_kv8_batch;
 /* A sequence with q_len < 0, q_len > max_q_len, kv_len < 0, kv_len > max_pages * page_tokens or rows outside q is skipped
  * with SLORA_STATUS_BAD_TABLE; so is a page outside [0, n_pages).  Outputs of rows that belong to no sequence, or to a
- * skipped one, are left as they are. */
+ * skipped one, are left as they are.  Sequences' rows must not overlap. */
 
 /*
  * Rotary embedding of q [T][q_heads][head_dim] and k [T][k_heads][head_dim] (either may be NULL with 0 heads; rows

@@ -72,14 +72,14 @@ __device__ __forceinline__ int64_t kv_seq_units(const KvAttendArgs& a, const KvS
 
 // Sum over all sequences and the sequence that holds unit `want(total)`.  Every thread adds up a run of sequences.
 struct KvFind {
-  long long sums[kAttendWarps];
+  long long sums[16];
   long long at;  // units before the sequence
   int seq;
 };
-template <typename Units, typename Want>
+template <int WARPS, typename Units, typename Want>
 __device__ __forceinline__ long long kv_find(int n_seq, KvFind* sh, const Units& units, const Want& want) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int per = (n_seq + kAttendThreads - 1) / kAttendThreads;
+  const int per = (n_seq + 32 * WARPS - 1) / (32 * WARPS);
   const int i0 = min(tid * per, n_seq), i1 = min(i0 + per, n_seq);
   long long mine = 0;
   for (int i = i0; i < i1; ++i) mine += units(i);
@@ -93,7 +93,7 @@ __device__ __forceinline__ long long kv_find(int n_seq, KvFind* sh, const Units&
   __syncthreads();
   long long before = incl - mine, total = 0;
 #pragma unroll
-  for (int w = 0; w < kAttendWarps; ++w) {
+  for (int w = 0; w < WARPS; ++w) {
     if (w < warp) before += sh->sums[w];
     total += sh->sums[w];
   }
@@ -299,7 +299,7 @@ __global__ void __launch_bounds__(kAttendThreads, NT == 1 && D <= 128 ? 4 : 2) k
   pdl_wait();
   const long long me = blockIdx.x, grid = gridDim.x;
   if (tid == 0) *reinterpret_cast<int4*>(a.rec + 4 * me) = make_int4(-1, 0, 0, 0);
-  const long long total = kv_find(
+  const long long total = kv_find<kAttendWarps>(
       a.b.n_seq, &sm.find,
       [&](int i) {
         const KvSeq x = kv_seq(a.b, i);
@@ -646,7 +646,7 @@ __global__ void __launch_bounds__(kAttendThreads, D <= 128 ? 4 : 2) kv_weights_k
     const KvRange r = kv_units(s, a.window);
     return static_cast<long long>(r.hi - r.lo) * a.c.hkv;
   };
-  const long long total = kv_find(a.b.n_seq, &find, units, [&](long long n) { return me * ((n + grid - 1) / grid); });
+  const long long total = kv_find<kAttendWarps>(a.b.n_seq, &find, units, [&](long long n) { return me * ((n + grid - 1) / grid); });
   const long long run = (total + grid - 1) / grid;
   long long u = me * run;
   const long long u_end = min(u + run, total);

@@ -8,6 +8,7 @@
 #include "kv_attend.cuh"
 #include "kv_common.cuh"
 #include "kv_evict.cuh"
+#include "kv_prefill.cuh"
 
 using namespace slora;
 
@@ -180,13 +181,23 @@ int attend_tiles(int max_q, int group, int d) {
 }
 int attend_grid(int nt, int d) { return sm_count() * (nt == 1 && d <= 128 ? 4 : 2); }
 
+// Sequences with at least this many rows go to the tensor-memory kernel (kv_prefill.cuh), the others to kv_attend.cuh.
+constexpr int kPrefillRows = 64;
+
 struct AttendLayout {
   int nt, grid;
+  int split;           // q_len from which sequences are the prefill kernel's; above max_q: none
+  int64_t pre_grid;    // its items, at most
   size_t part, rec, lse, total;
 };
 AttendLayout attend_layout(const KvCache& c, const KvBatch& b, int hq, int add_weights) {
   AttendLayout l;
-  l.nt = attend_tiles(b.max_q, hq / c.hkv, c.d);
+  const int group = hq / c.hkv;
+  l.split = c.d <= 128 ? (kPrefillRows + group - 1) / group : 0x7fffffff;
+  const bool pre = b.max_q >= l.split;
+  l.nt = attend_tiles(pre ? l.split - 1 : b.max_q, group, c.d);
+  const int64_t seqs = b.n_seq < b.T ? b.n_seq : b.T;
+  l.pre_grid = pre ? (b.T * group / kPreRows + seqs) * c.hkv : 0;
   l.grid = attend_grid(l.nt, c.d);
   const auto up = [](size_t x) { return (x + 15) & ~static_cast<size_t>(15); };
   l.part = 0;
@@ -212,6 +223,16 @@ int attend_launch(KvAttendArgs a, const AttendLayout& l, int add_weights, cudaSt
     if (l.nt == 4) rc = attend_nt<D, 4, KIND, T>(a, l.grid, s);
   }
   if (rc) return rc;
+  if constexpr (D <= 128) {
+    if (l.pre_grid > 0) {
+      KvAttendArgs p = a;
+      p.min_q = l.split;
+      p.lim_q = a.b.max_q;
+      rc = launch_pdl(kv_prefill_kernel<D, KIND, T>, dim3(static_cast<unsigned>(l.pre_grid)), kPreThreads, sizeof(PreSmem<D>) + 1024, s, p,
+                      "kv8_attend prefill");
+      if (rc) return rc;
+    }
+  }
   rc = launch_pdl(kv_join_kernel<D, T>, dim3(l.grid), kJoinThreads, 0, s, a, "kv8_attend join");
   if (rc || !add_weights) return rc;
   a.rows_per_block = 8;
@@ -391,7 +412,7 @@ int slora_kv8_attend(const slora_kv8_cache* cache, const slora_kv8_batch* batch,
   a.scale2 = scale * 1.4426950408889634f;
   a.window = window;
   a.min_q = 0;
-  a.lim_q = a.b.max_q;
+  a.lim_q = l.split - 1;
   a.part = reinterpret_cast<float*>(ws + l.part);
   a.rec = reinterpret_cast<int*>(ws + l.rec);
   cudaStream_t s = static_cast<cudaStream_t>(stream);

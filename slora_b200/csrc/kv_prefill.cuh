@@ -1,0 +1,466 @@
+// Attention over the 8-bit cache for many query rows per sequence and KV head (chunks of prompts): tcgen05.
+//
+// 4 d multiply-adds per key and row against 2 d bytes per key: from some dozens of rows on the tensor pipe bounds it, and
+// the exponentials next to it: 128 keys x 128 rows take 1024 cycles of the pipe (d 128) and as many of the SM's 16
+// exponentials a cycle.  Hence two row tiles of 128 per CTA that take turns: while one is in its softmax, the tensor pipe
+// works on the other.
+//   rows of a tile = (new token, q head of the KV head) pairs in that order, one thread each in the softmax
+//   S = Q K^T    128 x 128, Q and K in shared memory (f16, 128-byte swizzle, inner dimension d)
+//   P            over S in tensor memory (f16 pairs), the A operand of the second product
+//   O += P V     V in shared memory as it lies in the cache, keys outside: the outer-major form of the same layout
+// Roles: four warps convert 8-bit pages to f16 operands (values exact, as in kv_attend.cuh), one lane issues the MMAs, four
+// warps per row tile do the softmax.  Scales never touch the operands: a page's k scale multiplies its 16-column groups of
+// S (the maximum of a group is taken before it), its v scale, relative to the largest one of the sequence, goes into the
+// exponent of p, and comes out of the sum of p again per group.  The running maximum is raised only when a score passes
+// it by 2^8; then the row's O is rescaled in tensor memory.  P(j) replaces S(j) and S(j + 1) replaces P(j): the MMAs of a
+// CTA run in order, so the commit behind S(j + 1) also says that O has P(j) V(j).
+//
+// Every wait is bounded; a CTA that gives up records SLORA_STATUS_TIMEOUT and frees its tensor memory.
+#pragma once
+
+#include "kv_attend.cuh"
+#include "lora_mma.cuh"
+
+namespace slora {
+
+constexpr int kPreSoftWarps = 8, kPreCvtWarps = 4;
+constexpr int kPreThreads = (kPreSoftWarps + kPreCvtWarps + 1) * 32;
+constexpr int kPreKeys = 128;                // keys of a step
+constexpr int kPreRows = 256;                // rows of a CTA
+constexpr int kPreGroups = kPreKeys / 16;    // 16 keys share their scales whatever the page size
+constexpr int kPreScaleSlots = 4;            // steps whose scales are kept: the softmax of a step reads them after its K is gone
+constexpr float kPreRange = 64.f;            // p * vs / vmax * 64 <= 2^8 * 2^6: inside f16
+
+template <int D>
+struct PreSmem {
+  uint8_t q[2][128 * D * 2];   // row tiles; [64 elements][row][128 bytes]
+  uint8_t k[2][kPreKeys * D * 2];
+  uint8_t v[2][kPreKeys * D * 2];
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full;
+  uint32_t tmem;
+  int bad;
+  unsigned vmax;
+  float fk[kPreScaleSlots][kPreGroups], lv[kPreScaleSlots][kPreGroups], rv[kPreScaleSlots][kPreGroups];
+  KvFind find;
+};
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, "
+      "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
+        "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+        "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};\n" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+      "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// D[tmem] (+)= A[tmem] * B[smem], one K = 16 step: A's 16 columns of f16 lie in eight columns of tensor memory.
+__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n"
+      "}\n" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(0u)
+      : "memory");
+}
+// Outer-major operand with the 128-byte swizzle: rows (keys) of 64 elements of the outer dimension (d), eight of them 1024
+// bytes, the next eight keys 1024 bytes on, the next 64 elements `lbo` bytes on.
+__device__ __forceinline__ uint64_t umma_smem_desc_sw128_mn(uint32_t addr, uint32_t lbo) {
+  uint64_t d = static_cast<uint64_t>((addr & 0x3ffffu) >> 4);
+  d |= static_cast<uint64_t>(lbo >> 4) << 16;
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(2) << 61;
+  return d;
+}
+
+// (sequence, 256 rows, head) items; the last rows of a sequence see the most keys and come first.
+__device__ __forceinline__ long long pre_items(const KvAttendArgs& a, const KvSeq& s) {
+  if (s.q < a.min_q || s.q > a.lim_q || s.q == 0) return 0;
+  return static_cast<long long>((s.q * a.group + kPreRows - 1) / kPreRows) * a.c.hkv;
+}
+
+template <int D, int KIND, typename T>
+__global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_kernel(const KvAttendArgs a) {
+  using V8 = Kv8<KIND>;
+  constexpr int kHalf = kPreKeys * 128;  // bytes of 64 elements of a 128-row operand
+  extern __shared__ uint8_t smem_raw[];
+  PreSmem<D>& sm = *reinterpret_cast<PreSmem<D>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  pdl_launch_dependents();
+  pdl_wait();
+  const long long item = blockIdx.x;
+  const long long total = kv_find<kPreThreads / 32>(
+      a.b.n_seq, &sm.find, [&](int i) { return pre_items(a, kv_seq(a.b, i)); }, [&](long long) { return item; });
+  // the grid holds every item unless sequences share rows
+  if (total > static_cast<long long>(gridDim.x) && item == 0 && tid == 0) set_status(a.b.status, SLORA_STATUS_BAD_TABLE);
+  if (item >= total) return;
+  const int seq = sm.find.seq;
+  const KvSeq s = kv_seq(a.b, seq);
+  const int rows = s.q * a.group, blocks = (rows + kPreRows - 1) / kPreRows;
+  const int idx = static_cast<int>(item - sm.find.at);
+  const int head = idx % a.c.hkv, row0 = (blocks - 1 - idx / a.c.hkv) * kPreRows;
+  // keys that the CTA's rows see: [key0, key_end), in steps of 128
+  const int last_row = min(row0 + kPreRows, rows) - 1;
+  const int base_to = s.kv - s.q + 1;  // keys that new token 0 sees end here
+  const int key_end = max(base_to + last_row / a.group, 0);
+  const int key0 = a.window > 0 ? max(base_to + row0 / a.group - a.window, 0) / kPreKeys * kPreKeys : 0;
+  const int steps = key_end > key0 ? (key_end - key0 + kPreKeys - 1) / kPreKeys : 0;
+
+  if (warp == kPreThreads / 32 - 1) {
+    tmem_alloc(&sm.tmem, 512);
+    tmem_relinquish();
+  }
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sm.k_full[i], kPreCvtWarps * 32);
+      mbar_init(&sm.v_full[i], kPreCvtWarps * 32);
+      mbar_init(&sm.k_empty[i], 1);
+      mbar_init(&sm.v_empty[i], 1);
+      mbar_init(&sm.s_full[i], 1);
+      mbar_init(&sm.p_full[i], 128);
+    }
+    mbar_init(&sm.o_full, 1);
+    sm.bad = 0;
+    sm.vmax = 0;
+    fence_barrier_init();
+  }
+  __syncthreads();
+  // the largest v scale of the pages in reach
+  {
+    float m = 0.f;
+    const int p1 = (key_end + (1 << a.c.shift) - 1) >> a.c.shift;
+    for (int p = (key0 >> a.c.shift) + tid; p < p1; p += kPreThreads) {
+      const int64_t id = kv_page(a.c, a.b, seq, p << a.c.shift);
+      if (id >= 0) m = fmaxf(m, a.c.vs[id * a.c.hkv + head]);
+    }
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+    if (lane == 0 && m > 0.f) atomicMax(&sm.vmax, __float_as_uint(m));
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem;
+  const float vmax = sm.vmax > 0 ? __uint_as_float(sm.vmax) : 1.f;
+  bool ok = true;
+
+  if (warp < kPreSoftWarps) {
+    // ---- softmax: one thread per row --------------------------------------------------------------------------------
+    const int tile = warp >> 2, r = tid & 127;  // warp % 4 is the tensor-memory quarter that the warp may touch
+    const int row = row0 + tile * 128 + r;
+    const bool real = row < rows;
+    const int j = real ? row / a.group : 0;
+    float down = 0.f;
+    {
+      uint8_t* dst = sm.q[tile];
+      const T* src = static_cast<const T*>(a.q) + (static_cast<int64_t>(s.row) + j) * a.q_stride + (head * a.group + row - j * a.group) * D;
+      float top = 0.f;
+#pragma unroll 4
+      for (int c = 0; c < D / 8; ++c) {
+        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (real) cvt8<T>(*reinterpret_cast<const uint4*>(src + 8 * c), x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
+      }
+      const int e2 = top > 0.f ? min(max(141 - static_cast<int>(__float_as_uint(top) >> 23), -100), 100) : 0;
+      float up = __uint_as_float(static_cast<uint32_t>(127 + e2) << 23);
+      down = __uint_as_float(static_cast<uint32_t>(127 - e2) << 23) * fabsf(a.scale2) * V8::kScale;
+      if (a.scale2 < 0.f) up = -up;
+#pragma unroll 4
+      for (int c = 0; c < D / 8; ++c) {
+        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (real) cvt8<T>(*reinterpret_cast<const uint4*>(src + 8 * c), x);
+        uint4 w;
+        w.x = pack_f16(x[0] * up, x[1] * up);
+        w.y = pack_f16(x[2] * up, x[3] * up);
+        w.z = pack_f16(x[4] * up, x[5] * up);
+        w.w = pack_f16(x[6] * up, x[7] * up);
+        *reinterpret_cast<uint4*>(dst + (c >> 3) * kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = w;
+      }
+      fence_proxy_async();
+      mbar_arrive(&sm.p_full[tile]);  // phase 0: Q is there
+    }
+    const int to = real ? max(base_to + j, 0) : 0, from = a.window > 0 ? max(to - a.window, 0) : 0;
+    int to_min = to, from_max = from;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      to_min = min(to_min, __shfl_xor_sync(0xffffffffu, to_min, d));
+      from_max = max(from_max, __shfl_xor_sync(0xffffffffu, from_max, d));
+    }
+    const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + lane_off + tile * 128, t_o = tmem + lane_off + 256 + tile * D;
+    float m = kNegInf, l = 0.f;
+    for (int i = 0; i < steps && ok; ++i) {
+      // the step's scales were written before k_full, which the MMAs behind this barrier waited for
+      ok = __all_sync(0xffffffffu, mbar_wait(&sm.s_full[tile], i & 1));
+      if (!ok) break;
+      tc_fence_after();
+      const int key = key0 + i * kPreKeys, slot = i & (kPreScaleSlots - 1);
+      const bool masked = key < from_max || key + kPreKeys > to_min;
+      float top = kNegInf;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t w[32];
+        tmem_ld32(t_s + 32 * c, w);
+        tmem_ld_wait();
+        if (masked) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const int pos = key + 32 * c + e;
+            if (pos < from || pos >= to) w[e] = 0xff800000u;
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float gm = __uint_as_float(w[16 * h]);
+#pragma unroll
+          for (int e = 1; e < 16; ++e) gm = fmaxf(gm, __uint_as_float(w[16 * h + e]));
+          if (gm > kNegInf && sm.lv[slot][2 * c + h] > kNegInf) top = fmaxf(top, gm * (down * sm.fk[slot][2 * c + h]));
+        }
+      }
+      const bool raise = top > m + kLazyMax;
+      if (__any_sync(0xffffffffu, raise)) {
+        const float now = fmaxf(m, top);
+        const float f = now == kNegInf ? 1.f : ex2(m - now);
+        m = now;
+        l *= f;
+        if (i > 0) {
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t w[32];
+            tmem_ld32(t_o + 32 * c, w);
+            tmem_ld_wait();
+            uint32_t y[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) y[e] = __float_as_uint(__uint_as_float(w[e]) * f);
+            tmem_st16(t_o + 32 * c, y);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) y[e] = __float_as_uint(__uint_as_float(w[16 + e]) * f);
+            tmem_st16(t_o + 32 * c + 16, y);
+          }
+        }
+      }
+      const float m0 = m == kNegInf ? 0.f : m;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t w[32];
+        tmem_ld32(t_s + 32 * c, w);
+        tmem_ld_wait();
+        uint32_t y[16];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float f = down * sm.fk[slot][2 * c + h], add = sm.lv[slot][2 * c + h] - m0;
+          float sum = 0.f;
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) {
+            float x0 = ex2(__fmaf_rn(__uint_as_float(w[16 * h + e]), f, add));
+            float x1 = ex2(__fmaf_rn(__uint_as_float(w[16 * h + e + 1]), f, add));
+            if (masked) {
+              const int pos = key + 32 * c + 16 * h + e;
+              if (pos < from || pos >= to) x0 = 0.f;
+              if (pos + 1 < from || pos + 1 >= to) x1 = 0.f;
+            }
+            sum += x0 + x1;
+            y[8 * h + e / 2] = pack_f16(x0, x1);
+          }
+          l = __fmaf_rn(sum, sm.rv[slot][2 * c + h], l);
+        }
+        tmem_st16(t_s + 16 * c, y);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&sm.p_full[tile]);
+    }
+    // ---- epilogue ---------------------------------------------------------------------------------------------------
+    if (ok && steps > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sm.o_full, 0));
+    if (ok) {
+      tc_fence_after();
+      const float inv = l > 0.f ? vmax * (V8::kScale / kPreRange) / l : (l == 0.f ? 0.f : l);
+      T* dst = static_cast<T*>(a.out) + (static_cast<int64_t>(s.row) + j) * a.out_stride + (head * a.group + row - j * a.group) * D;
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t w[32];
+        if (steps > 0) {
+          tmem_ld32(t_o + 32 * c, w);
+          tmem_ld_wait();
+        }
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          union {
+            uint4 u;
+            T e[8];
+          } p;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) p.e[e] = from_f32<T>(l == 0.f ? 0.f : __uint_as_float(w[8 * h + e]) * inv);
+          if (real) *reinterpret_cast<uint4*>(dst + 32 * c + 8 * h) = p.u;
+        }
+      }
+      if (real && a.lse) {
+        a.lse[(static_cast<int64_t>(s.row) + j) * a.hq + head * a.group + row - j * a.group] =
+            l == 0.f ? kNegInf : (m + log2f(l)) * 0.69314718055994531f;
+      }
+    }
+  } else if (warp < kPreSoftWarps + kPreCvtWarps) {
+    // ---- 8-bit pages -> f16 operands ----------------------------------------------------------------------------------
+    // A pass of the 128 threads takes 16 keys (one page: one scale); eight lanes share a key's 128 bytes so that the two
+    // 16-byte chunks of f16 that a lane stores fall on all banks: lanes 0-3 key x, 4-7 key x + 1, first half of d, ...
+    constexpr int kLanes = D / 16;                  // lanes of a key
+    constexpr int kPer = kPreKeys * kLanes / 128;   // 16-byte loads of a thread and operand
+    constexpr int kPassKeys = 128 / kLanes;         // keys of a pass: 16, or 32 for d 64
+    const int ct = tid - kPreSoftWarps * 32;
+    const int l2 = ct & 31, cw = ct >> 5;
+    int sub, key_in;  // which 16 elements, which key of the pass
+    if (D == 128) {
+      sub = (l2 & 3) + ((l2 >> 3) & 1) * 4;
+      key_in = cw * 4 + (l2 >> 4) * 2 + ((l2 >> 2) & 1);
+    } else {
+      sub = l2 & 3;
+      key_in = cw * 8 + (l2 >> 2);
+    }
+    const int in_page = (1 << a.c.shift) - 1;
+    uint4 kr[kPer], vr[kPer];
+    int64_t page_l = -1;                            // lane g: page * hkv + head of 16-key group g of the step that is loaded next
+    auto lookup = [&](int i) {
+      page_l = -1;
+      const int pos = key0 + i * kPreKeys + 16 * (l2 & (kPreGroups - 1));
+      if (i < steps && pos < s.kv) {
+        const int64_t p = kv_page(a.c, a.b, seq, pos);
+        if (p >= 0) page_l = p * a.c.hkv + head;
+        else set_status(a.b.status, SLORA_STATUS_BAD_TABLE);
+      }
+    };
+    auto fetch = [&](int i, const uint8_t* base, uint4 (&regs)[kPer]) {
+#pragma unroll
+      for (int p = 0; p < kPer; ++p) {
+        const int key = p * kPassKeys + key_in;
+        const int64_t ph = __shfl_sync(0xffffffffu, page_l, key >> 4);
+        regs[p] = make_uint4(0, 0, 0, 0);
+        if (ph >= 0) regs[p] = ld_stream16(base + ((ph << a.c.shift) + ((key0 + i * kPreKeys + key) & in_page)) * D + 16 * sub);
+      }
+    };
+    auto put = [&](const uint4 (&regs)[kPer], uint8_t* dst) {
+#pragma unroll
+      for (int p = 0; p < kPer; ++p) {
+        const int key = p * kPassKeys + key_in;
+        const uint32_t x = V8::prepare(regs[p].x), y = V8::prepare(regs[p].y), z = V8::prepare(regs[p].z), w = V8::prepare(regs[p].w);
+        const int c = 2 * sub;
+        uint8_t* row = dst + (c >> 3) * kHalf + key * 128;
+        *reinterpret_cast<uint4*>(row + (((c & 7) ^ (key & 7)) << 4)) = make_uint4(V8::lo(x), V8::hi(x), V8::lo(y), V8::hi(y));
+        *reinterpret_cast<uint4*>(row + ((((c + 1) & 7) ^ (key & 7)) << 4)) = make_uint4(V8::lo(z), V8::hi(z), V8::lo(w), V8::hi(w));
+      }
+    };
+    lookup(0);
+    int64_t page_now = page_l;
+    fetch(0, a.c.k, kr);
+    fetch(0, a.c.v, vr);
+    for (int i = 0; i < steps && ok; ++i) {
+      const int st = i & 1, slot = i & (kPreScaleSlots - 1);
+      page_now = page_l;
+      lookup(i + 1);
+      if (i >= 2) ok = mbar_wait(&sm.k_empty[st], ((i >> 1) - 1) & 1);
+      if (!(ok = __all_sync(0xffffffffu, ok))) break;
+      float vs = 0.f;
+      if (cw == 0 && l2 < kPreGroups) {
+        float f = 0.f, lv = kNegInf, rv = 1.f;
+        if (page_now >= 0) {
+          f = a.c.ks[page_now];
+          vs = a.c.vs[page_now];
+          // a scale of zero (or next to nothing beside the largest): the values count as zero, p only in the sum
+          const float rel = vs / vmax;
+          const bool some = rel > 1e-30f;
+          lv = (some ? log2f(rel) : 0.f) + 6.f;
+          rv = (some ? 1.f / rel : 1.f) * (1.f / kPreRange);
+        }
+        sm.fk[slot][l2] = f;
+        sm.lv[slot][l2] = lv;
+        sm.rv[slot][l2] = rv;
+      }
+      put(kr, sm.k[st]);
+      fence_proxy_async();
+      mbar_arrive(&sm.k_full[st]);
+      if (i + 1 < steps) fetch(i + 1, a.c.k, kr);
+      if (i >= 2) ok = mbar_wait(&sm.v_empty[st], ((i >> 1) - 1) & 1);
+      if (!(ok = __all_sync(0xffffffffu, ok))) break;
+      // values of pages whose scale does not count
+#pragma unroll
+      for (int p = 0; p < kPer; ++p) {
+        const int64_t ph = __shfl_sync(0xffffffffu, page_now, (p * kPassKeys + key_in) >> 4);
+        if (ph >= 0 && !(a.c.vs[ph] / vmax > 1e-30f)) vr[p] = make_uint4(0, 0, 0, 0);
+      }
+      put(vr, sm.v[st]);
+      fence_proxy_async();
+      mbar_arrive(&sm.v_full[st]);
+      if (i + 1 < steps) fetch(i + 1, a.c.v, vr);
+    }
+  } else if (lane == 0 && steps > 0) {
+    // ---- MMAs -----------------------------------------------------------------------------------------------------
+    const uint32_t idesc_s = umma_idesc<__half>(kPreKeys), idesc_o = umma_idesc<__half>(D) | (1u << 16);  // V: outer-major
+    auto score = [&](int tile, int st) {
+      const uint32_t qa = smem_u32(sm.q[tile]), kb = smem_u32(sm.k[st]);
+#pragma unroll
+      for (int x = 0; x < D / 16; ++x) {
+        const uint32_t off = (x >> 2) * kHalf + (x & 3) * 32;
+        umma_f16(tmem + tile * 128, umma_smem_desc_sw128(qa + off), umma_smem_desc_sw128(kb + off), idesc_s, x > 0);
+      }
+      umma_commit(&sm.s_full[tile]);
+    };
+    auto value = [&](int tile, int st, bool more) {
+      const uint32_t vb = smem_u32(sm.v[st]);
+#pragma unroll
+      for (int x = 0; x < kPreKeys / 16; ++x)
+        umma_f16_ts(tmem + 256 + tile * D, tmem + tile * 128 + 8 * x, umma_smem_desc_sw128_mn(vb + x * 2048, kHalf), idesc_o,
+                    more || x > 0);
+    };
+    ok = mbar_wait(&sm.p_full[0], 0) && mbar_wait(&sm.p_full[1], 0) && mbar_wait(&sm.k_full[0], 0);
+    if (ok) {
+      tc_fence_after();
+      score(0, 0);
+      score(1, 0);
+      umma_commit(&sm.k_empty[0]);
+    }
+    for (int i = 0; i < steps && ok; ++i) {
+      const int st = i & 1, nx = (i + 1) & 1;
+      const bool next = i + 1 < steps;
+      ok = mbar_wait(&sm.v_full[st], (i >> 1) & 1) && mbar_wait(&sm.p_full[0], (i + 1) & 1);
+      if (!ok) break;
+      tc_fence_after();
+      value(0, st, i > 0);
+      if (next) {
+        if (!(ok = mbar_wait(&sm.k_full[nx], ((i + 1) >> 1) & 1))) break;
+        tc_fence_after();
+        score(0, nx);
+      }
+      if (!(ok = mbar_wait(&sm.p_full[1], (i + 1) & 1))) break;
+      tc_fence_after();
+      value(1, st, i > 0);
+      umma_commit(&sm.v_empty[st]);
+      if (next) {
+        score(1, nx);
+        umma_commit(&sm.k_empty[nx]);
+      } else {
+        umma_commit(&sm.o_full);
+      }
+    }
+  }
+  if (!ok) sm.bad = 1;
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (sm.bad && tid == 0) set_status(a.b.status, SLORA_STATUS_TIMEOUT);
+  if (warp == kPreThreads / 32 - 1) tmem_dealloc(tmem, 512);
+}
+
+}  // namespace slora
