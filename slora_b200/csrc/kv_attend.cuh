@@ -5,7 +5,10 @@
 //
 // What bounds it: the cache is read once, 2 d bytes per key and KV head against 4 d multiply-adds per row, so up to some
 // dozens of rows the copy rate does.  Hence: no shared memory on the way of k and v.  A tile is 16 keys of one page; a warp
-// loads it with 16-byte loads straight into the registers that mma.sync.m16n8k16 takes as its A operand.
+// loads it with 16-byte loads straight into the registers that mma.sync.m16n8k16 takes as its A operand, each operand of
+// the next tile as soon as the present one has been multiplied.  (Rings in shared memory, filled by cp.async or by the
+// copy engine, measured 20 % slower over long sequences: the copies' issue, 900 cycles a tile and warp, is more than
+// the registers they free are worth.)
 //   S^T [16 keys x 8 rows] = K [16 x d] Q^T     thread (g, t) holds keys g, g + 8 and, of every 64 elements, the 16 from
 //                                               16 t on: any order of the inner dimension will do as long as q's is the
 //                                               same, so it is the order the bytes lie in.
@@ -17,10 +20,17 @@
 // sums is p's to f16 (2^-12 relative in the mean).  p is multiplied by vs (relative to a running power of two, so its f16
 // range holds for any scales) and the maximum is only raised when some score passes it by 2^8: no shuffles in most steps.
 //
-// Work is split over the whole batch at once: units of 64 keys of every (sequence, row block, KV head) in one row, cut
-// into equal runs, one per CTA; four warps take the 16-key tiles of a unit.  Every CTA adds up the lengths itself (one
-// round trip for a few hundred sequences), so there is no plan to build or to keep.  A run that ends inside a (sequence,
-// rows, head) leaves its part in the workspace and kv_join_kernel adds the parts in order: results do not depend on timing.
+// Work is split over the whole batch at once: the tiles of every (sequence, row block, KV head) in one row, cut into runs
+// of equal cost, one per CTA (a piece costs kAttendPiece tiles before its first key: its q, its page table, its output).
+// The four warps of a CTA take its tiles in turn, so that 8 KB of k and of v that lie together are read together (runs per
+// warp, without any join inside the CTA, measured 15 % slower over long sequences).  While a piece ends the next one's
+// first tiles are on their way.  Every CTA adds up the lengths itself (one round trip for a few hundred sequences), so
+// there is no plan to build or to keep.  A run that ends inside a (sequence, rows, head) leaves its part in the workspace
+// and kv_join_kernel adds the parts in order: results do not depend on timing.
+//
+// Attention weights (add_weights) need the softmax's sum first: the scores go to the workspace (4 bytes per key and row,
+// against the 2 d that the key cost) and kv_weights_kernel adds up their exponentials; where that would take too much
+// memory or the rows are many, kv_reweigh_kernel computes the scores again.
 #pragma once
 
 #include "kv_common.cuh"
@@ -29,11 +39,13 @@ namespace slora {
 
 constexpr int kAttendWarps = 4;
 constexpr int kAttendThreads = kAttendWarps * 32;
-constexpr int kAttendUnit = 64;        // keys: one 16-key tile per warp
-constexpr int kAttendMinUnits = 2;     // per CTA: shorter runs cost more in the join than they save
+constexpr int kAttendTile = 16;        // keys
+constexpr int kAttendPiece = 12;       // tiles that starting and ending a piece is worth
+constexpr int kAttendMinRun = kAttendPiece + 8;  // per CTA: shorter runs cost more in the join than they save
 constexpr float kLazyMax = 8.f;        // log2 of how far a score may pass the running maximum before it is raised
 constexpr float kPRange = 32.f;        // p * vs / ref * 32 <= 2^8 * 2 * 2^5: inside f16
 constexpr float kNegInf = -INFINITY;
+constexpr float kNoMax = -1e30f;       // maximum of no score: finite, so that differences of maxima are numbers
 
 struct KvAttendArgs {
   KvCache c;
@@ -44,39 +56,44 @@ struct KvAttendArgs {
   int64_t q_stride, out_stride;
   int hq, group;
   int rows_per_block;  // 8 * NT
+  int part_rows;       // rows of a block that any sequence has
   float scale2;        // scale * log2(e)
   int window;
   int min_q, lim_q;    // sequences with min_q <= q_len <= lim_q are this launch's
-  float* part;         // [2 * grid][rows_per_block * (d + 2)]
-  int* rec;            // [grid][4]: the (sequence, row block, head) that CTA is the first of and does not finish, its parts
+  int runs;            // CTAs that share the work
+  float* part;         // [2 * runs][part_rows * (d + 4)]: sums, maximum and sum of p per row (a multiple of 16 bytes)
+  int* rec;            // [runs][4]: the (sequence, row block, head) that a run is the first of and does not finish, its parts
+  float* scores;       // [cost units][part_rows][16] or null: scores of every tile, log2 units
 };
 
-// ---- the run of units of a CTA -----------------------------------------------------------------------------------------
+// ---- the run of tiles of a CTA ------------------------------------------------------------------------------------------
 struct KvRange {
-  int lo, hi;  // units [lo, hi) of a sequence's keys that some row of the step sees
+  int lo, hi;  // tiles [lo, hi) of a sequence's keys that some row of the step sees
 };
-__device__ __forceinline__ KvRange kv_units(const KvSeq& s, int window) {
+__device__ __forceinline__ KvRange kv_tiles(const KvSeq& s, int window) {
   KvRange r;
-  r.hi = s.q > 0 ? (s.kv + kAttendUnit - 1) / kAttendUnit : 0;
+  r.hi = s.q > 0 ? (s.kv + kAttendTile - 1) / kAttendTile : 0;
   r.lo = 0;
-  if (window > 0 && s.q > 0) r.lo = max(0, s.kv - s.q + 1 - window) / kAttendUnit;
-  if (r.hi <= r.lo && s.q > 0) r.hi = r.lo + 1;  // no key at all: one empty unit, so that the rows are written
+  if (window > 0 && s.q > 0) r.lo = max(0, s.kv - s.q + 1 - window) / kAttendTile;
+  if (r.hi <= r.lo && s.q > 0) r.hi = r.lo + 1;  // no key at all: one empty tile, so that the rows are written
   return r;
 }
-__device__ __forceinline__ int64_t kv_seq_units(const KvAttendArgs& a, const KvSeq& s) {
+__device__ __forceinline__ long long kv_seq_cost(const KvAttendArgs& a, const KvSeq& s) {
   if (s.q < a.min_q || s.q > a.lim_q || s.q == 0) return 0;
-  const KvRange r = kv_units(s, a.window);
+  const KvRange r = kv_tiles(s, a.window);
   const int blocks = (s.q * a.group + a.rows_per_block - 1) / a.rows_per_block;
-  return static_cast<int64_t>(r.hi - r.lo) * blocks * a.c.hkv;
+  return static_cast<long long>(r.hi - r.lo + kAttendPiece) * blocks * a.c.hkv;
 }
 
-// Sum over all sequences and the sequence that holds unit `want(total)`.  Every thread adds up a run of sequences.
+// Sum over all sequences and, for each of N targets, the sequence that holds unit want(total, k).  Every thread adds up a
+// run of sequences.
+constexpr int kFindTargets = 4;
 struct KvFind {
   long long sums[16];
-  long long at;  // units before the sequence
-  int seq;
+  long long at[kFindTargets];  // units before the sequence
+  int seq[kFindTargets];
 };
-template <int WARPS, typename Units, typename Want>
+template <int WARPS, int N, typename Units, typename Want>
 __device__ __forceinline__ long long kv_find(int n_seq, KvFind* sh, const Units& units, const Want& want) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per = (n_seq + 32 * WARPS - 1) / (32 * WARPS);
@@ -97,24 +114,30 @@ __device__ __forceinline__ long long kv_find(int n_seq, KvFind* sh, const Units&
     if (w < warp) before += sh->sums[w];
     total += sh->sums[w];
   }
-  const long long u = want(total);
-  if (u >= before && u < before + mine) {
-    for (int i = i0; i < i1; ++i) {
-      const long long n = units(i);
-      if (u < before + n) {
-        sh->seq = i;
-        sh->at = before;
-        break;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const long long u = want(total, k);
+    if (u >= before && u < before + mine) {
+      long long b = before;
+      for (int i = i0; i < i1; ++i) {
+        const long long n = per == 1 ? mine : units(i);
+        if (u < b + n) {
+          sh->seq[k] = i;
+          sh->at[k] = b;
+          break;
+        }
+        b += n;
       }
-      before += n;
     }
   }
   __syncthreads();
   return total;
 }
-__device__ __forceinline__ long long kv_run(long long total, int grid) {
-  const long long r = (total + grid - 1) / grid;
-  return r < kAttendMinUnits ? kAttendMinUnits : r;
+// Units of a run.  (Totals beyond 2^32 are no real batch: the division is 32-bit wherever it can be.)
+__device__ __forceinline__ long long kv_run(long long total, int runs) {
+  const long long n = total + runs - 1;
+  const long long r = n <= 0xffffffffll ? static_cast<long long>(static_cast<uint32_t>(n) / static_cast<uint32_t>(runs)) : n / runs;
+  return r < kAttendMinRun ? kAttendMinRun : r;
 }
 
 // ---- registers and mma -------------------------------------------------------------------------------------------------
@@ -134,9 +157,6 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-// What sums taken relative to maximum m weigh relative to `now`; sums that no finite score entered have m = -inf and
-// l = 0, or l = NaN (a row of q with a NaN), which has to come through.
-__device__ __forceinline__ float part_factor(float m, float l, float now) { return m == kNegInf ? l : ex2(m - now); }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return reinterpret_cast<const uint32_t&>(h);
@@ -169,7 +189,7 @@ struct KTile {
 };
 template <int D>
 struct VTile {
-  static constexpr int N = D / 32;       // words per key: D / 8 bytes in runs of 16 (8 for d 64)
+  static constexpr int N = D / 32;       // words per key: 16 bytes of every 128 (8 of 64)
   uint32_t w[4][N];                      // keys 2t, 2t + 1, 2t + 8, 2t + 9
   // element of word i, byte j: VTile::elem(g, i) + j
   __device__ static __forceinline__ int elem(int g, int i) {
@@ -193,7 +213,7 @@ struct VTile {
   }
 };
 
-// q of one row block as mma B operands: thread (g, t) holds row g of each n-tile, 16 elements of every 64.
+// q of one row block as mma B operands: thread (g, t) holds row g of each n-tile, the chunks of KTile.
 template <int D, int NT, typename T>
 struct QTile {
   static constexpr int C = D / 64;
@@ -243,15 +263,23 @@ struct QTile {
 template <int D, int NT, int KIND>
 __device__ __forceinline__ void kv_scores(float (&c)[NT][4], const KTile<D>& k, const uint32_t (&q)[NT][D / 16][2]) {
   using V8 = Kv8<KIND>;
+  // two chains of sums per n-tile: an mma waits for the one before it in its chain
+  float d[NT][4];
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) c[nt][0] = c[nt][1] = c[nt][2] = c[nt][3] = 0.f;
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c[nt][e] = d[nt][e] = 0.f;
 #pragma unroll
   for (int s = 0; s < D / 16; ++s) {
     const uint32_t x = V8::prepare(k.w[0][s >> 2][s & 3]), y = V8::prepare(k.w[1][s >> 2][s & 3]);
     const uint32_t a0 = V8::lo(x), a2 = V8::hi(x), a1 = V8::lo(y), a3 = V8::hi(y);
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) mma_f16(c[nt], a0, a1, a2, a3, q[nt][s][0], q[nt][s][1]);
+    for (int nt = 0; nt < NT; ++nt) mma_f16(s & 1 ? d[nt] : c[nt], a0, a1, a2, a3, q[nt][s][0], q[nt][s][1]);
   }
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c[nt][e] += d[nt][e];
 }
 
 // What a warp carries through its tiles of one (sequence, row block, head).
@@ -262,93 +290,182 @@ struct AttendState {
   float ref;               // power of two the value scales are taken relative to; 0: none yet
 };
 
-template <int D, int NT, int KIND, typename T>
-struct AttendTypes {
-  static constexpr int kRows = 8 * NT;
-  static constexpr int kRegs = NT * D / 4;           // accumulator words of a thread
-  static constexpr int kPartWords = kRows * (D + 2);
-  struct Smem {
-    KvFind find;
-    float o[kAttendWarps][kRegs][32];
-    float m[kAttendWarps][kRows], l[kAttendWarps][kRows], ref[kAttendWarps];
-  };
+// One piece of a run: tiles [first, first + count) of the `per` of one (sequence, row block, head).
+struct KvPiece {
+  KvSeq s;
+  int seq, idx;  // idx: row block * hkv + head
+  int lo, first, count, per;
+  int tiles;       // of the count, those that hold keys (a sequence without keys has one empty tile)
+  long long unit;  // cost unit of tile 0
 };
 
-// Rows 8 nt + 2 t + c of the row block: where their output goes.
-template <int D, int KIND, typename T>
-__device__ __forceinline__ void store_row4(const KvAttendArgs& a, const KvSeq& s, int head, int r, int elem, const float (&v)[4]) {
-  const int j = r / a.group;
-  T* row = static_cast<T*>(a.out) + (static_cast<int64_t>(s.row) + j) * a.out_stride + (head * a.group + r - j * a.group) * D + elem;
-  union {
-    uint2 u;
-    T e[4];
-  } p;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) p.e[i] = from_f32<T>(v[i]);
-  *reinterpret_cast<uint2*>(row) = p.u;
+// What a CTA needs between pieces only: in shared memory, so that the registers go to the tiles.
+struct KvRun {
+  KvPiece piece[4];        // piece p in slot p & 3; count 0: there is none
+  long long u, u_end;      // what is left of the run
+  long long at, cost;      // units before the sequence that was reached, units of it
+  int2 see[2][32];         // keys [x, y) that each row of an even / odd piece sees
+};
+
+// The next piece of the run into *out; `from`: the one before it.  (Called by one warp, once per piece: not inlined.)
+__device__ __noinline__ void kv_next_piece(const KvAttendArgs& a, KvRun* run, const KvPiece* from, KvPiece* out, int lane) {
+  KvPiece p = *from;
+  long long u = run->u, at = run->at, cost = run->cost;
+  const long long u_end = run->u_end;
+  p.count = 0;
+  while (u < u_end && p.count <= 0) {
+    while (u >= at + cost) {
+      at += cost;
+      p.s = kv_seq(a.b, ++p.seq);
+      cost = kv_seq_cost(a, p.s);
+    }
+    const KvRange range = kv_tiles(p.s, a.window);
+    // a cut inside a piece's first kAttendPiece units belongs to the run behind it
+    p.lo = range.lo;
+    p.per = range.hi - range.lo;
+    const int each = p.per + kAttendPiece;
+    const long long in = u - at;
+    p.idx = in <= 0xffffffffll ? static_cast<int>(static_cast<uint32_t>(in) / static_cast<uint32_t>(each)) : static_cast<int>(in / each);
+    const int begin = static_cast<int>(in - static_cast<long long>(p.idx) * each);
+    const int until = static_cast<int>(min(static_cast<long long>(each), begin + (u_end - u)));
+    p.first = max(begin - kAttendPiece, 0);
+    p.count = max(until - kAttendPiece, 0) - p.first;
+    p.unit = u - begin + kAttendPiece;
+    p.tiles = max(min(p.count, (p.s.kv + kAttendTile - 1) / kAttendTile - p.lo - p.first), 0);
+    u += until - begin;
+  }
+  if (p.count < 0) p.count = 0;
+  if (p.count == 0) p.tiles = 0;
+  __syncwarp();
+  if (lane == 0) {
+    *out = p;
+    run->u = u;
+    run->at = at;
+    run->cost = cost;
+  }
+  __syncwarp();
 }
 
+// Place (tile of the cache, -1: a bad page) and scales of this warp's tile base + lane of a piece.
+struct KvPlace {
+  int tile;
+  float ks, vs;
+};
+__device__ __noinline__ KvPlace kv_places(const KvAttendArgs& a, const KvPiece* piece, int base, int warp, int lane) {
+  KvPlace r = {-1, 0.f, -1.f};
+  const int tile = warp + (base + lane) * kAttendWarps;
+  if (tile < piece->tiles) {
+    const int key = (piece->lo + piece->first + tile) * kAttendTile, head = piece->idx % a.c.hkv;
+    const int64_t p = kv_page(a.c, a.b, piece->seq, key);
+    if (p >= 0) {
+      const int64_t ph = p * a.c.hkv + head;
+      r.tile = static_cast<int>((ph << (a.c.shift - 4)) + ((key & ((1 << a.c.shift) - 1)) >> 4));
+      r.ks = a.c.ks[ph];
+      r.vs = a.c.vs[ph];
+    } else {
+      set_status(a.b.status, SLORA_STATUS_BAD_TABLE);
+    }
+  }
+  return r;
+}
+
+template <int D, int NT>
+struct AttendSmem {
+  struct {
+    float o[kAttendWarps][NT * D / 4][32];
+    float2 ml[kAttendWarps][8 * NT];
+    float ref[kAttendWarps];
+  } join[2];
+  KvRun run;
+  KvFind find;
+};
+
 template <int D, int NT, int KIND, typename T>
-__global__ void __launch_bounds__(kAttendThreads, NT == 1 && D <= 128 ? 4 : 2) kv_attend_kernel(const KvAttendArgs a) {
+__global__ void __launch_bounds__(kAttendThreads, NT == 1 && D <= 128 ? 4 : 2) kv_attend_kernel(const __grid_constant__ KvAttendArgs a) {
   using V8 = Kv8<KIND>;
-  using Ty = AttendTypes<D, NT, KIND, T>;
   extern __shared__ __align__(16) uint8_t smem_raw[];
-  typename Ty::Smem& sm = *reinterpret_cast<typename Ty::Smem*>(smem_raw);
+  AttendSmem<D, NT>& sm = *reinterpret_cast<AttendSmem<D, NT>*>(smem_raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  KvRun* const run_state = &sm.run;
   pdl_launch_dependents();
   pdl_wait();
-  const long long me = blockIdx.x, grid = gridDim.x;
-  if (tid == 0) *reinterpret_cast<int4*>(a.rec + 4 * me) = make_int4(-1, 0, 0, 0);
-  const long long total = kv_find<kAttendWarps>(
+  const int me = blockIdx.x;
+  const long long total = kv_find<kAttendWarps, 1>(
       a.b.n_seq, &sm.find,
       [&](int i) {
         const KvSeq x = kv_seq(a.b, i);
         if (x.bad && me == 0) set_status(a.b.status, SLORA_STATUS_BAD_TABLE);
-        return static_cast<long long>(kv_seq_units(a, x));
+        return kv_seq_cost(a, x);
       },
-      [&](long long n) { return me * kv_run(n, static_cast<int>(grid)); });
-  const long long run = kv_run(total, static_cast<int>(grid));
-  long long u = me * run;
-  const long long u_end = min(u + run, total);
-  if (u >= u_end) return;
-  int seq = sm.find.seq;
-  long long seq_at = sm.find.at;  // units before the sequence
-  KvSeq s = kv_seq(a.b, seq);
-
-  while (u < u_end) {
-    // the piece of the run inside one (sequence, row block, head)
-    long long n = kv_seq_units(a, s);
-    while (u >= seq_at + n) {
-      seq_at += n;
-      s = kv_seq(a.b, ++seq);
-      n = kv_seq_units(a, s);
+      [&](long long n, int) { return static_cast<long long>(me) * kv_run(n, a.runs); });
+  const long long run = kv_run(total, a.runs);
+  if (tid == 0) *reinterpret_cast<int4*>(a.rec + 4 * static_cast<int64_t>(me)) = make_int4(-1, 0, 0, 0);
+  if (me * run >= total) return;
+  if (warp == 0) {
+    if (lane == 0) {
+      run_state->u = me * run;
+      run_state->u_end = min(run_state->u + run, total);
+      run_state->at = sm.find.at[0];
+      KvPiece& p = run_state->piece[3];
+      p.seq = sm.find.seq[0];
+      p.s = kv_seq(a.b, p.seq);
+      run_state->cost = kv_seq_cost(a, p.s);
     }
-    const KvRange range = kv_units(s, a.window);
-    const int per = range.hi - range.lo;
-    const int idx = static_cast<int>((u - seq_at) / per);   // row block * hkv + head
-    const int first = static_cast<int>((u - seq_at) - static_cast<long long>(idx) * per);
-    const int count = static_cast<int>(min(static_cast<long long>(per - first), u_end - u));
-    const int rb = idx / a.c.hkv, head = idx - rb * a.c.hkv;
+    __syncwarp();
+    kv_next_piece(a, run_state, &run_state->piece[3], &run_state->piece[0], lane);
+    kv_next_piece(a, run_state, &run_state->piece[0], &run_state->piece[1], lane);
+  }
+  __syncthreads();
 
-    QTile<D, NT, T> q;
-    q.load(a, s, rb, head, g, t, a.scale2 * V8::kScale);
-    // keys that rows 2t, 2t + 1 of each n-tile see: [from, to)
-    int to[NT][2], from[NT][2], to_min = s.kv, from_max = 0;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int r = rb * a.rows_per_block + nt * 8 + 2 * t + c;
-        const int j = min(r / a.group, s.q - 1);
-        to[nt][c] = max(s.kv - s.q + j + 1, 0);
-        from[nt][c] = a.window > 0 ? max(to[nt][c] - a.window, 0) : 0;
-        to_min = min(to_min, to[nt][c]);
-        from_max = max(from_max, from[nt][c]);
+  KTile<D> k;
+  VTile<D> v;
+  float ks = 0.f, vs = 0.f;          // scales of the tile in k and v; vs < 0: a bad page, nothing is loaded
+  KvPlace place;                     // lane l: of this warp's tile base + l of the piece that is loaded from
+  int issued = 0, tiles = 0;         // of that piece, this warp's
+  bool there = false;                // the first tile of the present piece is loaded
+  for (int number = 0;; ++number) {
+    const KvPiece* const cur = &run_state->piece[number & 3];
+    const KvPiece* const pro = &run_state->piece[(number + 1) & 3];
+    if (cur->count == 0) return;
+    if (!there) {
+      tiles = max((cur->tiles - warp + kAttendWarps - 1) / kAttendWarps, 0);
+      issued = 0;
+      if (tiles > 0) {
+        place = kv_places(a, cur, 0, warp, lane);
+        const int tile = __shfl_sync(0xffffffffu, place.tile, 0);
+        ks = __shfl_sync(0xffffffffu, place.ks, 0);
+        vs = __shfl_sync(0xffffffffu, place.vs, 0);
+        issued = 1;
+        if (tile >= 0) {
+          k.load(a.c.k + static_cast<int64_t>(tile) * (kAttendTile * D), g, t);
+          v.load(a.c.v + static_cast<int64_t>(tile) * (kAttendTile * D), g, t);
+        }
       }
+    }
+    bool ahead = false;  // loads have gone over to `pro`
+    // piece number + 2 goes where number - 2 was, which nobody reads any more
+    if (warp == (number & 3)) kv_next_piece(a, run_state, pro, &run_state->piece[(number + 2) & 3], lane);
+    QTile<D, NT, T> q;
+    int2* const see = run_state->see[number & 1];
+    int inside_lo, inside_hi, key, left;  // keys that every row sees; the tile's first key; this warp's tiles left
+    float* scores = nullptr;
+    {
+      const KvSeq s = cur->s;
+      const int rb = cur->idx / a.c.hkv, head = cur->idx - rb * a.c.hkv;
+      q.load(a, s, rb, head, g, t, a.scale2 * V8::kScale);
+      const int j = min((rb * a.rows_per_block + min(lane, 8 * NT - 1)) / a.group, s.q - 1);
+      const int to = max(s.kv - s.q + j + 1, 0), from = a.window > 0 ? max(to - a.window, 0) : 0;
+      see[lane] = make_int2(from, to);  // every warp writes the same
+      inside_hi = to, inside_lo = from;
 #pragma unroll
-    for (int d = 1; d < 4; d <<= 1) {
-      to_min = min(to_min, __shfl_xor_sync(0xffffffffu, to_min, d));
-      from_max = max(from_max, __shfl_xor_sync(0xffffffffu, from_max, d));
+      for (int d = 1; d < 32; d <<= 1) {
+        inside_hi = min(inside_hi, __shfl_xor_sync(0xffffffffu, inside_hi, d));
+        inside_lo = max(inside_lo, __shfl_xor_sync(0xffffffffu, inside_lo, d));
+      }
+      key = (cur->lo + cur->first + warp) * kAttendTile;
+      left = tiles;
+      if (a.scores != nullptr) scores = a.scores + (cur->unit + cur->first + warp) * (a.part_rows * kAttendTile);
+      __syncwarp();
     }
 
     AttendState<D, NT> st;
@@ -356,58 +473,45 @@ __global__ void __launch_bounds__(kAttendThreads, NT == 1 && D <= 128 ? 4 : 2) k
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) st.o[nt][i][0] = st.o[nt][i][1] = st.o[nt][i][2] = st.o[nt][i][3] = 0.f;
-      st.m[nt][0] = st.m[nt][1] = kNegInf;
+      st.m[nt][0] = st.m[nt][1] = kNoMax;
       st.l[nt][0] = st.l[nt][1] = 0.f;
     }
     st.ref = 0.f;
+    float w_scale = 0.f;  // kPRange / ref
 
-    // this warp's tiles: 16 keys from key0 + 64 i on; lane l knows page and scales of tile base + l
-    const int key0 = (range.lo + first) * kAttendUnit + 16 * warp;
-    const int tiles = key0 < s.kv ? min(count, (s.kv - key0 + kAttendUnit - 1) / kAttendUnit) : 0;
-    const int in_page = (1 << a.c.shift) - 1;
-    int64_t off_l = -1;
-    float ks_l = 0.f, vs_l = 0.f;
-    auto fetch = [&](int base) {
-      off_l = -1;
-      if (base + lane < tiles) {
-        const int key = key0 + (base + lane) * kAttendUnit;
-        const int64_t p = kv_page(a.c, a.b, seq, key);
-        if (p >= 0) {
-          const int64_t ph = p * a.c.hkv + head;
-          off_l = ((ph << a.c.shift) + (key & in_page)) * D;
-          ks_l = a.c.ks[ph];
-          vs_l = a.c.vs[ph];
-        } else {
-          set_status(a.b.status, SLORA_STATUS_BAD_TABLE);
-        }
+    for (; left > 0; --left, key += kAttendTile * kAttendWarps) {
+      if (issued == tiles && !ahead) {
+        ahead = true;
+        tiles = max((pro->tiles - warp + kAttendWarps - 1) / kAttendWarps, 0);
+        issued = 0;
+        if (tiles > 0) place = kv_places(a, pro, 0, warp, lane);
       }
-    };
-    fetch(0);
-    int64_t off = __shfl_sync(0xffffffffu, off_l, 0);
-    KTile<D> k;
-    VTile<D> v;
-    if (off >= 0) {
-      k.load(a.c.k + off, g, t);
-      v.load(a.c.v + off, g, t);
-    }
-    for (int i = 0; i < tiles; ++i) {
-      const float ks = __shfl_sync(0xffffffffu, ks_l, i & 31);
-      const float vs = __shfl_sync(0xffffffffu, vs_l, i & 31);
-      if (((i + 1) & 31) == 0) fetch(i + 1);
-      const int64_t next = i + 1 < tiles ? __shfl_sync(0xffffffffu, off_l, (i + 1) & 31) : -1;
-      const bool here = off >= 0;  // the same in all lanes
-      off = next;
-      if (!here) {
+      int next = -1;
+      float ks_n = 0.f, vs_n = -1.f;
+      if (issued < tiles) {
+        if (issued > 0 && (issued & 31) == 0) place = kv_places(a, ahead ? pro : cur, issued, warp, lane);
+        next = __shfl_sync(0xffffffffu, place.tile, issued & 31);
+        ks_n = __shfl_sync(0xffffffffu, place.ks, issued & 31);
+        vs_n = __shfl_sync(0xffffffffu, place.vs, issued & 31);
+        ++issued;
+      }
+      const int64_t off = static_cast<int64_t>(next) * (kAttendTile * D);
+      if (vs < 0.f) {  // a bad page: no key of it counts
         if (next >= 0) {
-          k.load(a.c.k + next, g, t);
-          v.load(a.c.v + next, g, t);
+          k.load(a.c.k + off, g, t);
+          v.load(a.c.v + off, g, t);
+        }
+        ks = ks_n;
+        vs = vs_n;
+        if (scores != nullptr) {
+          for (int x = lane; x < a.part_rows * kAttendTile; x += 32) scores[x] = kNegInf;
+          scores += kAttendWarps * a.part_rows * kAttendTile;
         }
         continue;
       }
       float c[NT][4];
       kv_scores<D, NT, KIND>(c, k, q.w);
-      if (next >= 0) k.load(a.c.k + next, g, t);
-      const int key = key0 + i * kAttendUnit;
+      if (next >= 0) k.load(a.c.k + off, g, t);
       bool raise = vs > st.ref;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -417,14 +521,25 @@ __global__ void __launch_bounds__(kAttendThreads, NT == 1 && D <= 128 ? 4 : 2) k
         c[nt][2] *= f0;
         c[nt][3] *= f1;
       }
-      if (key < from_max || key + 16 > to_min) {
+      if (key < inside_lo || key + kAttendTile > inside_hi) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int pos = key + g + 8 * (e >> 1);
-            if (pos < from[nt][e & 1] || pos >= to[nt][e & 1]) c[nt][e] = kNegInf;
+            const int2 sees = see[nt * 8 + 2 * t + (e & 1)];
+            if (pos < sees.x || pos >= sees.y) c[nt][e] = kNegInf;
           }
+      }
+      if (scores != nullptr) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = nt * 8 + 2 * t + (e & 1);
+            if (r < a.part_rows) scores[r * kAttendTile + g + 8 * (e >> 1)] = c[nt][e];
+          }
+        scores += kAttendWarps * a.part_rows * kAttendTile;
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -435,6 +550,7 @@ __global__ void __launch_bounds__(kAttendThreads, NT == 1 && D <= 128 ? 4 : 2) k
           const float now = __uint_as_float(min(max((__float_as_uint(vs) >> 23) + 1u, 27u), 254u) << 23);  // above vs
           up = st.ref > 0.f ? st.ref / now : 0.f;
           st.ref = now;
+          w_scale = kPRange / now;
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -444,7 +560,7 @@ __global__ void __launch_bounds__(kAttendThreads, NT == 1 && D <= 128 ? 4 : 2) k
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
             const float m = fmaxf(st.m[nt][x], top);
-            const float f = m == kNegInf ? 1.f : ex2(st.m[nt][x] - m);
+            const float f = ex2(st.m[nt][x] - m);
             st.m[nt][x] = m;
             st.l[nt][x] *= f;
 #pragma unroll
@@ -454,16 +570,16 @@ __global__ void __launch_bounds__(kAttendThreads, NT == 1 && D <= 128 ? 4 : 2) k
             }
           }
       }
-      const float w = st.ref > 0.f ? vs * (kPRange / st.ref) : 0.f;
+      const float pv = vs * w_scale;
       uint32_t p[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const float m0 = st.m[nt][0] == kNegInf ? 0.f : st.m[nt][0], m1 = st.m[nt][1] == kNegInf ? 0.f : st.m[nt][1];
-        const float e0 = ex2(c[nt][0] - m0), e1 = ex2(c[nt][1] - m1), e2 = ex2(c[nt][2] - m0), e3 = ex2(c[nt][3] - m1);
+        const float e0 = ex2(c[nt][0] - st.m[nt][0]), e1 = ex2(c[nt][1] - st.m[nt][1]);
+        const float e2 = ex2(c[nt][2] - st.m[nt][0]), e3 = ex2(c[nt][3] - st.m[nt][1]);
         st.l[nt][0] += e0 + e2;
         st.l[nt][1] += e1 + e3;
-        p[nt][0] = transpose8x8(pack_f16(e0 * w, e1 * w));
-        p[nt][1] = transpose8x8(pack_f16(e2 * w, e3 * w));
+        p[nt][0] = transpose8x8(pack_f16(e0 * pv, e1 * pv));
+        p[nt][1] = transpose8x8(pack_f16(e2 * pv, e3 * pv));
       }
 #pragma unroll
       for (int x = 0; x < VTile<D>::N; ++x) {
@@ -479,161 +595,282 @@ __global__ void __launch_bounds__(kAttendThreads, NT == 1 && D <= 128 ? 4 : 2) k
           mma_f16(st.o[nt][2 * x + 1], b0, b1, b2, b3, p[nt][0], p[nt][1]);
         }
       }
-      if (next >= 0) v.load(a.c.v + next, g, t);
+      if (next >= 0) v.load(a.c.v + off, g, t);
+      ks = ks_n;
+      vs = vs_n;
     }
 
-    // join the warps: every warp leaves its sums, then each thread adds a quarter of the words over the warps
+    // The piece's sums: every warp leaves its own, then each thread adds eight words (four elements of two rows) at a time
+    // over the warps; to the output when the piece is whole, else to the workspace.  Two buffers take turns: one barrier.
+    auto& home = sm.join[number & 1];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
+        float l = st.l[nt][x];
 #pragma unroll
-        for (int d = 4; d < 32; d <<= 1) st.l[nt][x] += __shfl_xor_sync(0xffffffffu, st.l[nt][x], d);
-        if (g == 0) {
-          sm.m[warp][8 * nt + 2 * t + x] = st.m[nt][x];
-          sm.l[warp][8 * nt + 2 * t + x] = st.l[nt][x];
-        }
+        for (int d = 4; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+        if (g == 0) home.ml[warp][8 * nt + 2 * t + x] = make_float2(st.m[nt][x], l);
       }
-    if (lane == 0) sm.ref[warp] = st.ref * (V8::kScale / kPRange);
+    if (lane == 0) home.ref[warp] = st.ref * (V8::kScale / kPRange);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int mt = 0; mt < D / 16; ++mt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sm.o[warp][(nt * (D / 16) + mt) * 4 + e][lane] = st.o[nt][mt][e];
+        for (int e = 0; e < 4; ++e) home.o[warp][(nt * (D / 16) + mt) * 4 + e][lane] = st.o[nt][mt][e];
     __syncthreads();
-    const bool whole = count == per;
-    const int slot = whole ? -1 : static_cast<int>(2 * me) + (u == me * run ? 0 : 1);
-    float* part = whole ? nullptr : a.part + static_cast<int64_t>(slot) * Ty::kPartWords;
+    {
+      const KvSeq s = cur->s;
+      const int rb = cur->idx / a.c.hkv, head = cur->idx - rb * a.c.hkv;
+      const bool whole = cur->count == cur->per;
+      const int slot = 2 * me + (cur->first > 0 ? 0 : 1);
+      float* part = a.part + static_cast<int64_t>(slot) * a.part_rows * (D + 4);
+      for (int x = warp; x < NT * D / 32; x += kAttendWarps) {
+        // words [8 x, 8 x + 8) are m-tiles 2i, 2i + 1 of n-tile nt: elements elem(g, i) + 0 .. 3 of rows 2t, 2t + 1
+        const int nt = x / (D / 32), i = x - nt * (D / 32);
 #pragma unroll
-    for (int x = warp; x < Ty::kRegs / 8; x += kAttendWarps) {
-      // words [8 x, 8 x + 8) are m-tiles 2i, 2i + 1 of n-tile nt: elements elem(g, i) + 0 .. 3 of rows 2t, 2t + 1
-      const int nt = x / (D / 32), i = x - nt * (D / 32);
+        for (int c = 0; c < 2; ++c) {
+          const int r = 8 * nt + 2 * t + c, row = rb * a.rows_per_block + r;
+          if (row >= s.q * a.group) continue;
+          float m = kNoMax;
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int r = 8 * nt + 2 * t + c;
-        float m = kNegInf;
+          for (int w = 0; w < kAttendWarps; ++w) m = fmaxf(m, home.ml[w][r].x);
+          float l = 0.f, v4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < kAttendWarps; ++w) m = fmaxf(m, sm.m[w][r]);
-        float l = 0.f, v4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < kAttendWarps; ++w) {
-          const float f = part_factor(sm.m[w][r], sm.l[w][r], m);
-          l += f * sm.l[w][r];
-          const float fo = f * sm.ref[w];
-          if (fo != 0.f) {
-            v4[0] += fo * sm.o[w][8 * x + c][lane];
-            v4[1] += fo * sm.o[w][8 * x + 2 + c][lane];
-            v4[2] += fo * sm.o[w][8 * x + 4 + c][lane];
-            v4[3] += fo * sm.o[w][8 * x + 6 + c][lane];
+          for (int w = 0; w < kAttendWarps; ++w) {
+            const float2 ml = home.ml[w][r];
+            const float f = ex2(ml.x - m);
+            l += f * ml.y;
+            const float fo = f * home.ref[w];
+            v4[0] += fo * home.o[w][8 * x + c][lane];
+            v4[1] += fo * home.o[w][8 * x + 2 + c][lane];
+            v4[2] += fo * home.o[w][8 * x + 4 + c][lane];
+            v4[3] += fo * home.o[w][8 * x + 6 + c][lane];
           }
-        }
-        const int row = rb * a.rows_per_block + r;
-        if (row >= s.q * a.group) continue;
-        const int elem = VTile<D>::elem(g, i);
-        if (whole) {
-          const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+          const int elem = VTile<D>::elem(g, i);
+          if (whole) {
+            const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+            const int j = row / a.group, h = head * a.group + row - j * a.group;
+            const int64_t token = static_cast<int64_t>(s.row) + j;
+            union {
+              uint2 u;
+              T e[4];
+            } y;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v4[e] *= inv;
-          store_row4<D, KIND, T>(a, s, head, row, elem, v4);
-          if (a.lse && i == 0 && g == 0) {
-            const int j = row / a.group;
-            a.lse[(static_cast<int64_t>(s.row) + j) * a.hq + head * a.group + row - j * a.group] =
-                l == 0.f ? kNegInf : (m + log2f(l)) * 0.69314718055994531f;
-          }
-        } else {
-          *reinterpret_cast<float4*>(part + r * D + elem) = make_float4(v4[0], v4[1], v4[2], v4[3]);
-          if (i == 0 && g == 0) {
-            part[Ty::kRows * D + 2 * r] = m;
-            part[Ty::kRows * D + 2 * r + 1] = l;
+            for (int e = 0; e < 4; ++e) y.e[e] = from_f32<T>(v4[e] * inv);
+            *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + token * a.out_stride + h * D + elem) = y.u;
+            if (a.lse && i == 0 && g == 0) a.lse[token * a.hq + h] = l == 0.f ? kNegInf : (m + log2f(l)) * 0.69314718055994531f;
+          } else {
+            *reinterpret_cast<float4*>(part + r * D + elem) = make_float4(v4[0], v4[1], v4[2], v4[3]);
+            if (i == 0 && g == 0) *reinterpret_cast<float2*>(part + a.part_rows * D + 2 * r) = make_float2(m, l);
           }
         }
       }
+      if (!whole && cur->first == 0 && tid == 0) {
+        // the first run of a cut piece names it for the join: the runs after it hold their parts in slot 0
+        const long long end = cur->unit + cur->per;
+        const long long behind = end - 1 - static_cast<long long>(me) * run;
+        const int parts = (behind <= 0xffffffffll ? static_cast<int>(static_cast<uint32_t>(behind) / static_cast<uint32_t>(run)) : static_cast<int>(behind / run)) + 1;
+        *reinterpret_cast<int4*>(a.rec + 4 * static_cast<int64_t>(me)) = make_int4(cur->seq, cur->idx, slot, parts);
+      }
     }
-    if (!whole && first == 0 && tid == 0) {
-      // the first CTA of a cut piece names it for the join: the CTAs after it hold their parts in slot 0
-      const long long end = seq_at + static_cast<long long>(idx + 1) * per;
-      *reinterpret_cast<int4*>(a.rec + 4 * me) =
-          make_int4(seq, idx, slot, static_cast<int>((end - 1) / run - me) + 1);
-    }
-    u += count;
-    __syncthreads();
+    there = ahead && tiles > 0;
   }
 }
 
-// Adds the parts of the (sequence, row block, head) that CTA blockIdx.x of the attention left unfinished, in the order of
-// its keys.  Threads own (row, four elements); kJoinGroups of them share the parts.
+// Adds the parts of the (sequence, row block, head) that a run of the attention left unfinished, in the order of its
+// keys: what each part weighs first (all of them at once), then the sums, whose loads do not wait for one another.
+// 32 lanes share a row, the warps rows and parts.
 constexpr int kJoinThreads = 512;
+constexpr int kJoinParts = 128;  // parts whose weights are held at a time
 template <int D, typename T>
 __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const KvAttendArgs a) {
-  __shared__ float4 sh_o[kJoinThreads];
-  __shared__ float2 sh_ml[kJoinThreads];
+  constexpr int kLanes = D / 4 > 32 ? 32 : D / 4, kVec = D / 4 / kLanes;  // float4 of a lane
+  constexpr int kTeams = kJoinThreads / kLanes;
+  __shared__ float4 sh_o[kJoinThreads * kVec];
+  __shared__ float sh_f[32][kJoinParts];
+  __shared__ float sh_m[32], sh_l[32], sh_keep[32];
+  const int tid = threadIdx.x;
   pdl_launch_dependents();
   pdl_wait();
-  const int4 rec = *reinterpret_cast<const int4*>(a.rec + 4 * static_cast<int64_t>(blockIdx.x));
-  if (rec.x < 0) return;
-  const KvSeq s = kv_seq(a.b, rec.x);
-  const int rb = rec.y / a.c.hkv, head = rec.y - rb * a.c.hkv;
-  const int rows = min(a.rows_per_block, s.q * a.group - rb * a.rows_per_block);
-  const int64_t words = static_cast<int64_t>(a.rows_per_block) * (D + 2);
-  const int per_row = D / 4, at_once = kJoinThreads / per_row;
-  const int groups = rows >= at_once ? 1 : at_once / rows;    // threads that share an output's parts
-  for (int r0 = 0; r0 < rows; r0 += at_once) {
-    const int e = threadIdx.x % per_row, x = threadIdx.x / per_row;
-    const int r = groups == 1 ? r0 + x : x % rows, grp = groups == 1 ? 0 : x / rows;
-    float m = kNegInf, l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (r < rows && grp < groups) {
-      for (int p = grp; p < rec.w; p += groups) {
-        const int slot = p == 0 ? rec.z : 2 * (static_cast<int>(blockIdx.x) + p);
-        const float* part = a.part + slot * words;
-        const float2 ml = *reinterpret_cast<const float2*>(part + static_cast<int64_t>(a.rows_per_block) * D + 2 * r);
-        const float4 v = *reinterpret_cast<const float4*>(part + r * D + 4 * e);
-        const float now = fmaxf(m, ml.x);
-        const float f0 = part_factor(m, l, now), f1 = part_factor(ml.x, ml.y, now);
-        l = l * f0 + ml.y * f1;
-        o.x = o.x * f0 + v.x * f1;
-        o.y = o.y * f0 + v.y * f1;
-        o.z = o.z * f0 + v.z * f1;
-        o.w = o.w * f0 + v.w * f1;
-        m = now;
+  {
+    const int me = blockIdx.x;
+    const int4 rec = *reinterpret_cast<const int4*>(a.rec + 4 * static_cast<int64_t>(me));
+    if (rec.x < 0) return;
+    const KvSeq s = kv_seq(a.b, rec.x);
+    const int rb = rec.y / a.c.hkv, head = rec.y - rb * a.c.hkv;
+    const int rows = min(a.rows_per_block, s.q * a.group - rb * a.rows_per_block);
+    const int64_t words = static_cast<int64_t>(a.part_rows) * (D + 4);
+    auto part_of = [&](int p) { return a.part + (p == 0 ? rec.z : 2 * (me + p)) * words; };
+    const int e = tid % kLanes, team = tid / kLanes;
+    const int groups = max(kTeams / rows, 1);  // teams that share a row's parts
+    const int r_me = team % rows, grp = team / rows;
+    // rows <= 32 and teams >= 8: with more rows than teams a team takes several rows in turn
+    for (int r0 = 0; r0 < rows; r0 += kTeams) {
+      const int r = groups > 1 || kTeams >= rows ? r_me : r0 + team;
+      const bool on = groups > 1 || kTeams >= rows ? grp < groups : r < rows;
+      float4 o[kVec];
+#pragma unroll
+      for (int v = 0; v < kVec; ++v) o[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (tid < 32) {
+        sh_m[tid] = kNoMax;
+        sh_l[tid] = 0.f;
       }
+      for (int p0 = 0; p0 < rec.w; p0 += kJoinParts) {
+        const int np = min(kJoinParts, rec.w - p0);
+        __syncthreads();
+        // one warp per row: the weights of this stretch of parts relative to the maximum so far
+        for (int rr = tid >> 5; rr < rows; rr += kJoinThreads / 32) {
+          float m = kNoMax;
+          float2 ml[kJoinParts / 32];
+#pragma unroll
+          for (int k = 0; k < kJoinParts / 32; ++k) {
+            const int p = k * 32 + (tid & 31);
+            ml[k] = make_float2(kNoMax, 0.f);
+            if (p < np) ml[k] = *reinterpret_cast<const float2*>(part_of(p0 + p) + static_cast<int64_t>(a.part_rows) * D + 2 * rr);
+            m = fmaxf(m, ml[k].x);
+          }
+#pragma unroll
+          for (int d = 1; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+          const float was = sh_m[rr], now = fmaxf(was, m);
+          float l = 0.f;
+#pragma unroll
+          for (int k = 0; k < kJoinParts / 32; ++k) {
+            const float f = ex2(ml[k].x - now);
+            sh_f[rr][k * 32 + (tid & 31)] = f;
+            l += f * ml[k].y;
+          }
+#pragma unroll
+          for (int d = 1; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+          if ((tid & 31) == 0) {
+            const float keep = ex2(was - now);
+            sh_keep[rr] = keep;
+            sh_l[rr] = sh_l[rr] * keep + l;
+            sh_m[rr] = now;
+          }
+          __syncwarp();
+        }
+        __syncthreads();
+        if (on) {
+          const float keep = sh_keep[r];
+#pragma unroll
+          for (int v = 0; v < kVec; ++v) o[v].x *= keep, o[v].y *= keep, o[v].z *= keep, o[v].w *= keep;
+#pragma unroll 8
+          for (int p = grp; p < np; p += groups) {
+            const float f = sh_f[r][p];
+            const float* part = part_of(p0 + p) + r * D;
+#pragma unroll
+            for (int v = 0; v < kVec; ++v) {
+              const float4 y = *reinterpret_cast<const float4*>(part + 4 * (v * kLanes + e));
+              if (f != 0.f) {
+                o[v].x += y.x * f;
+                o[v].y += y.y * f;
+                o[v].z += y.z * f;
+                o[v].w += y.w * f;
+              }
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int v = 0; v < kVec; ++v) sh_o[v * kJoinThreads + tid] = o[v];
+      __syncthreads();
+      if (on && grp == 0) {
+        const float l = sh_l[r];
+        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+        const int row = rb * a.rows_per_block + r, j = row / a.group, h = head * a.group + row - j * a.group;
+        const int64_t token = static_cast<int64_t>(s.row) + j;
+#pragma unroll
+        for (int v = 0; v < kVec; ++v) {
+          for (int k = 1; k < groups; ++k) {
+            const float4 y = sh_o[v * kJoinThreads + tid + k * rows * kLanes];
+            o[v].x += y.x, o[v].y += y.y, o[v].z += y.z, o[v].w += y.w;
+          }
+          union {
+            uint2 u;
+            T e[4];
+          } p;
+          p.e[0] = from_f32<T>(o[v].x * inv);
+          p.e[1] = from_f32<T>(o[v].y * inv);
+          p.e[2] = from_f32<T>(o[v].z * inv);
+          p.e[3] = from_f32<T>(o[v].w * inv);
+          *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + token * a.out_stride + h * D + 4 * (v * kLanes + e)) = p.u;
+        }
+        if (a.lse && e == 0) a.lse[token * a.hq + h] = l == 0.f ? kNegInf : (sh_m[r] + log2f(l)) * 0.69314718055994531f;
+      }
+      __syncthreads();
     }
-    sh_o[threadIdx.x] = o;
-    sh_ml[threadIdx.x] = make_float2(m, l);
-    __syncthreads();
-    if (r < rows && grp == 0) {
-      for (int k = 1; k < groups; ++k) {
-        const int y = threadIdx.x + k * rows * per_row;
-        const float2 ml = sh_ml[y];
-        const float4 v = sh_o[y];
-        const float now = fmaxf(m, ml.x);
-        const float f0 = part_factor(m, l, now), f1 = part_factor(ml.x, ml.y, now);
-        l = l * f0 + ml.y * f1;
-        o.x = o.x * f0 + v.x * f1;
-        o.y = o.y * f0 + v.y * f1;
-        o.z = o.z * f0 + v.z * f1;
-        o.w = o.w * f0 + v.w * f1;
-        m = now;
-      }
-      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-      const float v4[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
-      const int row = rb * a.rows_per_block + r;
-      store_row4<D, 0, T>(a, s, head, row, 4 * e, v4);
-      if (a.lse && e == 0) {
-        const int j = row / a.group;
-        a.lse[(static_cast<int64_t>(s.row) + j) * a.hq + head * a.group + row - j * a.group] =
-            l == 0.f ? kNegInf : (m + log2f(l)) * 0.69314718055994531f;
-      }
-    }
-    __syncthreads();
   }
 }
 
-// Accumulated attention weights: with lse known, the keys' scores once more and their exponentials summed over the rows.
+// Accumulated attention weights from the stored scores: w[key] += sum over the rows of 2^(score - lse).  Runs of tiles as
+// in the attention; a lane takes a key of the tile and half of its rows.
+template <int D>
+__global__ void __launch_bounds__(kAttendThreads) kv_weights_kernel(const KvAttendArgs a) {
+  __shared__ KvFind find;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int me = blockIdx.x * kAttendWarps + warp;
+  const int runs = gridDim.x * kAttendWarps;
+  const long long total = kv_find<kAttendWarps, kAttendWarps>(
+      a.b.n_seq, &find, [&](int i) { return kv_seq_cost(a, kv_seq(a.b, i)); },
+      [&](long long n, int k) { return static_cast<long long>(blockIdx.x * kAttendWarps + k) * kv_run(n, runs); });
+  const long long run = kv_run(total, runs);
+  long long u = me * run;
+  const long long u_end = min(u + run, total);
+  if (u >= u_end) return;
+  int seq = find.seq[warp];
+  long long seq_at = find.at[warp];
+  KvSeq s = kv_seq(a.b, seq);
+  long long cost = kv_seq_cost(a, s);
+  const int key_in = lane & 15, half = lane >> 4;
+  while (u < u_end) {
+    while (u >= seq_at + cost) {
+      seq_at += cost;
+      s = kv_seq(a.b, ++seq);
+      cost = kv_seq_cost(a, s);
+    }
+    const KvRange range = kv_tiles(s, a.window);
+    const int per = range.hi - range.lo, piece = per + kAttendPiece;
+    const long long in = u - seq_at;
+    const int idx = in <= 0xffffffffll ? static_cast<int>(static_cast<uint32_t>(in) / static_cast<uint32_t>(piece)) : static_cast<int>(in / piece);
+    const int at = static_cast<int>(in - static_cast<long long>(idx) * piece);
+    const int until = static_cast<int>(min(static_cast<long long>(piece), at + (u_end - u)));
+    const long long base = u - at + kAttendPiece;  // unit of tile 0
+    u += until - at;
+    const int rb = idx / a.c.hkv, head = idx - rb * a.c.hkv;
+    const int rows = min(a.rows_per_block, s.q * a.group - rb * a.rows_per_block);
+    // lane r holds lse of row r (32 rows at most)
+    float lse_l = kNegInf;
+    if (lane < rows) {
+      const int row = rb * a.rows_per_block + lane, j = row / a.group;
+      lse_l = a.lse[(static_cast<int64_t>(s.row) + j) * a.hq + head * a.group + row - j * a.group] * 1.4426950408889634f;
+    }
+#pragma unroll 4
+    for (int i = max(at - kAttendPiece, 0); i < until - kAttendPiece; ++i) {
+      const int key = (range.lo + i) * kAttendTile;
+      if (key >= s.kv) break;
+      const float* src = a.scores + (base + i) * (a.part_rows * kAttendTile);
+      float sum = 0.f;
+      for (int r0 = 0; r0 < rows; r0 += 2) {
+        const float lse = __shfl_sync(0xffffffffu, lse_l, r0 + half);
+        if (r0 + half < rows && lse > kNegInf) sum += ex2(src[(r0 + half) * kAttendTile + key_in] - lse);
+      }
+      sum += __shfl_down_sync(0xffffffffu, sum, 16);
+      const int64_t p = kv_page(a.c, a.b, seq, key);
+      // an atomic add only because sequences may share a page; a page of one sequence gets one add per token and row block
+      if (p >= 0 && half == 0 && key + key_in < s.kv && sum != 0.f)
+        atomicAdd(a.c.w + ((p * a.c.hkv + head) << a.c.shift) + ((key + key_in) & ((1 << a.c.shift) - 1)), sum);
+    }
+  }
+}
+
+// The same with the scores computed again: where they would take too much memory, or for many rows.
 // Tiles are independent; a warp keeps the keys of a tile in registers and walks through the sequence's rows.
 template <int D, int KIND, typename T>
-__global__ void __launch_bounds__(kAttendThreads, D <= 128 ? 4 : 2) kv_weights_kernel(const KvAttendArgs a) {
+__global__ void __launch_bounds__(kAttendThreads, D <= 128 ? 4 : 2) kv_reweigh_kernel(const KvAttendArgs a) {
   using V8 = Kv8<KIND>;
   __shared__ KvFind find;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -643,16 +880,16 @@ __global__ void __launch_bounds__(kAttendThreads, D <= 128 ? 4 : 2) kv_weights_k
   auto units = [&](int i) {
     const KvSeq s = kv_seq(a.b, i);
     if (s.q == 0) return 0ll;
-    const KvRange r = kv_units(s, a.window);
-    return static_cast<long long>(r.hi - r.lo) * a.c.hkv;
+    const KvRange r = kv_tiles(s, a.window);
+    return static_cast<long long>((r.hi - r.lo + kAttendWarps - 1) / kAttendWarps) * a.c.hkv;
   };
-  const long long total = kv_find<kAttendWarps>(a.b.n_seq, &find, units, [&](long long n) { return me * ((n + grid - 1) / grid); });
+  const long long total = kv_find<kAttendWarps, 1>(a.b.n_seq, &find, units, [&](long long n, int) { return me * ((n + grid - 1) / grid); });
   const long long run = (total + grid - 1) / grid;
   long long u = me * run;
   const long long u_end = min(u + run, total);
   if (u >= u_end) return;
-  int seq = find.seq;
-  long long seq_at = find.at;
+  int seq = find.seq[0];
+  long long seq_at = find.at[0];
   long long n = units(seq);
   KvSeq s = kv_seq(a.b, seq);
   QTile<D, 1, T> q;
@@ -663,10 +900,10 @@ __global__ void __launch_bounds__(kAttendThreads, D <= 128 ? 4 : 2) kv_weights_k
       n = units(++seq);
       s = kv_seq(a.b, seq);
     }
-    const KvRange range = kv_units(s, a.window);
-    const int per = range.hi - range.lo;
+    const KvRange range = kv_tiles(s, a.window);
+    const int per = (range.hi - range.lo + kAttendWarps - 1) / kAttendWarps;
     const int head = static_cast<int>((u - seq_at) / per);
-    const int key = (range.lo + static_cast<int>((u - seq_at) - static_cast<long long>(head) * per)) * kAttendUnit + 16 * warp;
+    const int key = (range.lo + static_cast<int>((u - seq_at) - static_cast<long long>(head) * per) * kAttendWarps + warp) * kAttendTile;
     if (key >= s.kv) continue;
     const int64_t p = kv_page(a.c, a.b, seq, key);
     if (p < 0) continue;

@@ -14,14 +14,18 @@ using namespace slora;
 
 namespace {
 
-template <typename K, typename A>
-int launch_pdl(K kernel, dim3 grid, int threads, size_t smem, cudaStream_t stream, const A& args, const char* what) {
-  if (smem > 48 * 1024) {
+template <auto kernel, typename... A>
+int launch_pdl(dim3 grid, int threads, size_t smem, cudaStream_t stream, const char* what, const A&... args) {
+  // more than 48 KB of shared memory is opted in to once per kernel, device and size
+  static std::atomic<size_t> opted[64];
+  int dev = 0;
+  if (smem > 48 * 1024 && (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64 || opted[dev].load(std::memory_order_relaxed) < smem)) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) {
       cudaGetLastError();
       return fail(SLORA_ERR_LAUNCH, "%s: %zu bytes of shared memory: %s", what, smem, cudaGetErrorString(e));
     }
+    if (dev >= 0 && dev < 64) opted[dev].store(smem, std::memory_order_relaxed);
   }
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
@@ -34,7 +38,7 @@ int launch_pdl(K kernel, dim3 grid, int threads, size_t smem, cudaStream_t strea
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return fail(SLORA_ERR_LAUNCH, "%s: %s", what, cudaGetErrorString(e));
@@ -75,7 +79,9 @@ int check_cache(const slora_kv8_cache* c, KvCache* out) {
     return fail(SLORA_ERR_SHAPE, "cache: page_tokens=%d (16, 32, 64 or 128)", c->page_tokens);
   if (const int rc = check_head_dim(c->head_dim)) return rc;
   if (c->kv_heads < 1 || c->kv_heads > 65535) return fail(SLORA_ERR_SHAPE, "cache: kv_heads=%d", c->kv_heads);
-  if (c->n_pages < 1 || c->n_pages > (int64_t(1) << 40)) return fail(SLORA_ERR_SHAPE, "cache: n_pages=%lld", (long long)c->n_pages);
+  if (c->n_pages < 1 || c->n_pages > 0x7fffffffLL) return fail(SLORA_ERR_SHAPE, "cache: n_pages=%lld", (long long)c->n_pages);
+  if (((c->n_pages * c->kv_heads) << shift) > 0x7fffffffLL)
+    return fail(SLORA_ERR_SHAPE, "cache: more than 2^31 rows (tokens x heads) in a layer");
   if (!aligned16(c->k) || !aligned16(c->v) || !aligned16(c->k_scale) || !aligned16(c->v_scale) || !aligned16(c->weights))
     return fail(SLORA_ERR_ALIGN, "cache: a buffer is not 16-byte aligned");
   out->k = static_cast<uint8_t*>(c->k);
@@ -145,8 +151,8 @@ int head_splits(int64_t units, int rows) {
 
 template <int D>
 int rotary_d(const RowArgs& a, dim3 grid, size_t smem, int dtype, cudaStream_t s) {
-  return dtype == SLORA_F16 ? launch_pdl(rotary_kernel<D, __half>, grid, kRowThreads, smem, s, a, "rotary")
-                            : launch_pdl(rotary_kernel<D, __nv_bfloat16>, grid, kRowThreads, smem, s, a, "rotary");
+  return dtype == SLORA_F16 ? launch_pdl<rotary_kernel<D, __half>>(grid, kRowThreads, smem, s, "rotary", a)
+                            : launch_pdl<rotary_kernel<D, __nv_bfloat16>>(grid, kRowThreads, smem, s, "rotary", a);
 }
 
 // One instantiation per (head_dim, kind, I/O type).
@@ -184,33 +190,46 @@ int attend_grid(int nt, int d) { return sm_count() * (nt == 1 && d <= 128 ? 4 : 
 // Sequences with at least this many rows go to the tensor-memory kernel (kv_prefill.cuh), the others to kv_attend.cuh.
 constexpr int kPrefillRows = 64;
 
+// The scores that add_weights keeps take 4 bytes per key and row; beyond this many bytes they are computed again.
+constexpr int64_t kMaxScoreBytes = int64_t(1) << 29;
+
 struct AttendLayout {
-  int nt, grid;
+  int nt, grid, part_rows;
   int split;           // q_len from which sequences are the prefill kernel's; above max_q: none
   int64_t pre_grid;    // its items, at most
-  size_t part, rec, lse, total;
+  bool keep_scores;
+  size_t part, rec, lse, scores, total;
 };
 AttendLayout attend_layout(const KvCache& c, const KvBatch& b, int hq, int add_weights) {
   AttendLayout l;
   const int group = hq / c.hkv;
   l.split = c.d <= 128 ? (kPrefillRows + group - 1) / group : 0x7fffffff;
   const bool pre = b.max_q >= l.split;
-  l.nt = attend_tiles(pre ? l.split - 1 : b.max_q, group, c.d);
+  const int most_q = pre ? l.split - 1 : b.max_q;
+  l.nt = attend_tiles(most_q, group, c.d);
+  const int64_t rows = static_cast<int64_t>(most_q) * group;
+  l.part_rows = static_cast<int>(rows < 1 ? 1 : rows < 8 * l.nt ? rows : 8 * l.nt);
   const int64_t seqs = b.n_seq < b.T ? b.n_seq : b.T;
   l.pre_grid = pre ? (b.T * group / kPreRows + seqs) * c.hkv : 0;
   l.grid = attend_grid(l.nt, c.d);
   const auto up = [](size_t x) { return (x + 15) & ~static_cast<size_t>(15); };
+  const size_t runs = static_cast<size_t>(l.grid);
   l.part = 0;
-  l.rec = up(2u * static_cast<size_t>(l.grid) * 8 * l.nt * (c.d + 2) * sizeof(float));
-  l.lse = l.rec + up(static_cast<size_t>(l.grid) * 16);
-  l.total = l.lse + (add_weights ? up(static_cast<size_t>(b.T) * hq * sizeof(float)) : 0);
+  l.rec = up(2u * runs * l.part_rows * (c.d + 4) * sizeof(float));
+  l.lse = l.rec + up(runs * 16);
+  l.scores = l.lse + (add_weights ? up(static_cast<size_t>(b.T) * hq * sizeof(float)) : 0);
+  // cost units of all pieces (see kv_attend.cuh), if every sequence were as long as the page table allows
+  const int64_t blocks = (rows + 8 * l.nt - 1) / (8 * l.nt);
+  const double units = static_cast<double>(b.n_seq) * (static_cast<double>(b.max_tokens / kAttendTile) + 1 + kAttendPiece) * c.hkv * blocks;
+  const double bytes = units * l.part_rows * kAttendTile * sizeof(float);
+  l.keep_scores = add_weights && !pre && bytes <= static_cast<double>(kMaxScoreBytes);
+  l.total = l.scores + (l.keep_scores ? up(static_cast<size_t>(bytes)) : 0);
   return l;
 }
 
 template <int D, int NT, int KIND, typename T>
 int attend_nt(const KvAttendArgs& a, int grid, cudaStream_t s) {
-  using Smem = typename AttendTypes<D, NT, KIND, T>::Smem;
-  return launch_pdl(kv_attend_kernel<D, NT, KIND, T>, dim3(grid), kAttendThreads, sizeof(Smem), s, a, "kv8_attend");
+  return launch_pdl<kv_attend_kernel<D, NT, KIND, T>>(dim3(grid), kAttendThreads, sizeof(AttendSmem<D, NT>), s, "kv8_attend", a);
 }
 template <int D, int KIND, typename T>
 int attend_launch(KvAttendArgs a, const AttendLayout& l, int add_weights, cudaStream_t s) {
@@ -228,15 +247,15 @@ int attend_launch(KvAttendArgs a, const AttendLayout& l, int add_weights, cudaSt
       KvAttendArgs p = a;
       p.min_q = l.split;
       p.lim_q = a.b.max_q;
-      rc = launch_pdl(kv_prefill_kernel<D, KIND, T>, dim3(static_cast<unsigned>(l.pre_grid)), kPreThreads, sizeof(PreSmem<D>) + 1024, s, p,
-                      "kv8_attend prefill");
+      rc = launch_pdl<kv_prefill_kernel<D, KIND, T>>(dim3(static_cast<unsigned>(l.pre_grid)), kPreThreads, sizeof(PreSmem<D>) + 1024, s, "kv8_attend prefill", p);
       if (rc) return rc;
     }
   }
-  rc = launch_pdl(kv_join_kernel<D, T>, dim3(l.grid), kJoinThreads, 0, s, a, "kv8_attend join");
+  rc = launch_pdl<kv_join_kernel<D, T>>(dim3(l.grid), kJoinThreads, 0, s, "kv8_attend join", a);
   if (rc || !add_weights) return rc;
+  if (l.keep_scores) return launch_pdl<kv_weights_kernel<D>>(dim3(8 * sm_count()), kAttendThreads, 0, s, "kv8_attend weights", a);
   a.rows_per_block = 8;
-  return launch_pdl(kv_weights_kernel<D, KIND, T>, dim3(attend_grid(1, D)), kAttendThreads, 0, s, a, "kv8_attend weights");
+  return launch_pdl<kv_reweigh_kernel<D, KIND, T>>(dim3(attend_grid(1, D)), kAttendThreads, 0, s, "kv8_attend weights", a);
 }
 
 int check_attend(const slora_kv8_cache* cache, const slora_kv8_batch* batch, int64_t T, int q_heads, int add_weights,
@@ -253,15 +272,15 @@ int check_attend(const slora_kv8_cache* cache, const slora_kv8_batch* batch, int
 
 template <int D, int KIND, typename T>
 int append_launch(const AppendArgs& a, dim3 grid, size_t smem, cudaStream_t s) {
-  return launch_pdl(kv_append_kernel<D, KIND, T>, grid, kRowThreads, smem, s, a, "kv8_append");
+  return launch_pdl<kv_append_kernel<D, KIND, T>>(grid, kRowThreads, smem, s, "kv8_append", a);
 }
 template <int D, int KIND, typename T>
 int read_launch(const ReadArgs& a, int grid, cudaStream_t s) {
-  return launch_pdl(kv_read_kernel<D, KIND, T>, dim3(grid), kRowThreads, 0, s, a, "kv8_read");
+  return launch_pdl<kv_read_kernel<D, KIND, T>>(dim3(grid), kRowThreads, 0, s, "kv8_read", a);
 }
 template <int D, int KIND, typename T>
 int move_launch(const EvictArgs& a, dim3 grid, cudaStream_t s) {
-  return launch_pdl(kv_move_kernel<D, KIND>, grid, kMoveThreads, 0, s, a, "kv8_evict move");
+  return launch_pdl<kv_move_kernel<D, KIND>>(grid, kMoveThreads, 0, s, "kv8_evict move", a);
 }
 
 }  // namespace
@@ -413,6 +432,9 @@ int slora_kv8_attend(const slora_kv8_cache* cache, const slora_kv8_batch* batch,
   a.window = window;
   a.min_q = 0;
   a.lim_q = l.split - 1;
+  a.part_rows = l.part_rows;
+  a.runs = l.grid;
+  a.scores = l.keep_scores ? reinterpret_cast<float*>(ws + l.scores) : nullptr;
   a.part = reinterpret_cast<float*>(ws + l.part);
   a.rec = reinterpret_cast<int*>(ws + l.rec);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -445,8 +467,8 @@ int slora_kv8_evict(const slora_kv8_cache* cache, const slora_kv8_batch* batch, 
   // 12288 weights in shared memory (48 KB) leave two CTAs per SM; longer rests are read again in each pass
   a.cached = static_cast<int>(a.b.max_tokens < 40960 ? a.b.max_tokens : 40960);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (int rc = launch_pdl(kv_select_kernel, dim3(static_cast<unsigned>(heads)), kSelectThreads,
-                          static_cast<size_t>(a.cached) * sizeof(uint32_t), s, a, "kv8_evict select"))
+  if (int rc = launch_pdl<kv_select_kernel>(dim3(static_cast<unsigned>(heads)), kSelectThreads,
+                          static_cast<size_t>(a.cached) * sizeof(uint32_t), s, "kv8_evict select", a))
     return rc;
   const int64_t rounds = (2 * ((longest + (1 << a.c.shift) - 1) >> a.c.shift) * ((1 << a.c.shift) / 16) + kMoveWarps - 1) / kMoveWarps;
   int64_t chunks = a.in_place ? 1 : (16ll * sm_count() + heads - 1) / heads;

@@ -101,15 +101,15 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_kernel(const KvAtte
   pdl_launch_dependents();
   pdl_wait();
   const long long item = blockIdx.x;
-  const long long total = kv_find<kPreThreads / 32>(
-      a.b.n_seq, &sm.find, [&](int i) { return pre_items(a, kv_seq(a.b, i)); }, [&](long long) { return item; });
+  const long long total = kv_find<kPreThreads / 32, 1>(
+      a.b.n_seq, &sm.find, [&](int i) { return pre_items(a, kv_seq(a.b, i)); }, [&](long long, int) { return item; });
   // the grid holds every item unless sequences share rows
   if (total > static_cast<long long>(gridDim.x) && item == 0 && tid == 0) set_status(a.b.status, SLORA_STATUS_BAD_TABLE);
   if (item >= total) return;
-  const int seq = sm.find.seq;
+  const int seq = sm.find.seq[0];
   const KvSeq s = kv_seq(a.b, seq);
   const int rows = s.q * a.group, blocks = (rows + kPreRows - 1) / kPreRows;
-  const int idx = static_cast<int>(item - sm.find.at);
+  const int idx = static_cast<int>(item - sm.find.at[0]);
   const int head = idx % a.c.hkv, row0 = (blocks - 1 - idx / a.c.hkv) * kPreRows;
   // keys that the CTA's rows see: [key0, key_end), in steps of 128
   const int last_row = min(row0 + kPreRows, rows) - 1;
