@@ -346,27 +346,17 @@ __device__ __noinline__ void kv_next_piece(const KvAttendArgs& a, KvRun* run, co
   __syncwarp();
 }
 
-// Place (tile of the cache, -1: a bad page) and scales of this warp's tile base + lane of a piece.
-struct KvPlace {
-  int tile;
-  float ks, vs;
-};
-__device__ __noinline__ KvPlace kv_places(const KvAttendArgs& a, const KvPiece* piece, int base, int warp, int lane) {
-  KvPlace r = {-1, 0.f, -1.f};
+// Place in the cache (-1: a bad page) of this warp's tile base + lane of a piece.
+__device__ __noinline__ int kv_places(const KvAttendArgs& a, const KvPiece* piece, int base, int warp, int lane) {
   const int tile = warp + (base + lane) * kAttendWarps;
-  if (tile < piece->tiles) {
-    const int key = (piece->lo + piece->first + tile) * kAttendTile, head = piece->idx % a.c.hkv;
-    const int64_t p = kv_page(a.c, a.b, piece->seq, key);
-    if (p >= 0) {
-      const int64_t ph = p * a.c.hkv + head;
-      r.tile = static_cast<int>((ph << (a.c.shift - 4)) + ((key & ((1 << a.c.shift) - 1)) >> 4));
-      r.ks = a.c.ks[ph];
-      r.vs = a.c.vs[ph];
-    } else {
-      set_status(a.b.status, SLORA_STATUS_BAD_TABLE);
-    }
+  if (tile >= piece->tiles) return -1;
+  const int key = (piece->lo + piece->first + tile) * kAttendTile, head = piece->idx % a.c.hkv;
+  const int64_t p = kv_page(a.c, a.b, piece->seq, key);
+  if (p < 0) {
+    set_status(a.b.status, SLORA_STATUS_BAD_TABLE);
+    return -1;
   }
-  return r;
+  return static_cast<int>(((p * a.c.hkv + head) << (a.c.shift - 4)) + ((key & ((1 << a.c.shift) - 1)) >> 4));
 }
 
 template <int D, int NT>
@@ -413,14 +403,21 @@ __global__ void __launch_bounds__(kAttendThreads, NT == 1 && D <= 128 ? 4 : 2) k
     }
     __syncwarp();
     kv_next_piece(a, run_state, &run_state->piece[3], &run_state->piece[0], lane);
-    kv_next_piece(a, run_state, &run_state->piece[0], &run_state->piece[1], lane);
   }
   __syncthreads();
 
   KTile<D> k;
   VTile<D> v;
   float ks = 0.f, vs = 0.f;          // scales of the tile in k and v; vs < 0: a bad page, nothing is loaded
-  KvPlace place;                     // lane l: of this warp's tile base + l of the piece that is loaded from
+  int place = -1;                    // lane l: of this warp's tile base + l of the piece that is loaded from, and its scales
+  float ks_l = 0.f, vs_l = -1.f;
+  auto scales = [&]() {
+    vs_l = -1.f;
+    if (place >= 0) {
+      ks_l = a.c.ks[place >> (a.c.shift - 4)];
+      vs_l = a.c.vs[place >> (a.c.shift - 4)];
+    }
+  };
   int issued = 0, tiles = 0;         // of that piece, this warp's
   bool there = false;                // the first tile of the present piece is loaded
   for (int number = 0;; ++number) {
@@ -432,19 +429,16 @@ __global__ void __launch_bounds__(kAttendThreads, NT == 1 && D <= 128 ? 4 : 2) k
       issued = 0;
       if (tiles > 0) {
         place = kv_places(a, cur, 0, warp, lane);
-        const int tile = __shfl_sync(0xffffffffu, place.tile, 0);
-        ks = __shfl_sync(0xffffffffu, place.ks, 0);
-        vs = __shfl_sync(0xffffffffu, place.vs, 0);
+        const int tile = __shfl_sync(0xffffffffu, place, 0);
         issued = 1;
         if (tile >= 0) {
           k.load(a.c.k + static_cast<int64_t>(tile) * (kAttendTile * D), g, t);
           v.load(a.c.v + static_cast<int64_t>(tile) * (kAttendTile * D), g, t);
         }
+        scales();
       }
     }
     bool ahead = false;  // loads have gone over to `pro`
-    // piece number + 2 goes where number - 2 was, which nobody reads any more
-    if (warp == (number & 3)) kv_next_piece(a, run_state, pro, &run_state->piece[(number + 2) & 3], lane);
     QTile<D, NT, T> q;
     int2* const see = run_state->see[number & 1];
     int inside_lo, inside_hi, key, left;  // keys that every row sees; the tile's first key; this warp's tiles left
@@ -465,8 +459,22 @@ __global__ void __launch_bounds__(kAttendThreads, NT == 1 && D <= 128 ? 4 : 2) k
       key = (cur->lo + cur->first + warp) * kAttendTile;
       left = tiles;
       if (a.scores != nullptr) scores = a.scores + (cur->unit + cur->first + warp) * (a.part_rows * kAttendTile);
-      __syncwarp();
+      if (!there) {
+        ks = __shfl_sync(0xffffffffu, ks_l, 0);
+        vs = __shfl_sync(0xffffffffu, vs_l, 0);
+      }
     }
+    // the pieces to come, while the loads are on their way: number + 2 goes where number - 2 was, which nobody reads any more
+    if (number == 0) {
+      if (warp == 0) {
+        kv_next_piece(a, run_state, &run_state->piece[0], &run_state->piece[1], lane);
+        kv_next_piece(a, run_state, &run_state->piece[1], &run_state->piece[2], lane);
+      }
+      __syncthreads();
+    } else if (warp == (number & 3)) {
+      kv_next_piece(a, run_state, pro, &run_state->piece[(number + 2) & 3], lane);
+    }
+    __syncwarp();
 
     AttendState<D, NT> st;
 #pragma unroll
@@ -484,15 +492,21 @@ __global__ void __launch_bounds__(kAttendThreads, NT == 1 && D <= 128 ? 4 : 2) k
         ahead = true;
         tiles = max((pro->tiles - warp + kAttendWarps - 1) / kAttendWarps, 0);
         issued = 0;
-        if (tiles > 0) place = kv_places(a, pro, 0, warp, lane);
+        if (tiles > 0) {
+          place = kv_places(a, pro, 0, warp, lane);
+          scales();
+        }
       }
       int next = -1;
       float ks_n = 0.f, vs_n = -1.f;
       if (issued < tiles) {
-        if (issued > 0 && (issued & 31) == 0) place = kv_places(a, ahead ? pro : cur, issued, warp, lane);
-        next = __shfl_sync(0xffffffffu, place.tile, issued & 31);
-        ks_n = __shfl_sync(0xffffffffu, place.ks, issued & 31);
-        vs_n = __shfl_sync(0xffffffffu, place.vs, issued & 31);
+        if (issued > 0 && (issued & 31) == 0) {
+          place = kv_places(a, ahead ? pro : cur, issued, warp, lane);
+          scales();
+        }
+        next = __shfl_sync(0xffffffffu, place, issued & 31);
+        ks_n = __shfl_sync(0xffffffffu, ks_l, issued & 31);
+        vs_n = __shfl_sync(0xffffffffu, vs_l, issued & 31);
         ++issued;
       }
       const int64_t off = static_cast<int64_t>(next) * (kAttendTile * D);
@@ -530,6 +544,13 @@ __global__ void __launch_bounds__(kAttendThreads, NT == 1 && D <= 128 ? 4 : 2) k
             const int2 sees = see[nt * 8 + 2 * t + (e & 1)];
             if (pos < sees.x || pos >= sees.y) c[nt][e] = kNegInf;
           }
+        // what lies behind the sequence's end may be anything, NaN bytes among it: no p of 0 makes that 0
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (key + 2 * t + (j & 1) + 8 * (j >> 1) < cur->s.kv) continue;
+#pragma unroll
+          for (int x = 0; x < VTile<D>::N; ++x) v.w[j][x] = 0;
+        }
       }
       if (scores != nullptr) {
 #pragma unroll

@@ -347,7 +347,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_kernel(const KvAtte
         const int key = p * kPassKeys + key_in;
         const int64_t ph = __shfl_sync(0xffffffffu, page_l, key >> 4);
         regs[p] = make_uint4(0, 0, 0, 0);
-        if (ph >= 0) regs[p] = ld_stream16(base + ((ph << a.c.shift) + ((key0 + i * kPreKeys + key) & in_page)) * D + 16 * sub);
+        // keys behind the sequence's end may hold anything, NaN bytes among it
+        if (ph >= 0 && key0 + i * kPreKeys + key < s.kv) regs[p] = ld_stream16(base + ((ph << a.c.shift) + ((key0 + i * kPreKeys + key) & in_page)) * D + 16 * sub);
       }
     };
     auto put = [&](const uint4 (&regs)[kPer], uint8_t* dst) {
