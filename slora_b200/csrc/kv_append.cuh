@@ -232,29 +232,36 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, const T* src, i
   const float s_new = fmaxf(s_old, __fdiv_rn(top, V8::kTop));
   if (s_new != s_old && n0 > 0) {
     // older values at the new scale: 16 bytes a lane
+    const float mul = __fdiv_rn(s_old, s_new);
+#pragma unroll 2
     for (int i = lane; i < n0 * D / 16; i += 32) {
-      uint4 w = reinterpret_cast<uint4*>(page)[i];
-      uint8_t* b = reinterpret_cast<uint8_t*>(&w);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float q = V8::value(b[e]);
-        const float y = q * s_old;
-        b[e] = static_cast<uint8_t>(kv_round<KIND>(y, __fmaf_rn(q, s_old, -y), s_new));
-      }
-      reinterpret_cast<uint4*>(page)[i] = w;
+      const uint4 w = reinterpret_cast<const uint4*>(page)[i];
+      float q[4];
+      uint4 y;
+      V8::values(w.x, q);
+      y.x = kv_round4<KIND>(q, s_old, mul, s_new);
+      V8::values(w.y, q);
+      y.y = kv_round4<KIND>(q, s_old, mul, s_new);
+      V8::values(w.z, q);
+      y.z = kv_round4<KIND>(q, s_old, mul, s_new);
+      V8::values(w.w, q);
+      y.w = kv_round4<KIND>(q, s_old, mul, s_new);
+      reinterpret_cast<uint4*>(page)[i] = y;
     }
   }
+  const float mul = s_new > 0.f ? __fdiv_rn(1.f, s_new) : 0.f;
+#pragma unroll 2
   for (int base = n0; base < n1; base += kRows) {
     const bool real = load(base);
-    uint32_t w[2] = {0, 0};
+    uint2 w = make_uint2(0, 0);
     if (s_new > 0.f) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        kv_finite(x[e]);
-        w[e >> 2] |= kv_round<KIND>(x[e], 0.f, s_new) << (8 * (e & 3));
-      }
+      for (int e = 0; e < 8; ++e) kv_finite(x[e]);
+      const float lo[4] = {x[0], x[1], x[2], x[3]}, hi[4] = {x[4], x[5], x[6], x[7]};
+      w.x = kv_round4<KIND>(lo, 1.f, mul, s_new);
+      w.y = kv_round4<KIND>(hi, 1.f, mul, s_new);
     }
-    if (real) *reinterpret_cast<uint2*>(page + (base + rr) * D + 8 * sub) = make_uint2(w[0], w[1]);
+    if (real) *reinterpret_cast<uint2*>(page + (base + rr) * D + 8 * sub) = w;
   }
   __syncwarp();
   if (lane == 0) *scale = s_new;
@@ -346,9 +353,13 @@ __global__ void __launch_bounds__(kRowThreads) kv_read_kernel(const ReadArgs a) 
         const uint8_t* src = (w ? a.c.v : a.c.k) + ((ph << a.c.shift) + (pos & ((1 << a.c.shift) - 1))) * D + 8 * sub;
         const uint2 v = *reinterpret_cast<const uint2*>(src);
         const float s = (w ? a.c.vs : a.c.ks)[ph];
-        const uint8_t* b = reinterpret_cast<const uint8_t*>(&v);
+        float q[4];
+        Kv8<KIND>::values(v.x, q);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = Kv8<KIND>::value(b[e]) * s;
+        for (int e = 0; e < 4; ++e) x[e] = q[e] * s;
+        Kv8<KIND>::values(v.y, q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[4 + e] = q[e] * s;
       }
       store8<T>(static_cast<T*>(a.out[w]) + i * D + 8 * sub, x);
     }

@@ -85,7 +85,14 @@ struct Kv8<SLORA_KV_INT8> {
   // f16x2 of bytes 0, 1 / 2, 3 of a prepared word
   __device__ static __forceinline__ uint32_t lo(uint32_t w) { return finish(prmt(w, 0x64646464u, 0x4140)); }
   __device__ static __forceinline__ uint32_t hi(uint32_t w) { return finish(prmt(w, 0x64646464u, 0x4342)); }
-  __device__ static __forceinline__ float value(uint8_t b) { return static_cast<float>(static_cast<int8_t>(b)); }
+  // the four values of a word
+  __device__ static __forceinline__ void values(uint32_t w, float (&v)[4]) {
+    const uint32_t x = w ^ 0x80808080u;  // under the exponent of 2^23: 2^23 + 128 + q, exact
+    v[0] = __uint_as_float(prmt(x, 0x4b000000u, 0x7440)) - 8388736.f;
+    v[1] = __uint_as_float(prmt(x, 0x4b000000u, 0x7441)) - 8388736.f;
+    v[2] = __uint_as_float(prmt(x, 0x4b000000u, 0x7442)) - 8388736.f;
+    v[3] = __uint_as_float(prmt(x, 0x4b000000u, 0x7443)) - 8388736.f;
+  }
 };
 template <>
 struct Kv8<SLORA_KV_E4M3> {
@@ -100,19 +107,20 @@ struct Kv8<SLORA_KV_E4M3> {
   }
   __device__ static __forceinline__ uint32_t lo(uint32_t w) { return pair(w); }
   __device__ static __forceinline__ uint32_t hi(uint32_t w) { return pair(w >> 16); }
-  __device__ static __forceinline__ float value(uint8_t b) {
-    const __half_raw h = {static_cast<unsigned short>(((b & 0x80u) << 8) | ((b & 0x7fu) << 7))};
-    return __half2float(__half(h)) * 256.f;
+  __device__ static __forceinline__ void values(uint32_t w, float (&v)[4]) {
+    const uint32_t a = lo(w), b = hi(w);
+    const float2 x = __half22float2(reinterpret_cast<const __half2&>(a)), y = __half22float2(reinterpret_cast<const __half2&>(b));
+    v[0] = x.x, v[1] = x.y, v[2] = y.x, v[3] = y.y;
   }
 };
 
 // round((x + lo) / s) in the 8-bit type, to nearest, ties to even, of the exact quotient (s > 0; x + lo exact in two FP32
-// words, |lo| <= ulp(x) / 2).  The FP32 quotient is within an ulp or so of the exact one, so it decides everywhere but
-// next to a border between two 8-bit values; there the sign of x + lo - border * s does (fma: one rounding, and the
-// difference is small).  Pages that are scaled anew sit on such borders often: their ratios are small fractions.
-// Returns the stored byte.
+// words, |lo| <= ulp(x) / 2): the stored byte.  The FP32 quotient is within an ulp or so of the exact one, so it decides
+// everywhere but next to a border between two 8-bit values; there the sign of x + lo - border * s does (fma: one
+// rounding, and the difference is small).  Pages that are scaled anew sit on such borders often: their ratios are small
+// fractions.
 template <int KIND>
-__device__ __forceinline__ uint32_t kv_round(float x, float lo, float s) {
+__device__ __noinline__ uint32_t kv_round(float x, float lo, float s) {
   const float y = __fdiv_rn(x, s);
   float m = fabsf(y);
   float step = 1.f, inv = 1.f;
@@ -143,4 +151,44 @@ __device__ __forceinline__ uint32_t kv_round(float x, float lo, float s) {
   return (sign << 7) | (h >> 7);
 }
 
+// The same for four values x[e] = from[e] * by (by: what the values were scaled with; 1 for new ones) at once, packed into
+// a word.  y[e] = from[e] * mul with mul = by / s is, up to roundings, within 2^-22 of the exact quotient; only where that
+// is next to a border kv_round decides (for e4m3 also below 2^-6, where the steps no longer follow the exponent).
+template <int KIND>
+__device__ __forceinline__ uint32_t kv_round4(const float (&from)[4], float by, float mul, float s) {
+  uint32_t w;
+  bool near = !(mul < 1e37f);  // a scale next to FP32's smallest numbers has no inverse
+  if (Kv8<KIND>::kInt) {
+    float t[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float y = fminf(fmaxf(from[e] * mul, -127.f), 127.f);
+      t[e] = y + 12582912.f;  // 1.5 * 2^23: the sum's last bits are y rounded to a whole number
+      near = near || fabsf(y - (t[e] - 12582912.f)) > 0.4999f;
+    }
+    w = prmt(prmt(__float_as_uint(t[0]), __float_as_uint(t[1]), 0x0040), prmt(__float_as_uint(t[2]), __float_as_uint(t[3]), 0x0040), 0x5410);
+  } else {
+    float y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      y[e] = from[e] * mul;
+      const uint32_t b = __float_as_uint(y[e]) & 0x7fffffffu;
+      near = near || (b & 0xfffffu) - 0x7ffe0u < 0x40u || b - 1u < 0x3c800000u - 1u;
+    }
+    unsigned short lo, hi;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(y[1]), "f"(y[0]));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(y[3]), "f"(y[2]));
+    w = lo | static_cast<uint32_t>(hi) << 16;
+  }
+  if (near) {
+    w = 0;
+#pragma unroll 1
+    for (int e = 0; e < 4; ++e) {
+      const float f = e == 0 ? from[0] : e == 1 ? from[1] : e == 2 ? from[2] : from[3];
+      const float x = f * by;
+      w |= kv_round<KIND>(x, __fmaf_rn(f, by, -x), s) << (8 * e);
+    }
+  }
+  return w;
+}
 }  // namespace slora

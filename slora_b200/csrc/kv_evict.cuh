@@ -216,9 +216,13 @@ __global__ void __launch_bounds__(kMoveThreads) kv_move_kernel(const EvictArgs a
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
       float q = 0.f;
-      const uint8_t* b = reinterpret_cast<const uint8_t*>(&w[i]);
+      const uint32_t words[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
 #pragma unroll
-      for (int e = 0; e < 16; ++e) q = fmaxf(q, fabsf(V8::value(b[e])));
+      for (int x = 0; x < 4; ++x) {
+        float v[4];
+        V8::values(words[x], v);
+        q = fmaxf(fmaxf(q, fmaxf(fabsf(v[0]), fabsf(v[1]))), fmaxf(fabsf(v[2]), fabsf(v[3])));
+      }
       top = fmax(top, static_cast<double>(q) * static_cast<double>(s[i]));
     }
 #pragma unroll
@@ -246,13 +250,15 @@ __global__ void __launch_bounds__(kMoveThreads) kv_move_kernel(const EvictArgs a
         for (int i = 0; i < kSteps; ++i) {
           const int slot = part * 16 + i * kRows + rr;
           if (!same) {
-            uint8_t* b = reinterpret_cast<uint8_t*>(&w[i]);
+            const float mul = now > 0.f ? __fdiv_rn(s[i], now) : 0.f;
+            uint32_t words[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float q = V8::value(b[e]);
-              const float y = q * s[i];
-              b[e] = now > 0.f ? static_cast<uint8_t>(kv_round<KIND>(y, __fmaf_rn(q, s[i], -y), now)) : 0;
+            for (int x = 0; x < 4; ++x) {
+              float v[4];
+              V8::values(words[x], v);
+              words[x] = now > 0.f ? kv_round4<KIND>(v, s[i], mul, now) : 0u;
             }
+            w[i] = make_uint4(words[0], words[1], words[2], words[3]);
           }
           if (block * page + slot < m) *reinterpret_cast<uint4*>(dst + slot * D + 16 * sub) = w[i];
         }
