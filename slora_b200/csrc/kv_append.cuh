@@ -7,17 +7,19 @@
 // value sits rot / 16 lanes away (one shuffle per element), in the interleaved layout in the same lane.
 // What bounds it: q, k read and written once (16-bit), at the copy rate; one token: launch and one chain of loads.
 //
-// Append: the new tokens of one page belong to one CTA (the scale of a (page, head) is a maximum over them) and a warp takes
-// a (head, k or v): a first walk over the tokens for the maximum, a second that quantises (its loads come from L1).
-// When the scale grows, the page's older values are rounded to the new one in place.
+// Append: the new tokens of one page belong to one CTA (the scale of a (page, head) is a maximum over them): all warps take
+// a (head, k or v) together when there are many tokens, one warp each when there are few (decode).  When the scale grows,
+// the page's older values are rounded to the new one in place.
 #pragma once
 
 #include "kv_common.cuh"
+#include "lora_mma.cuh"
 
 namespace slora {
 
 constexpr int kRowThreads = 256;
 constexpr int kRowWarps = kRowThreads / 32;
+constexpr int kAppendWarpTokens = 4;  // new tokens of a page up to which a warp takes a (head, k or v) by itself
 
 struct RotaryArgs {
   const int64_t* positions;
@@ -53,44 +55,86 @@ struct AppendArgs {
   int max_units;  // pages a sequence's new tokens touch, at most
 };
 
+__device__ __forceinline__ float2 rotary_pair(const RotaryArgs& r, int64_t token, int pair) {
+  const double a = static_cast<double>(r.positions[token]) * r.turns[pair];
+  float s, c;
+  sincospif(2.f * static_cast<float>(a - rint(a)), &s, &c);
+  return make_float2(c * r.factor, (r.inverse ? -s : s) * r.factor);
+}
 // (cos, sin) of `n` tokens from `t0` on into cs[n][rot / 2].
 __device__ __forceinline__ void rotary_table(const RotaryArgs& r, int64_t t0, int n, float2* cs) {
   const int half = r.rot >> 1;
   for (int i = threadIdx.x; i < n * half; i += blockDim.x) {
-    const int t = i / half, p = i - t * half;
-    const double a = static_cast<double>(r.positions[t0 + t]) * r.turns[p];
-    float s, c;
-    sincospif(2.f * static_cast<float>(a - rint(a)), &s, &c);
-    cs[i] = make_float2(c * r.factor, (r.inverse ? -s : s) * r.factor);
+    const int t = i / half;
+    cs[i] = rotary_pair(r, t0 + t, i - t * half);
   }
+}
+// The same for CTAs of a cluster that work on the same tokens: each works out its share of the angles (150 instructions
+// apiece, what the rows' own work comes to) and stores it into every CTA's shared memory.
+__device__ __forceinline__ void rotary_table_cluster(const RotaryArgs& r, int64_t t0, int n, float2* cs, int size) {
+  const int half = r.rot >> 1, rank = static_cast<int>(cluster_rank());
+  cluster_sync_all();  // every CTA of the cluster runs, and is done with its last table
+  for (int i = rank * blockDim.x + threadIdx.x; i < n * half; i += size * blockDim.x) {
+    const int t = i / half;
+    const float2 v = rotary_pair(r, t0 + t, i - t * half);
+    const uint32_t at = smem_u32(cs + i);
+    for (int k = 0; k < size; ++k)
+      asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(peer_smem(at, k)), "f"(v.x), "f"(v.y) : "memory");
+  }
+  cluster_sync_all();
 }
 
-// Turns the eight elements `x` that this lane holds of a head row (elements 8 sub .. 8 sub + 7; all lanes of the warp take
-// part) by the row's cosines and sines.
-__device__ __forceinline__ void rotary_turn(float (&x)[8], const float2* cs, int sub, int rot, int layout) {
-  if (layout == 0) {
-    const int far = rot >> 4;  // lanes between the partners
-    const bool low = sub < far, in = sub < 2 * far;
+// The cosines and sines that a lane needs for the eight elements 8 sub .. 8 sub + 7 of a head row of one token.
+struct RotaryLane {
+  float2 w[8];
+  int other;      // half layout: lane with the partners
+  int part;       // 0 stays as it is, 1 first of the pairs (or interleaved), 2 second
+  __device__ __forceinline__ void load(const float2* cs, int sub, int rot, int layout) {
     const int lane = threadIdx.x & 31;
-    const int other = low ? lane + far : in ? lane - far : lane;
+    other = lane;
+    part = 0;
+    if (layout == 0) {
+      const int far = rot >> 4;  // lanes between the partners
+      if (sub < 2 * far) {
+        part = sub < far ? 1 : 2;
+        other = part == 1 ? lane + far : lane - far;
+        const float4* p = reinterpret_cast<const float4*>(cs + 8 * (part == 1 ? sub : sub - far));
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float y = __shfl_sync(0xffffffffu, x[e], other);
-      if (in) {
-        const float2 w = cs[8 * (low ? sub : sub - far) + e];
-        x[e] = low ? x[e] * w.x - y * w.y : y * w.y + x[e] * w.x;
+        for (int e = 0; e < 4; ++e) {
+          const float4 v = p[e];
+          w[2 * e] = make_float2(v.x, v.y);
+          w[2 * e + 1] = make_float2(v.z, v.w);
+        }
+      }
+    } else if (8 * sub < rot) {
+      part = 1;
+      const float4* p = reinterpret_cast<const float4*>(cs + 4 * sub);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float4 v = p[e];
+        w[2 * e] = make_float2(v.x, v.y);
+        w[2 * e + 1] = make_float2(v.z, v.w);
       }
     }
-  } else if (8 * sub < rot) {
+  }
+  // all lanes of the warp take part
+  __device__ __forceinline__ void turn(float (&x)[8], int layout) const {
+    if (layout == 0) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 w = cs[4 * sub + e];
-      const float a = x[2 * e], b = x[2 * e + 1];
-      x[2 * e] = a * w.x - b * w.y;
-      x[2 * e + 1] = a * w.y + b * w.x;
+      for (int e = 0; e < 8; ++e) {
+        const float y = __shfl_sync(0xffffffffu, x[e], other);
+        if (part != 0) x[e] = part == 1 ? x[e] * w[e].x - y * w[e].y : y * w[e].y + x[e] * w[e].x;
+      }
+    } else if (part != 0) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float a = x[2 * e], b = x[2 * e + 1];
+        x[2 * e] = a * w[e].x - b * w[e].y;
+        x[2 * e + 1] = a * w[e].y + b * w[e].x;
+      }
     }
   }
-}
+};
 
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
@@ -103,27 +147,40 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
   *reinterpret_cast<uint4*>(p) = v.u;
 }
 
-// Heads [h0, h1) of tokens [t0, t0 + n): turned rows src -> dst.  Rows of a warp's step: 256 / D.
+// Heads [h0, h1) of tokens [t0, t0 + n): turned rows src -> dst.  A warp takes a token and a few heads at a time: the
+// token's cosines stay in registers, and kRowUnroll loads of 512 bytes are in flight.
+constexpr int kRowUnroll = 4;
 template <int D, typename T>
 __device__ __forceinline__ void rotary_rows(const RotaryArgs& r, const T* src, T* dst, int64_t src_stride, int64_t dst_stride,
                                             int64_t t0, int n, int h0, int h1, const float2* cs) {
-  constexpr int kLanes = D / 8, kRows = 32 / kLanes;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % kLanes;
-  const int heads = h1 - h0, rows = n * heads, half = r.rot >> 1;
-  for (int base = warp * kRows; base < rows; base += kRowWarps * kRows) {
-    const int row = base + lane / kLanes;
-    const bool real = row < rows;
-    const int t = real ? row / heads : 0, h = h0 + (real ? row - t * heads : 0);
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (real) cvt8<T>(*reinterpret_cast<const uint4*>(src + (t0 + t) * src_stride + h * D + 8 * sub), x);
-    rotary_turn(x, cs + t * half, sub, r.rot, r.layout);
-    if (real) store8<T>(dst + (t0 + t) * dst_stride + h * D + 8 * sub, x);
+  constexpr int kLanes = D / 8, kRows = 32 / kLanes, kHeads = kRows * kRowUnroll;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % kLanes, rr = lane / kLanes;
+  const int chunks = (h1 - h0 + kHeads - 1) / kHeads, half = r.rot >> 1;
+  for (int item = warp; item < n * chunks; item += kRowWarps) {
+    const int t = item / chunks, h = h0 + (item - t * chunks) * kHeads + rr;
+    const T* from = src + (t0 + t) * src_stride + 8 * sub;
+    T* to = dst + (t0 + t) * dst_stride + 8 * sub;
+    uint4 raw[kRowUnroll];
+#pragma unroll
+    for (int u = 0; u < kRowUnroll; ++u) {
+      raw[u] = make_uint4(0, 0, 0, 0);
+      if (h + u * kRows < h1) raw[u] = *reinterpret_cast<const uint4*>(from + (h + u * kRows) * D);
+    }
+    RotaryLane w;
+    w.load(cs + t * half, sub, r.rot, r.layout);
+#pragma unroll
+    for (int u = 0; u < kRowUnroll; ++u) {
+      float x[8];
+      cvt8<T>(raw[u], x);
+      w.turn(x, r.layout);
+      if (h + u * kRows < h1) store8<T>(to + (h + u * kRows) * D, x);
+    }
   }
 }
 
 template <int D, typename T>
 __global__ void __launch_bounds__(kRowThreads) rotary_kernel(const RowArgs a) {
-  extern __shared__ float2 cs[];
+  extern __shared__ __align__(16) float2 cs[];
   pdl_launch_dependents();
   pdl_wait();
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.tokens_per_cta;
@@ -197,7 +254,100 @@ __device__ __forceinline__ bool kv_finite(float& x) {
   return false;
 }
 
-// One (page, head) of k or v: new tokens in slots [n0, n1) whose rows start at `src`, older ones in slots [0, n0).
+// Older values of a (page, head), `bytes` of them, rounded to a grown scale: 16 bytes a lane.
+template <int KIND>
+__device__ __forceinline__ void append_rescale(uint8_t* page, int bytes, float s_old, float s_new, int id, int step) {
+  using V8 = Kv8<KIND>;
+  const float mul = __fdiv_rn(s_old, s_new);
+#pragma unroll 1
+  for (int i = id; i < bytes / 16; i += step) {
+    const uint4 w = reinterpret_cast<const uint4*>(page)[i];
+    float q[4];
+    uint4 y;
+    V8::values(w.x, q);
+    y.x = kv_round4<KIND>(q, s_old, mul, s_new);
+    V8::values(w.y, q);
+    y.y = kv_round4<KIND>(q, s_old, mul, s_new);
+    V8::values(w.z, q);
+    y.z = kv_round4<KIND>(q, s_old, mul, s_new);
+    V8::values(w.w, q);
+    y.w = kv_round4<KIND>(q, s_old, mul, s_new);
+    reinterpret_cast<uint4*>(page)[i] = y;
+  }
+}
+
+// Eight values at scale s_new, packed.
+template <int KIND>
+__device__ __forceinline__ uint2 append_pack(float (&x)[8], float mul, float s_new) {
+  uint2 w = make_uint2(0, 0);
+  if (s_new > 0.f) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) kv_finite(x[e]);
+    const float lo[4] = {x[0], x[1], x[2], x[3]}, hi[4] = {x[4], x[5], x[6], x[7]};
+    w.x = kv_round4<KIND>(lo, 1.f, mul, s_new);
+    w.y = kv_round4<KIND>(hi, 1.f, mul, s_new);
+  }
+  return w;
+}
+
+// One (page, head) of k or v by the whole CTA, for pages with more than a few new tokens.  The rows are read twice, the
+// second time from L1: kept in registers they left room for one CTA per SM.
+template <int D, int KIND, typename T>
+__device__ __forceinline__ void append_page_cta(const AppendArgs& a, const T* src, int64_t stride, int n0, int n1, uint8_t* page,
+                                                float* scale, const float2* cs, bool turn) {
+  constexpr int kLanes = D / 8, kRows = 32 / kLanes, kPass = kRowWarps * kRows;
+  using V8 = Kv8<KIND>;
+  __shared__ float tops[kRowWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % kLanes, half = a.r.rot >> 1;
+  const int first = n0 + warp * kRows + lane / kLanes, passes = (n1 - n0 + kPass - 1) / kPass;
+  const float s_old = n0 > 0 ? *scale : 0.f;
+  auto row = [&](int p, float (&x)[8]) {
+    const int i = first + p * kPass;
+    uint4 raw = make_uint4(0, 0, 0, 0);
+    if (i < n1) raw = *reinterpret_cast<const uint4*>(src + static_cast<int64_t>(i - n0) * stride + 8 * sub);
+    cvt8<T>(raw, x);
+    if (turn) {
+      RotaryLane w;
+      w.load(cs + (i < n1 ? i - n0 : 0) * half, sub, a.r.rot, a.r.layout);
+      w.turn(x, a.r.layout);
+    }
+  };
+  float top = 0.f;
+  bool fine = true;
+#pragma unroll 1
+  for (int p = 0; p < passes; ++p) {
+    float x[8];
+    row(p, x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const bool ok = kv_finite(x[e]);
+      fine = fine && ok;
+      top = fmaxf(top, ok ? fabsf(x[e]) : 0.f);
+    }
+  }
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+  if (!fine) set_status(a.b.status, kStatusNonfinite);
+  if (lane == 0) tops[warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, tops[w]);
+  const float s_new = fmaxf(s_old, __fdiv_rn(top, V8::kTop));
+  if (s_new != s_old && n0 > 0) append_rescale<KIND>(page, n0 * D, s_old, s_new, threadIdx.x, kRowThreads);
+  const float mul = s_new > 0.f ? __fdiv_rn(1.f, s_new) : 0.f;
+#pragma unroll 1
+  for (int p = 0; p < passes; ++p) {
+    float x[8];
+    row(p, x);
+    const uint2 w = append_pack<KIND>(x, mul, s_new);
+    const int i = first + p * kPass;
+    if (i < n1) *reinterpret_cast<uint2*>(page + i * D + 8 * sub) = w;
+  }
+  __syncthreads();  // every thread has read the old scale and tops
+  if (threadIdx.x == 0) *scale = s_new;
+}
+
+// One (page, head) of k or v by a warp: new tokens in slots [n0, n1) whose rows start at `src`, older ones in slots [0, n0).
 template <int D, int KIND, typename T>
 __device__ __forceinline__ void append_page(const AppendArgs& a, const T* src, int64_t stride, int n0, int n1, uint8_t* page,
                                             float* scale, const float2* cs, bool turn) {
@@ -212,7 +362,11 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, const T* src, i
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = 0.f;
     if (real) cvt8<T>(*reinterpret_cast<const uint4*>(src + static_cast<int64_t>(i - n0) * stride + 8 * sub), x);
-    if (turn) rotary_turn(x, cs + (real ? i - n0 : 0) * half, sub, a.r.rot, a.r.layout);
+    if (turn) {
+      RotaryLane w;
+      w.load(cs + (real ? i - n0 : 0) * half, sub, a.r.rot, a.r.layout);
+      w.turn(x, a.r.layout);
+    }
     return real;
   };
   float top = 0.f;
@@ -230,37 +384,11 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, const T* src, i
   for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
   if (!fine) set_status(a.b.status, kStatusNonfinite);
   const float s_new = fmaxf(s_old, __fdiv_rn(top, V8::kTop));
-  if (s_new != s_old && n0 > 0) {
-    // older values at the new scale: 16 bytes a lane
-    const float mul = __fdiv_rn(s_old, s_new);
-#pragma unroll 2
-    for (int i = lane; i < n0 * D / 16; i += 32) {
-      const uint4 w = reinterpret_cast<const uint4*>(page)[i];
-      float q[4];
-      uint4 y;
-      V8::values(w.x, q);
-      y.x = kv_round4<KIND>(q, s_old, mul, s_new);
-      V8::values(w.y, q);
-      y.y = kv_round4<KIND>(q, s_old, mul, s_new);
-      V8::values(w.z, q);
-      y.z = kv_round4<KIND>(q, s_old, mul, s_new);
-      V8::values(w.w, q);
-      y.w = kv_round4<KIND>(q, s_old, mul, s_new);
-      reinterpret_cast<uint4*>(page)[i] = y;
-    }
-  }
+  if (s_new != s_old && n0 > 0) append_rescale<KIND>(page, n0 * D, s_old, s_new, lane, 32);
   const float mul = s_new > 0.f ? __fdiv_rn(1.f, s_new) : 0.f;
-#pragma unroll 2
   for (int base = n0; base < n1; base += kRows) {
     const bool real = load(base);
-    uint2 w = make_uint2(0, 0);
-    if (s_new > 0.f) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) kv_finite(x[e]);
-      const float lo[4] = {x[0], x[1], x[2], x[3]}, hi[4] = {x[4], x[5], x[6], x[7]};
-      w.x = kv_round4<KIND>(lo, 1.f, mul, s_new);
-      w.y = kv_round4<KIND>(hi, 1.f, mul, s_new);
-    }
+    const uint2 w = append_pack<KIND>(x, mul, s_new);
     if (real) *reinterpret_cast<uint2*>(page + (base + rr) * D + 8 * sub) = w;
   }
   __syncwarp();
@@ -276,9 +404,14 @@ __device__ __forceinline__ void append_unit(const AppendArgs& a, const AppendUni
   // rows of q, k, v; with q_len > kv_len (already reported) the first rows have no place and are left out
   const int64_t row = static_cast<int64_t>(s.row) + (s.q - s.kv) + begin + n0;
   const bool turn = a.r.turns != nullptr;
-  if (turn) rotary_table(a.r, row, n1 - n0, cs);
+  if (turn) {
+    if (a.head_splits > 1 && (n1 - n0) * a.r.rot > 2 * kRowThreads)
+      rotary_table_cluster(a.r, row, n1 - n0, cs, a.head_splits);
+    else
+      rotary_table(a.r, row, n1 - n0, cs);
+  }
   __syncthreads();
-  const int split = blockIdx.y;
+  const int split = blockIdx.y;  // the CTAs of a page are one cluster
   if (turn && a.q != nullptr) {
     const int h0 = static_cast<int>(static_cast<int64_t>(a.hq) * split / a.head_splits);
     const int h1 = static_cast<int>(static_cast<int64_t>(a.hq) * (split + 1) / a.head_splits);
@@ -289,23 +422,31 @@ __device__ __forceinline__ void append_unit(const AppendArgs& a, const AppendUni
     if (threadIdx.x == 0) set_status(a.b.status, SLORA_STATUS_BAD_TABLE);
     return;
   }
-  // (head, k or v) of this CTA's share, one warp each
+  // (head, k or v) of this CTA's share: all warps on one where the page has many new tokens, else one warp each
   const int g0 = static_cast<int>(2ll * a.c.hkv * split / a.head_splits), g1 = static_cast<int>(2ll * a.c.hkv * (split + 1) / a.head_splits);
-  for (int i = g0 + (threadIdx.x >> 5); i < g1; i += kRowWarps) {
+  const bool wide = n1 - n0 > kAppendWarpTokens;
+  for (int i = wide ? g0 : g0 + static_cast<int>(threadIdx.x >> 5); i < g1; i += wide ? 1 : kRowWarps) {
     const int h = i >> 1;
     const int64_t ph = p * a.c.hkv + h;
     uint8_t* bytes = ((i & 1) ? a.c.v : a.c.k) + (ph << a.c.shift) * D;
     const int64_t stride = (i & 1) ? a.v_stride : a.k_stride;
     const T* src = static_cast<const T*>((i & 1) ? a.v : a.k) + row * stride + h * D;
-    append_page<D, KIND, T>(a, src, stride, n0, n1, bytes, ((i & 1) ? a.c.vs : a.c.ks) + ph, cs, turn && !(i & 1));
-    if (a.c.w != nullptr && !(i & 1))
-      for (int x = n0 + (threadIdx.x & 31); x < n1; x += 32) a.c.w[(ph << a.c.shift) + x] = 0.f;
+    float* scale = ((i & 1) ? a.c.vs : a.c.ks) + ph;
+    const bool turned = turn && !(i & 1);
+    if (wide)
+      append_page_cta<D, KIND, T>(a, src, stride, n0, n1, bytes, scale, cs, turned);
+    else
+      append_page<D, KIND, T>(a, src, stride, n0, n1, bytes, scale, cs, turned);
+    if (a.c.w != nullptr && !(i & 1)) {
+      const int id = wide ? threadIdx.x : threadIdx.x & 31, step = wide ? kRowThreads : 32;
+      for (int x = n0 + id; x < n1; x += step) a.c.w[(ph << a.c.shift) + x] = 0.f;
+    }
   }
 }
 
 template <int D, int KIND, typename T>
-__global__ void __launch_bounds__(kRowThreads) kv_append_kernel(const AppendArgs a) {
-  extern __shared__ float2 cs[];
+__global__ void __launch_bounds__(kRowThreads, 3) kv_append_kernel(const AppendArgs a) {
+  extern __shared__ __align__(16) float2 cs[];
   pdl_launch_dependents();
   pdl_wait();
   // the grid holds every unit unless sequences share rows
@@ -331,9 +472,10 @@ __global__ void __launch_bounds__(kRowThreads) kv_read_kernel(const ReadArgs a) 
   const int64_t rows = a.b.n_seq * a.count * a.c.hkv;
   const int64_t step = static_cast<int64_t>(gridDim.x) * kRowWarps * kRows;
   for (int64_t i = (static_cast<int64_t>(blockIdx.x) * kRowWarps + (threadIdx.x >> 5)) * kRows + lane / kLanes; i < rows; i += step) {
-    const int64_t token = i / a.c.hkv;
+    // row -> token, head; token -> sequence (32-bit divisions unless there are more rows than that)
+    const int64_t token = rows <= 0xffffffffll ? static_cast<uint32_t>(i) / static_cast<uint32_t>(a.c.hkv) : i / a.c.hkv;
     const int h = static_cast<int>(i - token * a.c.hkv);
-    const int seq = static_cast<int>(token / a.count);
+    const int seq = static_cast<int>(rows <= 0xffffffffll ? static_cast<uint32_t>(token) / static_cast<uint32_t>(a.count) : token / a.count);
     const int64_t pos = token - seq * a.count + (a.first ? a.first[seq] : 0);
     int kv = a.b.kv_len[seq];
     if (kv < 0 || kv > a.b.max_tokens) {

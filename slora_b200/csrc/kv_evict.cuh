@@ -123,44 +123,56 @@ __global__ void __launch_bounds__(kSelectThreads) kv_select_kernel(const EvictAr
   const int equal = want > 0 ? s_left : 0;  // keys equal to the limit that are kept, the first ones
   int above = 0, ties = 0;                  // kept above the limit / equal to it, before this sweep's positions
   int buf = 0;
-  for (int base = 0; base < n; base += kSelectThreads, buf ^= 1) {
-    const int i = base + tid;
-    bool gt = false, eq = false;
-    if (i < n) {
-      if (i < c0 || i >= c1) {
-        gt = true;
-      } else if (want > 0) {
-        const uint32_t k = key_at(i);
-        gt = k > limit;
-        eq = k == limit;
+  for (int base = 0; base < n; base += 4 * kSelectThreads, buf ^= 1) {
+    const int i = base + 4 * tid;  // four positions a thread
+    unsigned gt = 0, eq = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (i + e < c0 || (i + e >= c1 && i + e < n)) {
+        gt |= 1u << e;
+      } else if (i + e < c1 && want > 0) {
+        const uint32_t k = key_at(i + e);
+        gt |= (k > limit ? 1u : 0u) << e;
+        eq |= (k == limit ? 1u : 0u) << e;
       }
     }
-    const uint32_t mg = __ballot_sync(0xffffffffu, gt), me = __ballot_sync(0xffffffffu, eq);
-    if (lane == 0) s_count[buf][warp] = __popc(mg) | __popc(me) << 16;
+    const int own = __popc(gt) | __popc(eq) << 16;  // at most 4096 of each in a sweep
+    int incl = own;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += y;
+    }
+    if (lane == 31) s_count[buf][warp] = incl;
     __syncthreads();
     int v = s_count[buf][lane];
-    const int own = v;
+    const int mine = v;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, v, d);
       if (lane >= d) v += y;
     }
     const int total = __shfl_sync(0xffffffffu, v, 31);
-    const int before = __shfl_sync(0xffffffffu, v - own, warp);
-    const uint32_t lower = (1u << lane) - 1u;
-    const int g = above + (before & 0xffff) + __popc(mg & lower), e = ties + (before >> 16) + __popc(me & lower);
-    if (gt || (eq && e < equal)) kept[g + min(e, equal)] = i;
+    const int before = __shfl_sync(0xffffffffu, v - mine, warp) + incl - own;
+    int g = above + (before & 0xffff), q = ties + (before >> 16);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const bool is_gt = gt >> e & 1u, is_eq = eq >> e & 1u;
+      if (is_gt || (is_eq && q < equal)) kept[g + min(q, equal)] = i + e;
+      g += is_gt;
+      q += is_eq;
+    }
     above += total & 0xffff;
     ties += total >> 16;
   }
 }
 
 template <int D, int KIND>
-__global__ void __launch_bounds__(kMoveThreads) kv_move_kernel(const EvictArgs a) {
+__global__ void __launch_bounds__(kMoveThreads, D <= 128 ? 2 : 1) kv_move_kernel(const EvictArgs a) {
   using V8 = Kv8<KIND>;
   constexpr int kLanes = D / 16, kRows = 32 / kLanes, kSteps = 16 / kRows;  // a warp: 16 tokens, 16 bytes a lane
-  __shared__ double s_top[kMoveWarps];
-  __shared__ int s_same[kMoveWarps];
+  __shared__ double s_top[2][kMoveWarps];
+  __shared__ int s_same[2][kMoveWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % kLanes, rr = lane / kLanes;
   pdl_launch_dependents();
   pdl_wait();
@@ -177,7 +189,8 @@ __global__ void __launch_bounds__(kMoveThreads) kv_move_kernel(const EvictArgs a
   const int units = 2 * ((m + page - 1) >> a.c.shift);
   const int rounds = (units + at_once - 1) / at_once;
   const int mine = warp / team, part = warp - mine * team;
-  for (int round = blockIdx.y; round < rounds; round += a.chunks) {
+  int turn = 0;
+  for (int round = blockIdx.y; round < rounds; round += a.chunks, turn ^= 1) {
     const int unit = round * at_once + mine;
     const int block = unit >> 1, is_v = unit & 1;
     const bool active = unit < units;
@@ -229,13 +242,19 @@ __global__ void __launch_bounds__(kMoveThreads) kv_move_kernel(const EvictArgs a
     for (int d = 1; d < 32; d <<= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, d));
     same = __all_sync(0xffffffffu, same);
     if (lane == 0) {
-      s_top[warp] = top;
-      s_same[warp] = same;
+      s_top[turn][warp] = top;
+      s_same[turn][warp] = same;
     }
-    __syncthreads();  // every warp has read its pages
+    // in place every warp has to have read its pages before any is written; else only the warps of a page exchange
+    if (a.in_place)
+      __syncthreads();
+    else if (team > 1)
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + mine), "r"(32 * team) : "memory");
+    else
+      __syncwarp();
     for (int x = 0; x < team; ++x) {
-      top = fmax(top, s_top[mine * team + x]);
-      same = same && s_same[mine * team + x];
+      top = fmax(top, s_top[turn][mine * team + x]);
+      same = same && s_same[turn][mine * team + x];
     }
     if (active) {
       const int64_t dp = a.dest[seq * a.dest_stride + block];
@@ -266,7 +285,7 @@ __global__ void __launch_bounds__(kMoveThreads) kv_move_kernel(const EvictArgs a
         if (!is_v && lane < 16 && jw < m) a.c.w[(ph << a.c.shift) + part * 16 + lane] = weight;
       }
     }
-    __syncthreads();  // s_top / s_same are free, and in place the round's pages are written before the next reads
+    if (a.in_place) __syncthreads();  // the round's pages are written before the next reads
   }
 }
 

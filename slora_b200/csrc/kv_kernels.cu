@@ -14,8 +14,9 @@ using namespace slora;
 
 namespace {
 
+// `cluster`: CTAs along y that form a cluster (1: none).
 template <auto kernel, typename... A>
-int launch_pdl(dim3 grid, int threads, size_t smem, cudaStream_t stream, const char* what, const A&... args) {
+int launch_cluster(int cluster, dim3 grid, int threads, size_t smem, cudaStream_t stream, const char* what, const A&... args) {
   // more than 48 KB of shared memory is opted in to once per kernel, device and size
   static std::atomic<size_t> opted[64];
   int dev = 0;
@@ -33,11 +34,18 @@ int launch_pdl(dim3 grid, int threads, size_t smem, cudaStream_t stream, const c
   cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  if (cluster > 1) {
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 1;
+    attr[1].val.clusterDim.y = static_cast<unsigned>(cluster);
+    attr[1].val.clusterDim.z = 1;
+    cfg.numAttrs = 2;
+  }
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
   if (e != cudaSuccess) {
     cudaGetLastError();
@@ -45,6 +53,11 @@ int launch_pdl(dim3 grid, int threads, size_t smem, cudaStream_t stream, const c
   }
   g_launches[3].fetch_add(1, std::memory_order_relaxed);
   return SLORA_OK;
+}
+
+template <auto kernel, typename... A>
+int launch_pdl(dim3 grid, int threads, size_t smem, cudaStream_t stream, const char* what, const A&... args) {
+  return launch_cluster<kernel>(1, grid, threads, smem, stream, what, args...);
 }
 
 int sm_count() {
@@ -142,9 +155,9 @@ int check_rotary(int head_dim, int rot, int layout, const void* positions, const
   return SLORA_OK;
 }
 
-// CTAs that share a block of tokens, so that a small call still fills the GPU: about two per SM, at least one row a warp.
+// CTAs that share a block of tokens, so that a small call still fills the GPU: about eight per SM, at least one row a warp.
 int head_splits(int64_t units, int rows) {
-  const int64_t want = 2 * sm_count() / (units > 0 ? units : 1);
+  const int64_t want = (8 * sm_count() + units - 1) / (units > 0 ? units : 1);
   const int most = (rows + kRowWarps - 1) / kRowWarps;
   return static_cast<int>(want < 1 ? 1 : want > most ? most : want);
 }
@@ -272,7 +285,7 @@ int check_attend(const slora_kv8_cache* cache, const slora_kv8_batch* batch, int
 
 template <int D, int KIND, typename T>
 int append_launch(const AppendArgs& a, dim3 grid, size_t smem, cudaStream_t s) {
-  return launch_pdl<kv_append_kernel<D, KIND, T>>(grid, kRowThreads, smem, s, "kv8_append", a);
+  return launch_cluster<kv_append_kernel<D, KIND, T>>(static_cast<int>(grid.y), grid, kRowThreads, smem, s, "kv8_append", a);
 }
 template <int D, int KIND, typename T>
 int read_launch(const ReadArgs& a, int grid, cudaStream_t s) {
@@ -315,8 +328,8 @@ int slora_rotary(void* q_out, void* k_out, const void* q, const void* k, int64_t
     a.heads[i] = heads[i];
   }
   a.T = T;
-  const int64_t per = (T + 4 * sm_count() - 1) / (4 * sm_count());
-  a.tokens_per_cta = static_cast<int>(per < 1 ? 1 : per > 16 ? 16 : per);
+  const int64_t per = (T + 8 * sm_count() - 1) / (8 * sm_count());
+  a.tokens_per_cta = static_cast<int>(per < 1 ? 1 : per > 8 ? 8 : per);
   const int64_t blocks = (T + a.tokens_per_cta - 1) / a.tokens_per_cta;
   a.head_splits = head_splits(blocks, q_heads + k_heads);
   const size_t smem = static_cast<size_t>(a.tokens_per_cta) * (rot / 2) * sizeof(float2);
@@ -364,7 +377,9 @@ int slora_kv8_append(const slora_kv8_cache* cache, const slora_kv8_batch* batch,
   int64_t units = (T >> a.c.shift) + 2 * seqs;
   if (units > T) units = T;
   if (a.b.max_q == 1 && units > seqs) units = seqs;
-  a.head_splits = head_splits(units, a.hq + 2 * a.c.hkv);
+  int splits = head_splits(units, a.hq + 2 * a.c.hkv);
+  splits = splits >= 8 ? 8 : splits >= 4 ? 4 : splits >= 2 ? 2 : 1;  // a cluster
+  a.head_splits = splits;
   const int page = 1 << a.c.shift;
   const int tokens = a.b.max_q < page ? a.b.max_q : page;
   const size_t smem = turns ? static_cast<size_t>(tokens) * (rot / 2) * sizeof(float2) : 0;
