@@ -276,16 +276,18 @@ __device__ __forceinline__ void append_rescale(uint8_t* page, int bytes, float s
   }
 }
 
-// Eight values at scale s_new, packed.
+// Eight values at scale s_new, packed; fine: all of them are finite.
 template <int KIND>
-__device__ __forceinline__ uint2 append_pack(float (&x)[8], float mul, float s_new) {
+__device__ __forceinline__ uint2 append_pack(float (&x)[8], float mul, float s_new, bool fine) {
   uint2 w = make_uint2(0, 0);
   if (s_new > 0.f) {
+    if (!fine) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) kv_finite(x[e]);
+      for (int e = 0; e < 8; ++e) kv_finite(x[e]);
+    }
     const float lo[4] = {x[0], x[1], x[2], x[3]}, hi[4] = {x[4], x[5], x[6], x[7]};
-    w.x = kv_round4<KIND>(lo, 1.f, mul, s_new);
-    w.y = kv_round4<KIND>(hi, 1.f, mul, s_new);
+    w.x = kv_round4<KIND>(lo, 1.f, mul, s_new, !fine);
+    w.y = kv_round4<KIND>(hi, 1.f, mul, s_new, !fine);
   }
   return w;
 }
@@ -314,7 +316,7 @@ __device__ __forceinline__ void append_page_cta(const AppendArgs& a, const T* sr
   };
   float top = 0.f;
   bool fine = true;
-#pragma unroll 1
+#pragma unroll 2
   for (int p = 0; p < passes; ++p) {
     float x[8];
     row(p, x);
@@ -332,14 +334,14 @@ __device__ __forceinline__ void append_page_cta(const AppendArgs& a, const T* sr
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, tops[w]);
-  const float s_new = fmaxf(s_old, __fdiv_rn(top, V8::kTop));
+  const float s_new = kv_scale(fmaxf(s_old, __fdiv_rn(top, V8::kTop)));
   if (s_new != s_old && n0 > 0) append_rescale<KIND>(page, n0 * D, s_old, s_new, threadIdx.x, kRowThreads);
   const float mul = s_new > 0.f ? __fdiv_rn(1.f, s_new) : 0.f;
-#pragma unroll 1
+#pragma unroll 2
   for (int p = 0; p < passes; ++p) {
     float x[8];
     row(p, x);
-    const uint2 w = append_pack<KIND>(x, mul, s_new);
+    const uint2 w = append_pack<KIND>(x, mul, s_new, fine);
     const int i = first + p * kPass;
     if (i < n1) *reinterpret_cast<uint2*>(page + i * D + 8 * sub) = w;
   }
@@ -383,12 +385,12 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, const T* src, i
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
   if (!fine) set_status(a.b.status, kStatusNonfinite);
-  const float s_new = fmaxf(s_old, __fdiv_rn(top, V8::kTop));
+  const float s_new = kv_scale(fmaxf(s_old, __fdiv_rn(top, V8::kTop)));
   if (s_new != s_old && n0 > 0) append_rescale<KIND>(page, n0 * D, s_old, s_new, lane, 32);
   const float mul = s_new > 0.f ? __fdiv_rn(1.f, s_new) : 0.f;
   for (int base = n0; base < n1; base += kRows) {
     const bool real = load(base);
-    const uint2 w = append_pack<KIND>(x, mul, s_new);
+    const uint2 w = append_pack<KIND>(x, mul, s_new, fine);
     if (real) *reinterpret_cast<uint2*>(page + (base + rr) * D + 8 * sub) = w;
   }
   __syncwarp();

@@ -114,81 +114,86 @@ struct Kv8<SLORA_KV_E4M3> {
   }
 };
 
-// round((x + lo) / s) in the 8-bit type, to nearest, ties to even, of the exact quotient (s > 0; x + lo exact in two FP32
-// words, |lo| <= ulp(x) / 2): the stored byte.  The FP32 quotient is within an ulp or so of the exact one, so it decides
-// everywhere but next to a border between two 8-bit values; there the sign of x + lo - border * s does (fma: one
-// rounding, and the difference is small).  Pages that are scaled anew sit on such borders often: their ratios are small
-// fractions.
+// The larger magnitudes of two pairs of f16.
+__device__ __forceinline__ uint32_t max_abs_f16(uint32_t a, uint32_t b) {
+  uint32_t r, t;
+  asm("abs.f16x2 %0, %1;" : "=r"(t) : "r"(b));
+  asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(t));
+  return r;
+}
+// The largest stored magnitude of 16 bytes.
 template <int KIND>
-__device__ __noinline__ uint32_t kv_round(float x, float lo, float s) {
-  const float y = __fdiv_rn(x, s);
-  float m = fabsf(y);
-  float step = 1.f, inv = 1.f;
-  if (!Kv8<KIND>::kInt) {  // spacing of the type at m: three bits behind the leading one, 2^-9 below 2^-6
-    const uint32_t e = max(__float_as_uint(m) >> 23, 121u);
-    step = __uint_as_float((e - 3u) << 23);
-    inv = __uint_as_float((257u - e) << 23);  // 2^(3 - (e - 127)), e <= 254 - 3 for every value below the clamp
-    if (m > 1024.f) return (__float_as_uint(y) >> 31 << 7) | 0x7eu;
-  } else {
-    m = fminf(m, 1024.f);
+__device__ __forceinline__ float kv_top(const uint4& v) {
+  using V8 = Kv8<KIND>;
+  uint32_t m = 0;
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t x = V8::prepare(w[i]);
+    m = max_abs_f16(max_abs_f16(m, V8::lo(x)), V8::hi(x));
   }
-  const float k = m * inv;  // in steps, exact
-  const float f = floorf(k);
-  const float off = k - f;
-  float r = off > 0.5f || (off == 0.5f && (static_cast<int>(f) & 1)) ? f + 1.f : f;
-  if (fabsf(off - 0.5f) < 2e-4f) {
-    const float border = copysignf((f + 0.5f) * step, y);
-    const float diff = copysignf(1.f, y) * (__fmaf_rn(-border, s, x) + lo);
-    r = diff > 0.f ? f + 1.f : diff < 0.f ? f : f + static_cast<float>(static_cast<int>(f) & 1);
-  }
-  const uint32_t sign = __float_as_uint(y) >> 31;
-  if (Kv8<KIND>::kInt) {
-    const int q = static_cast<int>(fminf(r, 127.f));
-    return static_cast<uint32_t>(sign ? -q : q) & 0xffu;
-  }
-  const float v = fminf(r * step, 448.f);  // a value of the type
-  const uint32_t h = __half_as_ushort(__float2half_rn(v * (1.f / 256.f)));  // sign-less f16 fields, exact
-  return (sign << 7) | (h >> 7);
+  const float2 f = __half22float2(reinterpret_cast<const __half2&>(m));
+  return fmaxf(f.x, f.y) * V8::kScale;
 }
 
-// The same for four values x[e] = from[e] * by (by: what the values were scaled with; 1 for new ones) at once, packed into
-// a word.  y[e] = from[e] * mul with mul = by / s is, up to roundings, within 2^-22 of the exact quotient; only where that
-// is next to a border kv_round decides (for e4m3 also below 2^-6, where the steps no longer follow the exponent).
+// Scales below FP32's smallest normal number count as 0 (their inverse need not exist).
+constexpr float kLeastScale = 1.17549435e-38f;
+__device__ __forceinline__ float kv_scale(float s) { return s < kLeastScale ? 0.f : s; }
+
+// round(from[e] * by / s) in the 8-bit type for four values (by: what they were scaled with; 1 for new ones), to nearest,
+// ties to even, of the exact quotient, packed into a word.  s >= kLeastScale, mul = by / s.
+//
+// from * mul is, up to two or three roundings, within 2^-21.4 of the quotient, so it decides everywhere but next to a border
+// between two 8-bit values (for e4m3 also below 2^-6, where the steps no longer follow the exponent); there the sign of
+// from * by - border * s does, exactly: from * by in two words, an fma with one rounding, and the difference is small.
+// Pages that are scaled anew sit on such borders often: their ratios are small fractions.
+// int8: from * mul + 384 lies in [256, 512), whose FP32 numbers are 2^-15 apart: one fma leaves 128 + the quotient in fixed
+// point, twice that plus a half its rounding in byte 2 and what was rounded in the lower half.
+// far: some value may lie beyond the type's range (an infinity): all take the exact way, which clamps.
 template <int KIND>
-__device__ __forceinline__ uint32_t kv_round4(const float (&from)[4], float by, float mul, float s) {
-  uint32_t w;
-  bool near = !(mul < 1e37f);  // a scale next to FP32's smallest numbers has no inverse
+__device__ __forceinline__ uint32_t kv_round4(const float (&from)[4], float by, float mul, float s, bool far = false) {
+  uint32_t r[4];
+  float y[4];
+  bool near = far;
   if (Kv8<KIND>::kInt) {
-    float t[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float y = fminf(fmaxf(from[e] * mul, -127.f), 127.f);
-      t[e] = y + 12582912.f;  // 1.5 * 2^23: the sum's last bits are y rounded to a whole number
-      near = near || fabsf(y - (t[e] - 12582912.f)) > 0.4999f;
+      r[e] = __float_as_uint(__fmaf_rn(from[e], mul, 384.f)) * 2u + 0x8000u;
+      near = near || r[e] * 0x10000u + 0x40000u <= 0x80000u;  // within two steps of a half
     }
-    w = prmt(prmt(__float_as_uint(t[0]), __float_as_uint(t[1]), 0x0040), prmt(__float_as_uint(t[2]), __float_as_uint(t[3]), 0x0040), 0x5410);
   } else {
-    float y[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       y[e] = from[e] * mul;
-      const uint32_t b = __float_as_uint(y[e]) & 0x7fffffffu;
-      near = near || (b & 0xfffffu) - 0x7ffe0u < 0x40u || b - 1u < 0x3c800000u - 1u;
+      near = near || __float_as_uint(y[e]) * 0x1000u - 0x7ffe0000u < 0x40000u || (fabsf(y[e]) < 0.015625f && from[e] != 0.f);
     }
-    unsigned short lo, hi;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(y[1]), "f"(y[0]));
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(y[3]), "f"(y[2]));
-    w = lo | static_cast<uint32_t>(hi) << 16;
   }
   if (near) {
-    w = 0;
-#pragma unroll 1
+#pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float f = e == 0 ? from[0] : e == 1 ? from[1] : e == 2 ? from[2] : from[3];
-      const float x = f * by;
-      w |= kv_round<KIND>(x, __fmaf_rn(f, by, -x), s) << (8 * e);
+      const float top = Kv8<KIND>::kTop;
+      const float q = fminf(fmaxf(from[e] * mul, -top), top);
+      // steps of the type at q: 1, or three bits behind the leading one and 2^-9 below 2^-6
+      float step = 1.f, inv = 1.f;
+      if (!Kv8<KIND>::kInt) {
+        const uint32_t x = max(__float_as_uint(fabsf(q)) >> 23, 121u);
+        step = __uint_as_float((x - 3u) << 23);
+        inv = __uint_as_float((257u - x) << 23);
+      }
+      const float low = floorf(q * inv);  // the value is low or low + 1 steps
+      const float x = from[e] * by;
+      const float over = __fmaf_rn(-(low + 0.5f) * step, s, x) + __fmaf_rn(from[e], by, -x);
+      const float odd = static_cast<float>(static_cast<int>(low) & 1);
+      const float k = over > 0.f ? low + 1.f : over < 0.f ? low : low + odd;
+      y[e] = k * step;
+      r[e] = static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(k, -top), top)) + 128) << 16;
     }
   }
-  return w;
+  if (Kv8<KIND>::kInt) return prmt(prmt(r[0], r[1], 0x0062), prmt(r[2], r[3], 0x0062), 0x5410) ^ 0x80808080u;
+  unsigned short lo, hi;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(y[1]), "f"(y[0]));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(y[3]), "f"(y[2]));
+  return lo | static_cast<uint32_t>(hi) << 16;
 }
+
 }  // namespace slora

@@ -167,11 +167,41 @@ __global__ void __launch_bounds__(kSelectThreads) kv_select_kernel(const EvictAr
   }
 }
 
+// One page's part of a warp: 16 tokens of k or of v, 16 bytes a lane.
+template <int D>
+struct MoveRows {
+  static constexpr int kLanes = D / 16, kRows = 32 / kLanes, kSteps = 16 / kRows;
+  uint4 w[kSteps];
+  float s[kSteps];
+};
+
+// Rounds the rows to the page's scale (or leaves them) and stores those that `write` has a bit for.
 template <int D, int KIND>
-__global__ void __launch_bounds__(kMoveThreads, D <= 128 ? 2 : 1) kv_move_kernel(const EvictArgs a) {
+__device__ __forceinline__ void move_store(MoveRows<D>& m, uint8_t* dst, bool same, float now, unsigned write) {
   using V8 = Kv8<KIND>;
-  constexpr int kLanes = D / 16, kRows = 32 / kLanes, kSteps = 16 / kRows;  // a warp: 16 tokens, 16 bytes a lane
-  __shared__ double s_top[2][kMoveWarps];
+  const float inv = now > 0.f ? __fdiv_rn(1.f, now) : 0.f;
+#pragma unroll
+  for (int i = 0; i < MoveRows<D>::kSteps; ++i) {
+    if (!same) {
+      const float mul = m.s[i] * inv;
+      uint32_t words[4] = {m.w[i].x, m.w[i].y, m.w[i].z, m.w[i].w};
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        float v[4];
+        V8::values(words[x], v);
+        words[x] = now > 0.f ? kv_round4<KIND>(v, m.s[i], mul, now) : 0u;
+      }
+      m.w[i] = make_uint4(words[0], words[1], words[2], words[3]);
+    }
+    if (write >> i & 1u) *reinterpret_cast<uint4*>(dst + i * MoveRows<D>::kRows * D) = m.w[i];
+  }
+}
+
+template <int D, int KIND>
+__global__ void __launch_bounds__(kMoveThreads, D <= 128 ? 3 : 1) kv_move_kernel(const EvictArgs a) {
+  using V8 = Kv8<KIND>;
+  constexpr int kLanes = D / 16, kRows = 32 / kLanes, kSteps = 16 / kRows;
+  __shared__ double s_top[2][2][kMoveWarps];  // [round's parity][k, v]
   __shared__ int s_same[2][kMoveWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % kLanes, rr = lane / kLanes;
   pdl_launch_dependents();
@@ -183,66 +213,60 @@ __global__ void __launch_bounds__(kMoveThreads, D <= 128 ? 2 : 1) kv_move_kernel
   const int m = min(n, a.budget);
   if (a.in_place && n <= a.budget) return;
   const int32_t* kept = a.kept + static_cast<int64_t>(sh) * a.budget;
-  const int page = 1 << a.c.shift, in_page = page - 1;
-  const int team = page / 16;              // warps of a unit: (page, k or v)
-  const int at_once = kMoveWarps / team;   // units of a round
-  const int units = 2 * ((m + page - 1) >> a.c.shift);
-  const int rounds = (units + at_once - 1) / at_once;
+  const int shift = a.c.shift, page = 1 << shift, in_page = page - 1;
+  const int team = page / 16;              // warps of a page
+  const int at_once = kMoveWarps / team;   // pages of a round
+  const int pages = (m + page - 1) >> shift;
+  const int rounds = (pages + at_once - 1) / at_once;
   const int mine = warp / team, part = warp - mine * team;
   int turn = 0;
   for (int round = blockIdx.y; round < rounds; round += a.chunks, turn ^= 1) {
-    const int unit = round * at_once + mine;
-    const int block = unit >> 1, is_v = unit & 1;
-    const bool active = unit < units;
-    const uint8_t* src8 = is_v ? a.c.v : a.c.k;
-    const float* src_s = is_v ? a.c.vs : a.c.ks;
-    // read: this warp's 16 tokens
-    uint4 w[kSteps];
-    float s[kSteps];
-    double top = 0.0;
+    const int block = round * at_once + mine;
+    const bool active = block < pages;
+    // places (token rows of the cache, -1 none) of this warp's 16 tokens: lane l < 16 looks up token l
+    const int j = block * page + part * 16 + (lane & 15);
+    int place = -1;
     bool same = true;
-    float weight = 0.f;
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-      w[i] = make_uint4(0, 0, 0, 0);
-      s[i] = 0.f;
-      const int j = block * page + part * 16 + i * kRows + rr;
-      if (active && j < m) {
-        const int from = kept[j];
-        same = same && from == j;
-        const int64_t p = kv_page(a.c, a.b, seq, from);
-        if (p >= 0) {
-          const int64_t ph = p * a.c.hkv + head;
-          w[i] = *reinterpret_cast<const uint4*>(src8 + ((ph << a.c.shift) + (from & in_page)) * D + 16 * sub);
-          s[i] = src_s[ph];
-        } else {
-          set_status(a.b.status, SLORA_STATUS_BAD_TABLE);
-        }
-      }
-    }
-    const int jw = block * page + part * 16 + lane;  // lanes 0..15: the weight of a token each
-    if (active && !is_v && lane < 16 && jw < m) {
-      const int from = kept[jw];
+    if (active && j < m) {
+      const int from = kept[j];
+      same = from == j;
       const int64_t p = kv_page(a.c, a.b, seq, from);
-      if (p >= 0) weight = a.c.w[((p * a.c.hkv + head) << a.c.shift) + (from & in_page)];
+      if (p >= 0)
+        place = static_cast<int>(((p * a.c.hkv + head) << shift) + (from & in_page));
+      else
+        set_status(a.b.status, SLORA_STATUS_BAD_TABLE);
     }
+    same = __all_sync(0xffffffffu, same);
+    MoveRows<D> k, v;
 #pragma unroll
     for (int i = 0; i < kSteps; ++i) {
-      float q = 0.f;
-      const uint32_t words[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        float v[4];
-        V8::values(words[x], v);
-        q = fmaxf(fmaxf(q, fmaxf(fabsf(v[0]), fabsf(v[1]))), fmaxf(fabsf(v[2]), fabsf(v[3])));
+      const int at = __shfl_sync(0xffffffffu, place, i * kRows + rr);
+      k.w[i] = v.w[i] = make_uint4(0, 0, 0, 0);
+      k.s[i] = v.s[i] = 0.f;
+      if (at >= 0) {
+        k.w[i] = *reinterpret_cast<const uint4*>(a.c.k + static_cast<int64_t>(at) * D + 16 * sub);
+        v.w[i] = *reinterpret_cast<const uint4*>(a.c.v + static_cast<int64_t>(at) * D + 16 * sub);
+        k.s[i] = a.c.ks[at >> shift];
+        v.s[i] = a.c.vs[at >> shift];
       }
-      top = fmax(top, static_cast<double>(q) * static_cast<double>(s[i]));
     }
+    const float weight = place >= 0 ? a.c.w[place] : 0.f;
+    double top_k = 0.0, top_v = 0.0;
+    if (!same || team > 1) {
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, d));
-    same = __all_sync(0xffffffffu, same);
+      for (int i = 0; i < kSteps; ++i) {
+        top_k = fmax(top_k, static_cast<double>(kv_top<KIND>(k.w[i])) * static_cast<double>(k.s[i]));
+        top_v = fmax(top_v, static_cast<double>(kv_top<KIND>(v.w[i])) * static_cast<double>(v.s[i]));
+      }
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        top_k = fmax(top_k, __shfl_xor_sync(0xffffffffu, top_k, d));
+        top_v = fmax(top_v, __shfl_xor_sync(0xffffffffu, top_v, d));
+      }
+    }
     if (lane == 0) {
-      s_top[turn][warp] = top;
+      s_top[turn][0][warp] = top_k;
+      s_top[turn][1][warp] = top_v;
       s_same[turn][warp] = same;
     }
     // in place every warp has to have read its pages before any is written; else only the warps of a page exchange
@@ -253,7 +277,8 @@ __global__ void __launch_bounds__(kMoveThreads, D <= 128 ? 2 : 1) kv_move_kernel
     else
       __syncwarp();
     for (int x = 0; x < team; ++x) {
-      top = fmax(top, s_top[turn][mine * team + x]);
+      top_k = fmax(top_k, s_top[turn][0][mine * team + x]);
+      top_v = fmax(top_v, s_top[turn][1][mine * team + x]);
       same = same && s_same[turn][mine * team + x];
     }
     if (active) {
@@ -262,27 +287,20 @@ __global__ void __launch_bounds__(kMoveThreads, D <= 128 ? 2 : 1) kv_move_kernel
         if (lane == 0) set_status(a.b.status, SLORA_STATUS_BAD_TABLE);
       } else if (!(a.in_place && same)) {
         const int64_t ph = dp * a.c.hkv + head;
-        uint8_t* dst = (is_v ? a.c.v : a.c.k) + (ph << a.c.shift) * D;
-        const float keep_s = __shfl_sync(0xffffffffu, s[0], 0);
-        const float now = static_cast<float>(top / static_cast<double>(V8::kTop));
+        unsigned write = 0;
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-          const int slot = part * 16 + i * kRows + rr;
-          if (!same) {
-            const float mul = now > 0.f ? __fdiv_rn(s[i], now) : 0.f;
-            uint32_t words[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              float v[4];
-              V8::values(words[x], v);
-              words[x] = now > 0.f ? kv_round4<KIND>(v, s[i], mul, now) : 0u;
-            }
-            w[i] = make_uint4(words[0], words[1], words[2], words[3]);
-          }
-          if (block * page + slot < m) *reinterpret_cast<uint4*>(dst + slot * D + 16 * sub) = w[i];
+        for (int i = 0; i < kSteps; ++i) write |= (block * page + part * 16 + i * kRows + rr < m ? 1u : 0u) << i;
+        const int64_t at = ((ph << shift) + part * 16 + rr) * D + 16 * sub;
+        const float was_k = __shfl_sync(0xffffffffu, k.s[0], 0), was_v = __shfl_sync(0xffffffffu, v.s[0], 0);
+        const float now_k = same ? was_k : kv_scale(static_cast<float>(top_k * (1.0 / V8::kTop)));
+        const float now_v = same ? was_v : kv_scale(static_cast<float>(top_v * (1.0 / V8::kTop)));
+        move_store<D, KIND>(k, a.c.k + at, same, now_k, write);
+        move_store<D, KIND>(v, a.c.v + at, same, now_v, write);
+        if (part == 0 && lane == 0) {
+          a.c.ks[ph] = now_k;
+          a.c.vs[ph] = now_v;
         }
-        if (part == 0 && lane == 0) (is_v ? a.c.vs : a.c.ks)[ph] = same ? keep_s : now;
-        if (!is_v && lane < 16 && jw < m) a.c.w[(ph << a.c.shift) + part * 16 + lane] = weight;
+        if (lane < 16 && j < m) a.c.w[(ph << shift) + part * 16 + lane] = weight;
       }
     }
     if (a.in_place) __syncthreads();  // the round's pages are written before the next reads

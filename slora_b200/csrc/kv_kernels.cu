@@ -485,7 +485,7 @@ int slora_kv8_evict(const slora_kv8_cache* cache, const slora_kv8_batch* batch, 
   if (int rc = launch_pdl<kv_select_kernel>(dim3(static_cast<unsigned>(heads)), kSelectThreads,
                           static_cast<size_t>(a.cached) * sizeof(uint32_t), s, "kv8_evict select", a))
     return rc;
-  const int64_t rounds = (2 * ((longest + (1 << a.c.shift) - 1) >> a.c.shift) * ((1 << a.c.shift) / 16) + kMoveWarps - 1) / kMoveWarps;
+  const int64_t rounds = (((longest + (1 << a.c.shift) - 1) >> a.c.shift) * ((1 << a.c.shift) / 16) + kMoveWarps - 1) / kMoveWarps;
   int64_t chunks = a.in_place ? 1 : (16ll * sm_count() + heads - 1) / heads;
   if (chunks > rounds) chunks = rounds < 1 ? 1 : rounds;
   if (chunks > 65535) chunks = 65535;
