@@ -19,7 +19,7 @@ namespace slora {
 
 constexpr int kRowThreads = 256;
 constexpr int kRowWarps = kRowThreads / 32;
-constexpr int kAppendWarpTokens = 4;  // new tokens of a page up to which a warp takes a (head, k or v) by itself
+constexpr int kAppendWarpTokens = 4;  // new tokens of a sequence up to which a warp takes a (head, k or v) by itself
 
 struct RotaryArgs {
   const int64_t* positions;
@@ -52,7 +52,7 @@ struct AppendArgs {
   int64_t q_stride, q_out_stride, k_stride, v_stride;
   int hq;
   int head_splits;
-  int max_units;  // pages a sequence's new tokens touch, at most
+  int rows_at, rows_step;  // shared memory behind the cosines: rows of one (page, head), and of the next (0: one buffer)
 };
 
 __device__ __forceinline__ float2 rotary_pair(const RotaryArgs& r, int64_t token, int pair) {
@@ -84,31 +84,30 @@ __device__ __forceinline__ void rotary_table_cluster(const RotaryArgs& r, int64_
   cluster_sync_all();
 }
 
-// The cosines and sines that a lane needs for the eight elements 8 sub .. 8 sub + 7 of a head row of one token.
+// The cosines and sines that a lane needs for the eight elements 8 sub .. 8 sub + 7 of a head row of one token; in the half
+// layout the sines carry the sign of the lane's part, so that both parts are x cos + partner sin.
 struct RotaryLane {
   float2 w[8];
-  int other;      // half layout: lane with the partners
-  int part;       // 0 stays as it is, 1 first of the pairs (or interleaved), 2 second
+  int other;  // half layout: lane with the partners
+  bool in;    // these elements turn
   __device__ __forceinline__ void load(const float2* cs, int sub, int rot, int layout) {
     const int lane = threadIdx.x & 31;
     other = lane;
-    part = 0;
+    in = 8 * sub < rot;
     if (layout == 0) {
       const int far = rot >> 4;  // lanes between the partners
-      if (sub < 2 * far) {
-        part = sub < far ? 1 : 2;
-        other = part == 1 ? lane + far : lane - far;
-        const float4* p = reinterpret_cast<const float4*>(cs + 8 * (part == 1 ? sub : sub - far));
+      const bool low = sub < far;
+      if (in) other = low ? lane + far : lane - far;
+      const float4* p = reinterpret_cast<const float4*>(cs + (in ? 8 * (low ? sub : sub - far) : 0));
+      const float sign = low ? -1.f : 1.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float4 v = p[e];
-          w[2 * e] = make_float2(v.x, v.y);
-          w[2 * e + 1] = make_float2(v.z, v.w);
-        }
+      for (int e = 0; e < 4; ++e) {
+        const float4 v = p[e];
+        w[2 * e] = make_float2(v.x, v.y * sign);
+        w[2 * e + 1] = make_float2(v.z, v.w * sign);
       }
-    } else if (8 * sub < rot) {
-      part = 1;
-      const float4* p = reinterpret_cast<const float4*>(cs + 4 * sub);
+    } else {
+      const float4* p = reinterpret_cast<const float4*>(cs + (in ? 4 * sub : 0));
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const float4 v = p[e];
@@ -123,9 +122,10 @@ struct RotaryLane {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float y = __shfl_sync(0xffffffffu, x[e], other);
-        if (part != 0) x[e] = part == 1 ? x[e] * w[e].x - y * w[e].y : y * w[e].y + x[e] * w[e].x;
+        const float z = x[e] * w[e].x + y * w[e].y;
+        x[e] = in ? z : x[e];
       }
-    } else if (part != 0) {
+    } else if (in) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float a = x[2 * e], b = x[2 * e + 1];
@@ -135,6 +135,21 @@ struct RotaryLane {
     }
   }
 };
+
+// The largest magnitude of eight values into top; `odd` stays 0 while all are finite (NaN and infinities make it NaN).
+__device__ __forceinline__ void append_top(const float (&x)[8], float* top, float* odd) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    *top = fmaxf(*top, fabsf(x[e]));
+    *odd = __fmaf_rn(x[e], 0.f, *odd);
+  }
+}
+// The same without what is not finite.
+__device__ __forceinline__ void append_top_finite(const float (&x)[8], float* top) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (fabsf(x[e]) <= 3.4028234663852886e38f) *top = fmaxf(*top, fabsf(x[e]));
+}
 
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
@@ -247,11 +262,9 @@ __device__ __forceinline__ bool append_find(const AppendArgs& a, int u, AppendUn
   return found.seq >= 0;
 }
 
-// NaN -> 0, infinities -> the largest FP32; tells whether x was one of them.
-__device__ __forceinline__ bool kv_finite(float& x) {
-  if (fabsf(x) <= 3.4028234663852886e38f) return true;
-  x = x == x ? copysignf(3.4028234663852886e38f, x) : 0.f;
-  return false;
+// NaN -> 0, infinities -> the largest FP32.
+__device__ __forceinline__ void kv_finite(float& x) {
+  if (!(fabsf(x) <= 3.4028234663852886e38f)) x = x == x ? copysignf(3.4028234663852886e38f, x) : 0.f;
 }
 
 // Older values of a (page, head), `bytes` of them, rounded to a grown scale: 16 bytes a lane.
@@ -292,44 +305,55 @@ __device__ __forceinline__ uint2 append_pack(float (&x)[8], float mul, float s_n
   return w;
 }
 
-// One (page, head) of k or v by the whole CTA, for pages with more than a few new tokens.  The rows are read twice, the
-// second time from L1: kept in registers they left room for one CTA per SM.
+// New rows of one (page, head) of k or v into shared memory, [token][d], asynchronously.
+template <int D, typename T>
+__device__ __forceinline__ void append_fetch(uint8_t* to, const T* src, int64_t stride, int n) {
+  for (int x = threadIdx.x; x < n * (D / 8); x += kRowThreads) {
+    const int i = x / (D / 8), c = x % (D / 8);
+    cp_async16(smem_u32(to + x * 16), src + i * stride + 8 * c);
+  }
+  cp_async_commit();
+}
+
+// One (page, head) of k or v by the whole CTA, for pages with more than a few new tokens, from its rows in shared memory.
 template <int D, int KIND, typename T>
-__device__ __forceinline__ void append_page_cta(const AppendArgs& a, const T* src, int64_t stride, int n0, int n1, uint8_t* page,
+__device__ __forceinline__ void append_page_cta(const AppendArgs& a, const uint8_t* rows, int n0, int n1, uint8_t* page,
                                                 float* scale, const float2* cs, bool turn) {
   constexpr int kLanes = D / 8, kRows = 32 / kLanes, kPass = kRowWarps * kRows;
   using V8 = Kv8<KIND>;
   __shared__ float tops[kRowWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % kLanes, half = a.r.rot >> 1;
-  const int first = n0 + warp * kRows + lane / kLanes, passes = (n1 - n0 + kPass - 1) / kPass;
+  const int mine = warp * kRows + lane / kLanes, n = n1 - n0, passes = (n + kPass - 1) / kPass;
   const float s_old = n0 > 0 ? *scale : 0.f;
   auto row = [&](int p, float (&x)[8]) {
-    const int i = first + p * kPass;
-    uint4 raw = make_uint4(0, 0, 0, 0);
-    if (i < n1) raw = *reinterpret_cast<const uint4*>(src + static_cast<int64_t>(i - n0) * stride + 8 * sub);
-    cvt8<T>(raw, x);
+    const int i = min(mine + p * kPass, n - 1);  // lanes without a row repeat the last one
+    cvt8<T>(*reinterpret_cast<const uint4*>(rows + (i * kLanes + sub) * 16), x);
     if (turn) {
       RotaryLane w;
-      w.load(cs + (i < n1 ? i - n0 : 0) * half, sub, a.r.rot, a.r.layout);
+      w.load(cs + i * half, sub, a.r.rot, a.r.layout);
       w.turn(x, a.r.layout);
     }
   };
-  float top = 0.f;
-  bool fine = true;
-#pragma unroll 2
+  float top = 0.f, odd = 0.f;
+#pragma unroll 1
   for (int p = 0; p < passes; ++p) {
     float x[8];
     row(p, x);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const bool ok = kv_finite(x[e]);
-      fine = fine && ok;
-      top = fmaxf(top, ok ? fabsf(x[e]) : 0.f);
+    append_top(x, &top, &odd);
+  }
+  const bool fine = !__any_sync(0xffffffffu, odd != 0.f);
+  if (!fine) {
+    top = 0.f;
+#pragma unroll 1
+    for (int p = 0; p < passes; ++p) {
+      float x[8];
+      row(p, x);
+      append_top_finite(x, &top);
     }
+    if (lane == 0) set_status(a.b.status, kStatusNonfinite);
   }
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-  if (!fine) set_status(a.b.status, kStatusNonfinite);
   if (lane == 0) tops[warp] = top;
   __syncthreads();
 #pragma unroll
@@ -337,15 +361,15 @@ __device__ __forceinline__ void append_page_cta(const AppendArgs& a, const T* sr
   const float s_new = kv_scale(fmaxf(s_old, __fdiv_rn(top, V8::kTop)));
   if (s_new != s_old && n0 > 0) append_rescale<KIND>(page, n0 * D, s_old, s_new, threadIdx.x, kRowThreads);
   const float mul = s_new > 0.f ? __fdiv_rn(1.f, s_new) : 0.f;
-#pragma unroll 2
+#pragma unroll 1
   for (int p = 0; p < passes; ++p) {
     float x[8];
     row(p, x);
     const uint2 w = append_pack<KIND>(x, mul, s_new, fine);
-    const int i = first + p * kPass;
-    if (i < n1) *reinterpret_cast<uint2*>(page + i * D + 8 * sub) = w;
+    const int i = mine + p * kPass;
+    if (i < n) *reinterpret_cast<uint2*>(page + (n0 + i) * D + 8 * sub) = w;
   }
-  __syncthreads();  // every thread has read the old scale and tops
+  __syncthreads();  // every thread has read the rows, the old scale and tops
   if (threadIdx.x == 0) *scale = s_new;
 }
 
@@ -371,20 +395,22 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, const T* src, i
     }
     return real;
   };
-  float top = 0.f;
-  bool fine = true;
+  float top = 0.f, odd = 0.f;
   for (int base = n0; base < n1; base += kRows) {
     load(base);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const bool ok = kv_finite(x[e]);
-      fine = fine && ok;
-      top = fmaxf(top, ok ? fabsf(x[e]) : 0.f);
+    append_top(x, &top, &odd);
+  }
+  const bool fine = !__any_sync(0xffffffffu, odd != 0.f);
+  if (!fine) {
+    top = 0.f;
+    for (int base = n0; base < n1; base += kRows) {
+      load(base);
+      append_top_finite(x, &top);
     }
+    if (lane == 0) set_status(a.b.status, kStatusNonfinite);
   }
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-  if (!fine) set_status(a.b.status, kStatusNonfinite);
   const float s_new = kv_scale(fmaxf(s_old, __fdiv_rn(top, V8::kTop)));
   if (s_new != s_old && n0 > 0) append_rescale<KIND>(page, n0 * D, s_old, s_new, lane, 32);
   const float mul = s_new > 0.f ? __fdiv_rn(1.f, s_new) : 0.f;
@@ -397,8 +423,10 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, const T* src, i
   if (lane == 0) *scale = s_new;
 }
 
-// The new tokens of one page: their q rows, and k and v of this CTA's share of the heads.
-template <int D, int KIND, typename T>
+// The new tokens of one page: their q rows, and k and v of this CTA's share of the heads.  Where pages have many new tokens
+// (WIDE) the two are launches of their own: q's wants few registers and many CTAs.
+enum AppendPart { APPEND_FEW = 0, APPEND_Q = 1, APPEND_KV = 2 };
+template <int D, int KIND, typename T, int PART>
 __device__ __forceinline__ void append_unit(const AppendArgs& a, const AppendUnit& u, float2* cs) {
   const KvSeq s = kv_seq(a.b, u.seq);
   const int page = 1 << a.c.shift, old = max(s.kv - s.q, 0), begin = u.block << a.c.shift;
@@ -414,11 +442,12 @@ __device__ __forceinline__ void append_unit(const AppendArgs& a, const AppendUni
   }
   __syncthreads();
   const int split = blockIdx.y;  // the CTAs of a page are one cluster
-  if (turn && a.q != nullptr) {
+  if (PART != APPEND_KV && turn && a.q != nullptr) {
     const int h0 = static_cast<int>(static_cast<int64_t>(a.hq) * split / a.head_splits);
     const int h1 = static_cast<int>(static_cast<int64_t>(a.hq) * (split + 1) / a.head_splits);
     rotary_rows<D, T>(a.r, static_cast<const T*>(a.q), static_cast<T*>(a.q_out), a.q_stride, a.q_out_stride, row, n1 - n0, h0, h1, cs);
   }
+  if (PART == APPEND_Q) return;
   const int64_t p = kv_page(a.c, a.b, u.seq, begin);
   if (p < 0) {
     if (threadIdx.x == 0) set_status(a.b.status, SLORA_STATUS_BAD_TABLE);
@@ -426,34 +455,62 @@ __device__ __forceinline__ void append_unit(const AppendArgs& a, const AppendUni
   }
   // (head, k or v) of this CTA's share: all warps on one where the page has many new tokens, else one warp each
   const int g0 = static_cast<int>(2ll * a.c.hkv * split / a.head_splits), g1 = static_cast<int>(2ll * a.c.hkv * (split + 1) / a.head_splits);
-  const bool wide = n1 - n0 > kAppendWarpTokens;
-  for (int i = wide ? g0 : g0 + static_cast<int>(threadIdx.x >> 5); i < g1; i += wide ? 1 : kRowWarps) {
-    const int h = i >> 1;
-    const int64_t ph = p * a.c.hkv + h;
-    uint8_t* bytes = ((i & 1) ? a.c.v : a.c.k) + (ph << a.c.shift) * D;
-    const int64_t stride = (i & 1) ? a.v_stride : a.k_stride;
-    const T* src = static_cast<const T*>((i & 1) ? a.v : a.k) + row * stride + h * D;
-    float* scale = ((i & 1) ? a.c.vs : a.c.ks) + ph;
-    const bool turned = turn && !(i & 1);
-    if (wide)
-      append_page_cta<D, KIND, T>(a, src, stride, n0, n1, bytes, scale, cs, turned);
-    else
-      append_page<D, KIND, T>(a, src, stride, n0, n1, bytes, scale, cs, turned);
-    if (a.c.w != nullptr && !(i & 1)) {
-      const int id = wide ? threadIdx.x : threadIdx.x & 31, step = wide ? kRowThreads : 32;
-      for (int x = n0 + id; x < n1; x += step) a.c.w[(ph << a.c.shift) + x] = 0.f;
+  auto source = [&](int i, int64_t* stride) {
+    *stride = (i & 1) ? a.v_stride : a.k_stride;
+    return static_cast<const T*>((i & 1) ? a.v : a.k) + row * *stride + (i >> 1) * D;
+  };
+  auto place = [&](int i, float** scale) {
+    const int64_t ph = p * a.c.hkv + (i >> 1);
+    *scale = ((i & 1) ? a.c.vs : a.c.ks) + ph;
+    return ((i & 1) ? a.c.v : a.c.k) + (ph << a.c.shift) * D;
+  };
+  const int n = n1 - n0;
+  int64_t stride;
+  float* scale;
+  if (PART == APPEND_KV) {
+    uint8_t* rows[2] = {reinterpret_cast<uint8_t*>(cs) + a.rows_at, reinterpret_cast<uint8_t*>(cs) + a.rows_at + a.rows_step};
+    const bool two = a.rows_step > 0;  // two buffers: the next rows come in while these are rounded
+    if (two && g0 < g1) {
+      const T* src = source(g0, &stride);
+      append_fetch<D, T>(rows[0], src, stride, n);
+    }
+    for (int i = g0; i < g1; ++i) {
+      const int buf = two ? (i - g0) & 1 : 0;
+      if (!two || i + 1 < g1) {
+        const T* src = source(two ? i + 1 : i, &stride);
+        append_fetch<D, T>(rows[two ? buf ^ 1 : 0], src, stride, n);
+        if (two)
+          cp_async_wait<1>();
+        else
+          cp_async_wait<0>();
+      } else {
+        cp_async_wait<0>();
+      }
+      __syncthreads();
+      uint8_t* bytes = place(i, &scale);
+      append_page_cta<D, KIND, T>(a, rows[buf], n0, n1, bytes, scale, cs, turn && !(i & 1));
+    }
+  } else {
+    for (int i = g0 + static_cast<int>(threadIdx.x >> 5); i < g1; i += kRowWarps) {
+      const T* src = source(i, &stride);
+      uint8_t* bytes = place(i, &scale);
+      append_page<D, KIND, T>(a, src, stride, n0, n1, bytes, scale, cs, turn && !(i & 1));
     }
   }
+  // weights of new tokens start at 0; the CTA that has a head's k writes them
+  if (a.c.w != nullptr)
+    for (int x = threadIdx.x; x < ((g1 + 1) / 2 - (g0 + 1) / 2) * n; x += kRowThreads)
+      a.c.w[((p * a.c.hkv + (g0 + 1) / 2 + x / n) << a.c.shift) + n0 + x % n] = 0.f;
 }
 
-template <int D, int KIND, typename T>
-__global__ void __launch_bounds__(kRowThreads, 3) kv_append_kernel(const AppendArgs a) {
+template <int D, int KIND, typename T, int PART>
+__global__ void __launch_bounds__(kRowThreads, PART == APPEND_Q ? 4 : 3) kv_append_kernel(const AppendArgs a) {
   extern __shared__ __align__(16) float2 cs[];
   pdl_launch_dependents();
   pdl_wait();
   // the grid holds every unit unless sequences share rows
   AppendUnit u;
-  for (int at = blockIdx.x; append_find(a, at, &u); at += gridDim.x) append_unit<D, KIND, T>(a, u, cs);
+  for (int at = blockIdx.x; append_find(a, at, &u); at += gridDim.x) append_unit<D, KIND, T, PART>(a, u, cs);
 }
 
 struct ReadArgs {

@@ -283,9 +283,31 @@ int check_attend(const slora_kv8_cache* cache, const slora_kv8_batch* batch, int
   return SLORA_OK;
 }
 
+// CTAs of a page's units (a cluster: 1, 2, 4 or 8) for `rows` head rows per token.
+int append_splits(int64_t units, int rows) {
+  const int splits = head_splits(units, rows);
+  return splits >= 8 ? 8 : splits >= 4 ? 4 : splits >= 2 ? 2 : 1;
+}
 template <int D, int KIND, typename T>
-int append_launch(const AppendArgs& a, dim3 grid, size_t smem, cudaStream_t s) {
-  return launch_cluster<kv_append_kernel<D, KIND, T>>(static_cast<int>(grid.y), grid, kRowThreads, smem, s, "kv8_append", a);
+int append_launch(AppendArgs a, int64_t units, int tokens, cudaStream_t s) {
+  const size_t angles = a.r.turns ? static_cast<size_t>(tokens) * (a.r.rot / 2) * sizeof(float2) : 0;
+  if (a.b.max_q <= kAppendWarpTokens) {
+    a.head_splits = append_splits(units, a.hq + 2 * a.c.hkv);
+    return launch_cluster<kv_append_kernel<D, KIND, T, APPEND_FEW>>(a.head_splits, dim3(static_cast<unsigned>(units), a.head_splits),
+                                                                    kRowThreads, angles, s, "kv8_append", a);
+  }
+  if (a.q) {
+    a.head_splits = append_splits(units, a.hq);
+    if (const int rc = launch_cluster<kv_append_kernel<D, 0, T, APPEND_Q>>(a.head_splits, dim3(static_cast<unsigned>(units), a.head_splits),
+                                                                           kRowThreads, angles, s, "kv8_append q", a))
+      return rc;
+  }
+  a.head_splits = append_splits(units, kRowWarps * 2 * a.c.hkv);
+  const size_t rows = static_cast<size_t>(tokens) * D * 2;
+  a.rows_at = static_cast<int>(angles);
+  a.rows_step = angles + 2 * rows <= 200 * 1024 ? static_cast<int>(rows) : 0;
+  return launch_cluster<kv_append_kernel<D, KIND, T, APPEND_KV>>(a.head_splits, dim3(static_cast<unsigned>(units), a.head_splits), kRowThreads,
+                                                                 angles + (a.rows_step > 0 ? 2 : 1) * rows, s, "kv8_append k, v", a);
 }
 template <int D, int KIND, typename T>
 int read_launch(const ReadArgs& a, int grid, cudaStream_t s) {
@@ -377,15 +399,10 @@ int slora_kv8_append(const slora_kv8_cache* cache, const slora_kv8_batch* batch,
   int64_t units = (T >> a.c.shift) + 2 * seqs;
   if (units > T) units = T;
   if (a.b.max_q == 1 && units > seqs) units = seqs;
-  int splits = head_splits(units, a.hq + 2 * a.c.hkv);
-  splits = splits >= 8 ? 8 : splits >= 4 ? 4 : splits >= 2 ? 2 : 1;  // a cluster
-  a.head_splits = splits;
   const int page = 1 << a.c.shift;
   const int tokens = a.b.max_q < page ? a.b.max_q : page;
-  const size_t smem = turns ? static_cast<size_t>(tokens) * (rot / 2) * sizeof(float2) : 0;
-  const dim3 grid(static_cast<unsigned>(units), static_cast<unsigned>(a.head_splits));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return KV_DISPATCH(a.c.d, cache->kind, dtype, (append_launch<D, KIND, T>(a, grid, smem, s)));
+  return KV_DISPATCH(a.c.d, cache->kind, dtype, (append_launch<D, KIND, T>(a, units, tokens, s)));
 }
 
 int slora_kv8_read(const slora_kv8_cache* cache, const slora_kv8_batch* batch, const int32_t* first, int64_t count,
