@@ -106,8 +106,8 @@ struct RotaryLane {
         w[2 * e] = make_float2(v.x, v.y * sign);
         w[2 * e + 1] = make_float2(v.z, v.w * sign);
       }
-    } else {
-      const float4* p = reinterpret_cast<const float4*>(cs + (in ? 4 * sub : 0));
+    } else if (in) {
+      const float4* p = reinterpret_cast<const float4*>(cs + 4 * sub);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const float4 v = p[e];
@@ -434,6 +434,14 @@ __device__ __forceinline__ void append_unit(const AppendArgs& a, const AppendUni
   // rows of q, k, v; with q_len > kv_len (already reported) the first rows have no place and are left out
   const int64_t row = static_cast<int64_t>(s.row) + (s.q - s.kv) + begin + n0;
   const bool turn = a.r.turns != nullptr;
+  if (PART == APPEND_Q) {
+    // the CTAs of a page share its tokens, so each works out its own angles only
+    const int t0 = (n1 - n0) * static_cast<int>(blockIdx.y) / a.head_splits, t1 = (n1 - n0) * static_cast<int>(blockIdx.y + 1) / a.head_splits;
+    rotary_table(a.r, row + t0, t1 - t0, cs);
+    __syncthreads();
+    rotary_rows<D, T>(a.r, static_cast<const T*>(a.q), static_cast<T*>(a.q_out), a.q_stride, a.q_out_stride, row + t0, t1 - t0, 0, a.hq, cs);
+    return;
+  }
   if (turn) {
     if (a.head_splits > 1 && (n1 - n0) * a.r.rot > 2 * kRowThreads)
       rotary_table_cluster(a.r, row, n1 - n0, cs, a.head_splits);
@@ -442,12 +450,11 @@ __device__ __forceinline__ void append_unit(const AppendArgs& a, const AppendUni
   }
   __syncthreads();
   const int split = blockIdx.y;  // the CTAs of a page are one cluster
-  if (PART != APPEND_KV && turn && a.q != nullptr) {
+  if (PART == APPEND_FEW && turn && a.q != nullptr) {
     const int h0 = static_cast<int>(static_cast<int64_t>(a.hq) * split / a.head_splits);
     const int h1 = static_cast<int>(static_cast<int64_t>(a.hq) * (split + 1) / a.head_splits);
     rotary_rows<D, T>(a.r, static_cast<const T*>(a.q), static_cast<T*>(a.q_out), a.q_stride, a.q_out_stride, row, n1 - n0, h0, h1, cs);
   }
-  if (PART == APPEND_Q) return;
   const int64_t p = kv_page(a.c, a.b, u.seq, begin);
   if (p < 0) {
     if (threadIdx.x == 0) set_status(a.b.status, SLORA_STATUS_BAD_TABLE);

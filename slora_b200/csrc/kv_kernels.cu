@@ -17,10 +17,10 @@ namespace {
 // `cluster`: CTAs along y that form a cluster (1: none).
 template <auto kernel, typename... A>
 int launch_cluster(int cluster, dim3 grid, int threads, size_t smem, cudaStream_t stream, const char* what, const A&... args) {
-  // more than 48 KB of shared memory is opted in to once per kernel, device and size
+  // more than 48 KB of shared memory (up to 16 of them static) is opted in to once per kernel, device and size
   static std::atomic<size_t> opted[64];
   int dev = 0;
-  if (smem > 48 * 1024 && (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64 || opted[dev].load(std::memory_order_relaxed) < smem)) {
+  if (smem > 32 * 1024 && (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64 || opted[dev].load(std::memory_order_relaxed) < smem)) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) {
       cudaGetLastError();
@@ -297,9 +297,9 @@ int append_launch(AppendArgs a, int64_t units, int tokens, cudaStream_t s) {
                                                                     kRowThreads, angles, s, "kv8_append", a);
   }
   if (a.q) {
-    a.head_splits = append_splits(units, a.hq);
-    if (const int rc = launch_cluster<kv_append_kernel<D, 0, T, APPEND_Q>>(a.head_splits, dim3(static_cast<unsigned>(units), a.head_splits),
-                                                                           kRowThreads, angles, s, "kv8_append q", a))
+    a.head_splits = (tokens + 7) / 8;  // about eight tokens a CTA
+    if (const int rc = launch_pdl<kv_append_kernel<D, 0, T, APPEND_Q>>(dim3(static_cast<unsigned>(units), a.head_splits), kRowThreads,
+                                                                       static_cast<size_t>(8) * (a.r.rot / 2) * sizeof(float2), s, "kv8_append q", a))
       return rc;
   }
   a.head_splits = append_splits(units, kRowWarps * 2 * a.c.hkv);

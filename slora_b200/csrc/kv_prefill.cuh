@@ -85,6 +85,73 @@ __device__ __forceinline__ uint64_t umma_smem_desc_sw128_mn(uint32_t addr, uint3
   return d;
 }
 
+// The largest score (log2 units) of this thread's row of S: groups of 16 columns share their scale.  The next 32 columns are on
+// their way from tensor memory while 32 are looked at.  MASKED: only columns [from, to) count.
+template <int D, bool MASKED>
+__device__ __forceinline__ float pre_max(const PreSmem<D>& sm, int slot, uint32_t t_s, float down, int from, int to) {
+  float top = kNegInf;
+  uint32_t w[2][32];
+  tmem_ld32(t_s, w[0]);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    tmem_ld_wait();
+    if (c < 3) tmem_ld32(t_s + 32 * (c + 1), w[(c + 1) & 1]);
+    uint32_t(&x)[32] = w[c & 1];
+    if (MASKED) {
+#pragma unroll
+      for (int e = 0; e < 32; ++e)
+        if (32 * c + e < from || 32 * c + e >= to) x[e] = 0xff800000u;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float g0 = __uint_as_float(x[16 * h]), g1 = __uint_as_float(x[16 * h + 1]);
+#pragma unroll
+      for (int e = 2; e < 16; e += 2) {
+        g0 = fmaxf(g0, __uint_as_float(x[16 * h + e]));
+        g1 = fmaxf(g1, __uint_as_float(x[16 * h + e + 1]));
+      }
+      g0 = fmaxf(g0, g1);
+      if (g0 > kNegInf && sm.lv[slot][2 * c + h] > kNegInf) top = fmaxf(top, g0 * (down * sm.fk[slot][2 * c + h]));
+    }
+  }
+  return top;
+}
+
+// p of this thread's row over S (f16 pairs), their sum into l.
+template <int D, bool MASKED>
+__device__ __forceinline__ void pre_exp(const PreSmem<D>& sm, int slot, uint32_t t_s, float down, float m0, float& l, int from, int to) {
+  uint32_t w[2][32];
+  tmem_ld32(t_s, w[0]);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    tmem_ld_wait();
+    if (c < 3) tmem_ld32(t_s + 32 * (c + 1), w[(c + 1) & 1]);
+    const uint32_t(&x)[32] = w[c & 1];
+    uint32_t y[16];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float f = down * sm.fk[slot][2 * c + h], add = sm.lv[slot][2 * c + h] - m0;
+      float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) {
+        float x0 = ex2(__fmaf_rn(__uint_as_float(x[16 * h + e]), f, add));
+        float x1 = ex2(__fmaf_rn(__uint_as_float(x[16 * h + e + 1]), f, add));
+        if (MASKED) {
+          const int at = 32 * c + 16 * h + e;
+          if (at < from || at >= to) x0 = 0.f;
+          if (at + 1 < from || at + 1 >= to) x1 = 0.f;
+        }
+        s0 += x0;
+        s1 += x1;
+        y[8 * h + e / 2] = pack_f16(x0, x1);
+      }
+      l = __fmaf_rn(s0 + s1, sm.rv[slot][2 * c + h], l);
+    }
+    // over columns of S that have been read: 16 c .. 16 c + 15 (the loads in flight are of columns from 32 (c + 1) on)
+    tmem_st16(t_s + 16 * c, y);
+  }
+}
+
 // (sequence, 256 rows, head) items; the last rows of a sequence see the most keys and come first.
 __device__ __forceinline__ long long pre_items(const KvAttendArgs& a, const KvSeq& s) {
   if (s.q < a.min_q || s.q > a.lim_q || s.q == 0) return 0;
@@ -209,27 +276,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_kernel(const KvAtte
       tc_fence_after();
       const int key = key0 + i * kPreKeys, slot = i & (kPreScaleSlots - 1);
       const bool masked = key < from_max || key + kPreKeys > to_min;
-      float top = kNegInf;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t w[32];
-        tmem_ld32(t_s + 32 * c, w);
-        tmem_ld_wait();
-        if (masked) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const int pos = key + 32 * c + e;
-            if (pos < from || pos >= to) w[e] = 0xff800000u;
-          }
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float gm = __uint_as_float(w[16 * h]);
-#pragma unroll
-          for (int e = 1; e < 16; ++e) gm = fmaxf(gm, __uint_as_float(w[16 * h + e]));
-          if (gm > kNegInf && sm.lv[slot][2 * c + h] > kNegInf) top = fmaxf(top, gm * (down * sm.fk[slot][2 * c + h]));
-        }
-      }
+      const float top = masked ? pre_max<D, true>(sm, slot, t_s, down, from - key, to - key) : pre_max<D, false>(sm, slot, t_s, down, 0, 0);
       const bool raise = top > m + kLazyMax;
       if (__any_sync(0xffffffffu, raise)) {
         const float now = fmaxf(m, top);
@@ -253,32 +300,10 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_kernel(const KvAtte
         }
       }
       const float m0 = m == kNegInf ? 0.f : m;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t w[32];
-        tmem_ld32(t_s + 32 * c, w);
-        tmem_ld_wait();
-        uint32_t y[16];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float f = down * sm.fk[slot][2 * c + h], add = sm.lv[slot][2 * c + h] - m0;
-          float sum = 0.f;
-#pragma unroll
-          for (int e = 0; e < 16; e += 2) {
-            float x0 = ex2(__fmaf_rn(__uint_as_float(w[16 * h + e]), f, add));
-            float x1 = ex2(__fmaf_rn(__uint_as_float(w[16 * h + e + 1]), f, add));
-            if (masked) {
-              const int pos = key + 32 * c + 16 * h + e;
-              if (pos < from || pos >= to) x0 = 0.f;
-              if (pos + 1 < from || pos + 1 >= to) x1 = 0.f;
-            }
-            sum += x0 + x1;
-            y[8 * h + e / 2] = pack_f16(x0, x1);
-          }
-          l = __fmaf_rn(sum, sm.rv[slot][2 * c + h], l);
-        }
-        tmem_st16(t_s + 16 * c, y);
-      }
+      if (masked)
+        pre_exp<D, true>(sm, slot, t_s, down, m0, l, from - key, to - key);
+      else
+        pre_exp<D, false>(sm, slot, t_s, down, m0, l, 0, 0);
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(&sm.p_full[tile]);
