@@ -23,7 +23,10 @@
 
 namespace slora {
 
-constexpr int kPreSoftWarps = 8, kPreCvtWarps = 4;
+constexpr int kPreSoftWarps = 8, kPreCvtWarps = 7;  // and one that issues the MMAs
+// Registers of a thread after the roles have parted: 2 x 168 + 2 x 88 for the four groups of four warps, which is what the
+// launch gave them (4 x 128).
+constexpr int kPreSoftRegs = 168, kPreOtherRegs = 88;
 constexpr int kPreThreads = (kPreSoftWarps + kPreCvtWarps + 1) * 32;
 constexpr int kPreKeys = 128;                // keys of a step
 constexpr int kPreRows = 256;                // rows of a CTA
@@ -40,7 +43,7 @@ struct PreSmem {
   uint32_t tmem;
   int bad;
   unsigned vmax;
-  float fk[kPreScaleSlots][kPreGroups], lv[kPreScaleSlots][kPreGroups], rv[kPreScaleSlots][kPreGroups];
+  alignas(16) float fk[kPreScaleSlots][kPreGroups], lv[kPreScaleSlots][kPreGroups], rv[kPreScaleSlots][kPreGroups];
   KvFind find;
 };
 
@@ -117,20 +120,26 @@ __device__ __forceinline__ float pre_max(const PreSmem<D>& sm, int slot, uint32_
   return top;
 }
 
-// p of this thread's row over S (f16 pairs), their sum into l.
+// p of this thread's row as f16 pairs, relative to m0, and their sum; tells whether one passes 2^14 (a score far above m0).
+// The next 32 columns are on their way from tensor memory while 32 are worked on.
 template <int D, bool MASKED>
-__device__ __forceinline__ void pre_exp(const PreSmem<D>& sm, int slot, uint32_t t_s, float down, float m0, float& l, int from, int to) {
+__device__ __forceinline__ bool pre_exp(const PreSmem<D>& sm, int slot, uint32_t t_s, float down, float m0, float* sum, int from, int to,
+                                        uint32_t (&y)[64]) {
   uint32_t w[2][32];
   tmem_ld32(t_s, w[0]);
+  float l = 0.f;
+  uint32_t high = 0;
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
+    const float2 fk = *reinterpret_cast<const float2*>(&sm.fk[slot][2 * c]);
+    const float2 lv = *reinterpret_cast<const float2*>(&sm.lv[slot][2 * c]);
+    const float2 rv = *reinterpret_cast<const float2*>(&sm.rv[slot][2 * c]);
     tmem_ld_wait();
     if (c < 3) tmem_ld32(t_s + 32 * (c + 1), w[(c + 1) & 1]);
     const uint32_t(&x)[32] = w[c & 1];
-    uint32_t y[16];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const float f = down * sm.fk[slot][2 * c + h], add = sm.lv[slot][2 * c + h] - m0;
+      const float f = down * (h ? fk.y : fk.x), add = (h ? lv.y : lv.x) - m0;
       float s0 = 0.f, s1 = 0.f;
 #pragma unroll
       for (int e = 0; e < 16; e += 2) {
@@ -143,13 +152,16 @@ __device__ __forceinline__ void pre_exp(const PreSmem<D>& sm, int slot, uint32_t
         }
         s0 += x0;
         s1 += x1;
-        y[8 * h + e / 2] = pack_f16(x0, x1);
+        const uint32_t p = pack_f16(x0, x1);
+        y[16 * c + 8 * h + e / 2] = p;
+        asm("max.f16x2 %0, %1, %2;" : "=r"(high) : "r"(high), "r"(p));
       }
-      l = __fmaf_rn(s0 + s1, sm.rv[slot][2 * c + h], l);
+      l = __fmaf_rn(s0 + s1, h ? rv.y : rv.x, l);
     }
-    // over columns of S that have been read: 16 c .. 16 c + 15 (the loads in flight are of columns from 32 (c + 1) on)
-    tmem_st16(t_s + 16 * c, y);
   }
+  *sum = l;
+  const float2 top = __half22float2(reinterpret_cast<const __half2&>(high));
+  return fmaxf(top.x, top.y) > 16384.f;
 }
 
 // (sequence, 256 rows, head) items; the last rows of a sequence see the most keys and come first.
@@ -224,6 +236,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_kernel(const KvAtte
   bool ok = true;
 
   if (warp < kPreSoftWarps) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPreSoftRegs));
     // ---- softmax: one thread per row --------------------------------------------------------------------------------
     const int tile = warp >> 2, r = tid & 127;  // warp % 4 is the tensor-memory quarter that the warp may touch
     const int row = row0 + tile * 128 + r;
@@ -276,9 +289,17 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_kernel(const KvAtte
       tc_fence_after();
       const int key = key0 + i * kPreKeys, slot = i & (kPreScaleSlots - 1);
       const bool masked = key < from_max || key + kPreKeys > to_min;
-      const float top = masked ? pre_max<D, true>(sm, slot, t_s, down, from - key, to - key) : pre_max<D, false>(sm, slot, t_s, down, 0, 0);
-      const bool raise = top > m + kLazyMax;
-      if (__any_sync(0xffffffffu, raise)) {
+      uint32_t p[64];
+      float sum = 0.f;
+      // p relative to the maximum so far; only where a score lies far above it (and in the first step) is the maximum taken
+      // anew, O and the sum so far rescaled, and p computed again (S is still there)
+      bool again = i == 0;
+      if (!again)
+        again = masked ? pre_exp<D, true>(sm, slot, t_s, down, m == kNegInf ? 0.f : m, &sum, from - key, to - key, p)
+                       : pre_exp<D, false>(sm, slot, t_s, down, m == kNegInf ? 0.f : m, &sum, 0, 0, p);
+      again = again || m == kNegInf;
+      if (__any_sync(0xffffffffu, again)) {
+        const float top = masked ? pre_max<D, true>(sm, slot, t_s, down, from - key, to - key) : pre_max<D, false>(sm, slot, t_s, down, 0, 0);
         const float now = fmaxf(m, top);
         const float f = now == kNegInf ? 1.f : ex2(m - now);
         m = now;
@@ -298,12 +319,16 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_kernel(const KvAtte
             tmem_st16(t_o + 32 * c + 16, y);
           }
         }
+        pre_exp<D, true>(sm, slot, t_s, down, m == kNegInf ? 0.f : m, &sum, masked ? from - key : 0, masked ? to - key : kPreKeys, p);
       }
-      const float m0 = m == kNegInf ? 0.f : m;
-      if (masked)
-        pre_exp<D, true>(sm, slot, t_s, down, m0, l, from - key, to - key);
-      else
-        pre_exp<D, false>(sm, slot, t_s, down, m0, l, 0, 0);
+      l += sum;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t y[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) y[e] = p[16 * c + e];
+        tmem_st16(t_s + 16 * c, y);
+      }
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(&sm.p_full[tile]);
@@ -337,81 +362,88 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_kernel(const KvAtte
             l == 0.f ? kNegInf : (m + log2f(l)) * 0.69314718055994531f;
       }
     }
-  } else if (warp < kPreSoftWarps + kPreCvtWarps) {
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPreOtherRegs));
+  }
+  if (warp >= kPreSoftWarps && warp < kPreSoftWarps + kPreCvtWarps) {
     // ---- 8-bit pages -> f16 operands ----------------------------------------------------------------------------------
-    // A pass of the 128 threads takes 16 keys (one page: one scale); eight lanes share a key's 128 bytes so that the two
-    // 16-byte chunks of f16 that a lane stores fall on all banks: lanes 0-3 key x, 4-7 key x + 1, first half of d, ...
-    constexpr int kLanes = D / 16;                  // lanes of a key
-    constexpr int kPer = kPreKeys * kLanes / 128;   // 16-byte loads of a thread and operand
-    constexpr int kPassKeys = 128 / kLanes;         // keys of a pass: 16, or 32 for d 64
+    // Unit x of an operand: 16 bytes of a key.  Eight lanes of a store take chunks that fall on all banks: for d 128 units
+    // 0 - 3 the first half of key 2 y, 4 - 7 that of key 2 y + 1, 8 - 15 their second halves.
+    constexpr int kUnits = kPreKeys * (D / 16), kCvtThreads = kPreCvtWarps * 32;
+    constexpr int kPer = (kUnits + kCvtThreads - 1) / kCvtThreads;  // units of a thread and operand
     const int ct = tid - kPreSoftWarps * 32;
     const int l2 = ct & 31, cw = ct >> 5;
-    int sub, key_in;  // which 16 elements, which key of the pass
-    if (D == 128) {
-      sub = (l2 & 3) + ((l2 >> 3) & 1) * 4;
-      key_in = cw * 4 + (l2 >> 4) * 2 + ((l2 >> 2) & 1);
-    } else {
-      sub = l2 & 3;
-      key_in = cw * 8 + (l2 >> 2);
-    }
+    auto unit_key = [&](int x) { return D == 128 ? 2 * (x >> 4) + (x >> 2 & 1) : x >> 2; };
+    auto unit_sub = [&](int x) { return D == 128 ? (x & 3) + (x >> 3 & 1) * 4 : x & 3; };
     const int in_page = (1 << a.c.shift) - 1;
     uint4 kr[kPer], vr[kPer];
-    int64_t page_l = -1;                            // lane g: page * hkv + head of 16-key group g of the step that is loaded next
+    int page_l = -1;  // lane g: page * hkv + head of 16-key group g of the step that is loaded next, its scales
+    float ks_l = 0.f, vs_l = 0.f;
     auto lookup = [&](int i) {
       page_l = -1;
       const int pos = key0 + i * kPreKeys + 16 * (l2 & (kPreGroups - 1));
       if (i < steps && pos < s.kv) {
         const int64_t p = kv_page(a.c, a.b, seq, pos);
-        if (p >= 0) page_l = p * a.c.hkv + head;
-        else set_status(a.b.status, SLORA_STATUS_BAD_TABLE);
+        if (p >= 0) {
+          page_l = static_cast<int>(p * a.c.hkv + head);
+          ks_l = a.c.ks[page_l];
+          vs_l = a.c.vs[page_l];
+        } else {
+          set_status(a.b.status, SLORA_STATUS_BAD_TABLE);
+        }
       }
     };
     auto fetch = [&](int i, const uint8_t* base, uint4 (&regs)[kPer]) {
 #pragma unroll
       for (int p = 0; p < kPer; ++p) {
-        const int key = p * kPassKeys + key_in;
-        const int64_t ph = __shfl_sync(0xffffffffu, page_l, key >> 4);
+        const int x = p * kCvtThreads + ct, key = min(unit_key(x), kPreKeys - 1);
+        const int ph = __shfl_sync(0xffffffffu, page_l, key >> 4);
         regs[p] = make_uint4(0, 0, 0, 0);
         // keys behind the sequence's end may hold anything, NaN bytes among it
-        if (ph >= 0 && key0 + i * kPreKeys + key < s.kv) regs[p] = ld_stream16(base + ((ph << a.c.shift) + ((key0 + i * kPreKeys + key) & in_page)) * D + 16 * sub);
+        if (ph >= 0 && x < kUnits && key0 + i * kPreKeys + key < s.kv)
+          regs[p] = ld_stream16(base + static_cast<int64_t>((ph << a.c.shift) + ((key0 + i * kPreKeys + key) & in_page)) * D + 16 * unit_sub(x));
       }
     };
     auto put = [&](const uint4 (&regs)[kPer], uint8_t* dst) {
 #pragma unroll
       for (int p = 0; p < kPer; ++p) {
-        const int key = p * kPassKeys + key_in;
+        const int u = p * kCvtThreads + ct, key = unit_key(u);
+        if (u >= kUnits) continue;
         const uint32_t x = V8::prepare(regs[p].x), y = V8::prepare(regs[p].y), z = V8::prepare(regs[p].z), w = V8::prepare(regs[p].w);
-        const int c = 2 * sub;
+        const int c = 2 * unit_sub(u);
         uint8_t* row = dst + (c >> 3) * kHalf + key * 128;
         *reinterpret_cast<uint4*>(row + (((c & 7) ^ (key & 7)) << 4)) = make_uint4(V8::lo(x), V8::hi(x), V8::lo(y), V8::hi(y));
         *reinterpret_cast<uint4*>(row + ((((c + 1) & 7) ^ (key & 7)) << 4)) = make_uint4(V8::lo(z), V8::hi(z), V8::lo(w), V8::hi(w));
       }
     };
     lookup(0);
-    int64_t page_now = page_l;
+    int page_now = page_l;
     fetch(0, a.c.k, kr);
     fetch(0, a.c.v, vr);
     for (int i = 0; i < steps && ok; ++i) {
       const int st = i & 1, slot = i & (kPreScaleSlots - 1);
       page_now = page_l;
+      const float ks_now = ks_l, vs_now = vs_l;
       lookup(i + 1);
       if (i >= 2) ok = mbar_wait(&sm.k_empty[st], ((i >> 1) - 1) & 1);
       if (!(ok = __all_sync(0xffffffffu, ok))) break;
-      float vs = 0.f;
-      if (cw == 0 && l2 < kPreGroups) {
+      // lane g of each warp: scales of 16-key group g (lanes 8 and up repeat them)
+      int counts = 1;
+      {
         float f = 0.f, lv = kNegInf, rv = 1.f;
         if (page_now >= 0) {
-          f = a.c.ks[page_now];
-          vs = a.c.vs[page_now];
           // a scale of zero (or next to nothing beside the largest): the values count as zero, p only in the sum
-          const float rel = vs / vmax;
-          const bool some = rel > 1e-30f;
-          lv = (some ? log2f(rel) : 0.f) + 6.f;
-          rv = (some ? 1.f / rel : 1.f) * (1.f / kPreRange);
+          const float rel = vs_now / vmax;
+          counts = rel > 1e-30f;
+          f = ks_now;
+          lv = (counts ? log2f(rel) : 0.f) + 6.f;
+          rv = (counts ? 1.f / rel : 1.f) * (1.f / kPreRange);
         }
-        sm.fk[slot][l2] = f;
-        sm.lv[slot][l2] = lv;
-        sm.rv[slot][l2] = rv;
+        if (cw == 0 && l2 < kPreGroups) {
+          sm.fk[slot][l2] = f;
+          sm.lv[slot][l2] = lv;
+          sm.rv[slot][l2] = rv;
+        }
       }
       put(kr, sm.k[st]);
       fence_proxy_async();
@@ -422,15 +454,15 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_kernel(const KvAtte
       // values of pages whose scale does not count
 #pragma unroll
       for (int p = 0; p < kPer; ++p) {
-        const int64_t ph = __shfl_sync(0xffffffffu, page_now, (p * kPassKeys + key_in) >> 4);
-        if (ph >= 0 && !(a.c.vs[ph] / vmax > 1e-30f)) vr[p] = make_uint4(0, 0, 0, 0);
+        const int group = min(unit_key(p * kCvtThreads + ct), kPreKeys - 1) >> 4;
+        if (__shfl_sync(0xffffffffu, counts, group) == 0) vr[p] = make_uint4(0, 0, 0, 0);
       }
       put(vr, sm.v[st]);
       fence_proxy_async();
       mbar_arrive(&sm.v_full[st]);
       if (i + 1 < steps) fetch(i + 1, a.c.v, vr);
     }
-  } else if (lane == 0 && steps > 0) {
+  } else if (warp == kPreSoftWarps + kPreCvtWarps && lane == 0 && steps > 0) {
     // ---- MMAs -----------------------------------------------------------------------------------------------------
     const uint32_t idesc_s = umma_idesc<__half>(kPreKeys), idesc_o = umma_idesc<__half>(D) | (1u << 16);  // V: outer-major
     auto score = [&](int tile, int st) {
