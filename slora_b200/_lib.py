@@ -185,25 +185,28 @@ def current_stream_ptr() -> int:
     return _C._cuda_getCurrentRawStream(_C._cuda_getDevice())
 
 
-class _Here:
-    def __enter__(self):
-        return self
-
-    def __exit__(self, *exc):
-        return False
-
-
-_HERE_CTX = _Here()
-
-
-def on_device(first, *others):
-    """Context in which the device of ``first`` is the current one.  All tensors must lie on it."""
-    index = first.device.index
-    for t in others:
-        if t is not None and t.device.index != index:
-            raise RuntimeError(f"tensors of one call lie on devices {index} and {t.device.index}")
+def device_of(first, *others):
+    """``None`` when all tensors (``None`` entries aside) lie on the current device; a context that makes theirs current when
+    they lie on another one; an error when they lie on several or on the host."""
     from torch import _C
+    index = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != index:
+            require_cuda(first, t)
+            raise RuntimeError(f"tensors of one call lie on devices {index} and {t.get_device()}")
     if index == _C._cuda_getDevice():
-        return _HERE_CTX
+        return None
+    require_cuda(first)
     import torch
     return torch.cuda.device(index)
+
+
+def call(ctx, fn, *args):
+    """``fn(*args, stream)`` on the current stream of the device that ``ctx`` (of :func:`device_of`) names."""
+    if ctx is None:
+        rc = fn(*args, current_stream_ptr())
+    else:
+        with ctx:
+            rc = fn(*args, current_stream_ptr())
+    if rc != 0:
+        check(rc)

@@ -580,7 +580,8 @@ __global__ void __launch_bounds__(kAttendThreads, NT == 1 && D <= 128 ? 4 : 2) k
             float top = fmaxf(c[nt][x], c[nt][x + 2]);
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-            const float m = fmaxf(st.m[nt][x], top);
+            // only rows that need it: what a row computes does not depend on the others
+            const float m = top > st.m[nt][x] + kLazyMax ? top : st.m[nt][x];
             const float f = ex2(st.m[nt][x] - m);
             st.m[nt][x] = m;
             st.l[nt][x] *= f;

@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_kernel(const KvAtte
       again = again || m == kNegInf;
       if (__any_sync(0xffffffffu, again)) {
         const float top = masked ? pre_max<D, true>(sm, slot, t_s, down, from - key, to - key) : pre_max<D, false>(sm, slot, t_s, down, 0, 0);
-        const float now = fmaxf(m, top);
+        const float now = again ? fmaxf(m, top) : m;  // only rows that need it: a row's p do not depend on the others
         const float f = now == kNegInf ? 1.f : ex2(m - now);
         m = now;
         l *= f;

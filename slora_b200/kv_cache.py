@@ -20,7 +20,7 @@ import torch
 
 from . import _lib
 from .mem_allocator import MemoryAllocator
-from .rotary import LAYOUTS, _positions, _rows
+from .rotary import _positions, _rows
 
 KINDS = {"int8": (torch.int8, _lib.KV_INT8, 127.0), "e4m3": (torch.float8_e4m3fn, _lib.KV_E4M3, 448.0)}
 
@@ -56,6 +56,7 @@ class KvBatch:
                                q_start.data_ptr(), q_len.data_ptr(), self._status.data_ptr(), n, page_table.size(1),
                                self.max_q_len)
         self.ptr = ctypes.addressof(self.c)
+        self.workspaces = {}    # bytes that attention over this batch needs, by the call's sizes
 
     def status(self) -> int:
         """Status bits (``_lib.STATUS_BITS``) of the calls so far -- synchronises the current stream."""
@@ -126,6 +127,7 @@ class KvCache8:
                                 w[i].data_ptr() if w is not None else 0, self.n_pages, self.page_tokens, self.kv_heads,
                                 self.head_dim, KINDS[self.kind][1]) for i in range(self.layer_num)]
         self._ptr = [ctypes.addressof(c) for c in self.c]
+        self._key = (self.kv_heads, self.head_dim, self.page_tokens)
         self._pages = None
 
     # -- pages ------------------------------------------------------------------------------------------
@@ -151,36 +153,40 @@ class KvCache8:
         raises it, the page's older values are rounded to the new scale.  A page that is appended to must belong to one
         sequence only.  C entry ``slora_kv8_append``.
         """
+        d, dtype = self.head_dim, k.dtype
         table = positions = None
-        d = self.head_dim
-        _lib.require_cuda(k, v, q, q_out, self.k[layer])
-        if k.dim() != 3 or k.size(1) != self.kv_heads or k.shape != v.shape or k.dtype != v.dtype:
-            raise RuntimeError(f"k and v must be [tokens, {self.kv_heads}, {d}] tensors of one dtype")
-        _rows(k, "k", d)
-        _rows(v, "v", d)
         if rope is not None:
             table, positions = rope
-            _lib.require_cuda(positions, table.turns)
+        ctx = _lib.device_of(k, v, self.k[layer], batch.kv_len, q, q_out, positions, None if table is None else table.turns)
+        shape, k_stride = _rows(k, "k", d)
+        v_shape, v_stride = _rows(v, "v", d)
+        if shape[1] != self.kv_heads or v_shape != shape or v.dtype != dtype:
+            raise RuntimeError(f"k and v must be [tokens, {self.kv_heads}, {d}] tensors of one dtype")
+        pos = turns = rot = layout = 0
+        factor = 1.0
+        if rope is not None:
             if table.head_dim != d:
                 raise RuntimeError(f"the rotary table is for head_dim {table.head_dim}, the cache has {d}")
-            _positions(positions, k.size(0))
+            _positions(positions, shape[0])
+            pos, turns, rot, factor, layout = positions.data_ptr(), table.turns_ptr, table.rotary_dim, table.factor, table.layout_code
+        qp = qop = q_heads = q_stride = qo_stride = 0
         if q is not None:
             if rope is None:
                 raise RuntimeError("q is only turned: it needs rope=(table, positions)")
-            q_out = q if q_out is None else q_out
-            _rows(q, "q", d)
-            _rows(q_out, "q_out", d)
-            if q.size(0) != k.size(0) or q.dtype != k.dtype or q_out.shape != q.shape or q_out.dtype != q.dtype:
-                raise RuntimeError("q and q_out must have k's tokens and dtype")
+            q_shape, q_stride = _rows(q, "q", d)
+            if q_out is None:
+                q_out, qo_stride = q, q_stride
+            else:
+                out_shape, qo_stride = _rows(q_out, "q_out", d)
+                if out_shape != q_shape or q_out.dtype != dtype:
+                    raise RuntimeError("q_out must have q's shape and dtype")
+            if q_shape[0] != shape[0] or q.dtype != dtype:
+                raise RuntimeError("q must have k's tokens and dtype")
+            qp, qop, q_heads = q.data_ptr(), q_out.data_ptr(), q_shape[1]
         elif q_out is not None:
             raise RuntimeError("q_out without q")
-        with _lib.on_device(k, v, q, q_out, self.k[layer], batch.kv_len, positions, None if table is None else table.turns):
-            _lib.check(_lib.lib.slora_kv8_append(
-                self._ptr[layer], batch.ptr, k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0), k.size(0), _lib.ptr(q),
-                _lib.ptr(q_out), 0 if q is None else q.size(1), 0 if q is None else q.stride(0),
-                0 if q is None else q_out.stride(0), _lib.ptr(positions), 0 if table is None else table.turns.data_ptr(),
-                0 if table is None else table.rotary_dim, 1.0 if table is None else table.factor,
-                0 if table is None else LAYOUTS[table.layout], _lib.dtype_code(k.dtype), _lib.current_stream_ptr()))
+        _lib.call(ctx, _lib.lib.slora_kv8_append, self._ptr[layer], batch.ptr, k.data_ptr(), v.data_ptr(), k_stride, v_stride,
+                  shape[0], qp, qop, q_heads, q_stride, qo_stride, pos, turns, rot, factor, layout, _lib.dtype_code(dtype))
         return q_out
 
     def read(self, layer, batch, dtype, count, first=None):
@@ -189,16 +195,13 @@ class KvCache8:
         code = _lib.dtype_code(dtype)
         if count < 0:
             raise RuntimeError("count must not be negative")
-        if first is not None:
-            _lib.require_cuda(first)
-            if first.dtype != torch.int32 or first.numel() != batch.c.n_seq or not first.is_contiguous():
-                raise RuntimeError("first must be a contiguous int32 tensor with one entry per sequence")
-        shape = (2, batch.c.n_seq, int(count), self.kv_heads, self.head_dim)
-        with _lib.on_device(self.k[layer], batch.kv_len, first):
-            out = torch.empty(shape, dtype=dtype, device=self.device)
-            k, v = out[0], out[1]
-            _lib.check(_lib.lib.slora_kv8_read(self._ptr[layer], batch.ptr, _lib.ptr(first), int(count), k.data_ptr(),
-                                               v.data_ptr(), code, _lib.current_stream_ptr()))
+        ctx = _lib.device_of(self.k[layer], batch.kv_len, first)
+        if first is not None and (first.dtype != torch.int32 or first.numel() != batch.c.n_seq or not first.is_contiguous()):
+            raise RuntimeError("first must be a contiguous int32 tensor with one entry per sequence")
+        shape = (batch.c.n_seq, int(count), self.kv_heads, self.head_dim)
+        k, v = torch.empty(shape, dtype=dtype, device=self.device), torch.empty(shape, dtype=dtype, device=self.device)
+        _lib.call(ctx, _lib.lib.slora_kv8_read, self._ptr[layer], batch.ptr, _lib.ptr(first), int(count), k.data_ptr(), v.data_ptr(),
+                  code)
         return k, v
 
     def attend(self, layer, batch, q, out=None, lse=None, scale=None, window=0, add_weights=False):
@@ -211,33 +214,38 @@ class KvCache8:
         key's attention weight, summed over queries and the heads of its KV head, to ``weights[layer]``.
         C entry ``slora_kv8_attend``.
         """
-        d = self.head_dim
-        _lib.require_cuda(q, out, lse, self.k[layer])
-        _rows(q, "q", d)
-        if q.size(1) % self.kv_heads or q.size(1) == 0:
-            raise RuntimeError(f"q has {q.size(1)} heads, which is no multiple of the cache's {self.kv_heads}")
+        d, dtype = self.head_dim, q.dtype
+        ctx = _lib.device_of(q, self.k[layer], batch.kv_len, out, lse)
+        shape, q_stride = _rows(q, "q", d)
+        tokens, heads = shape[0], shape[1]
+        if heads % self.kv_heads or heads == 0:
+            raise RuntimeError(f"q has {heads} heads, which is no multiple of the cache's {self.kv_heads}")
         if add_weights and self.weights is None:
             raise RuntimeError("add_weights needs a cache with track_weights")
         if window < 0:
             raise RuntimeError("window must not be negative")
-        if out is not None:
-            _rows(out, "out", d)
-            if out.shape != q.shape or out.dtype != q.dtype:
+        code = _lib.dtype_code(dtype)
+        if out is None:
+            out = torch.empty(shape, dtype=dtype, device=q.device)
+            o_stride = heads * d
+        else:
+            out_shape, o_stride = _rows(out, "out", d)
+            if out_shape != shape or out.dtype != dtype:
                 raise RuntimeError("out must have q's shape and dtype")
-        if lse is not None and (lse.dtype != torch.float32 or lse.shape != q.shape[:2] or not lse.is_contiguous()):
+        if lse is not None and (lse.dtype != torch.float32 or lse.shape != (tokens, heads) or not lse.is_contiguous()):
             raise RuntimeError("lse must be a contiguous float32 tensor [tokens, heads]")
-        code = _lib.dtype_code(q.dtype)
-        with _lib.on_device(q, out, lse, self.k[layer], batch.kv_len):
-            if out is None:
-                out = torch.empty_like(q, memory_format=torch.contiguous_format)
-            if q.size(0) == 0 or batch.c.n_seq == 0:
-                return out
-            need = _lib.lib.slora_kv8_attend_workspace_bytes(self._ptr[layer], batch.ptr, q.size(0), q.size(1), int(add_weights))
-            ws = torch.empty((max(need, 16),), dtype=torch.uint8, device=q.device)
-            _lib.check(_lib.lib.slora_kv8_attend(
-                self._ptr[layer], batch.ptr, q.data_ptr(), q.stride(0), q.size(0), q.size(1), out.data_ptr(), out.stride(0),
-                _lib.ptr(lse), d ** -0.5 if scale is None else float(scale), int(window), int(add_weights), ws.data_ptr(),
-                ws.numel(), code, _lib.current_stream_ptr()))
+        if tokens == 0 or batch.c.n_seq == 0:
+            return out
+        # the size follows from the sizes in the key (and the device, which is the cache's)
+        key = (self._key, tokens, heads, bool(add_weights))
+        need = batch.workspaces.get(key)
+        if need is None:
+            need = batch.workspaces[key] = max(_lib.lib.slora_kv8_attend_workspace_bytes(
+                self._ptr[layer], batch.ptr, tokens, heads, int(add_weights)), 16)
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        _lib.call(ctx, _lib.lib.slora_kv8_attend, self._ptr[layer], batch.ptr, q.data_ptr(), q_stride, tokens, heads, out.data_ptr(),
+                  o_stride, _lib.ptr(lse), d ** -0.5 if scale is None else float(scale), int(window), int(add_weights), ws.data_ptr(),
+                  need, code)
         return out
 
     def evict(self, layer, batch, budget, recent, sink=0, dest=None):
@@ -257,9 +265,8 @@ class KvCache8:
             raise RuntimeError("dest must have one row of pages per sequence")
         if budget < 1 or recent < 0 or sink < 0 or recent + sink > budget:
             raise RuntimeError("budget must hold the sink and the recent tokens")
-        with _lib.on_device(self.k[layer], batch.kv_len, table):
-            kept = torch.empty((batch.c.n_seq, self.kv_heads, int(budget)), dtype=torch.int32, device=self.device)
-            _lib.check(_lib.lib.slora_kv8_evict(
-                self._ptr[layer], batch.ptr, int(budget), int(recent), int(sink), kept.data_ptr(), table.data_ptr(),
-                max(table.stride(0), table.size(1)), table.size(1), _lib.current_stream_ptr()))
+        ctx = _lib.device_of(self.k[layer], batch.kv_len, table)
+        kept = torch.empty((batch.c.n_seq, self.kv_heads, int(budget)), dtype=torch.int32, device=self.device)
+        _lib.call(ctx, _lib.lib.slora_kv8_evict, self._ptr[layer], batch.ptr, int(budget), int(recent), int(sink), kept.data_ptr(),
+                  table.data_ptr(), max(table.stride(0), table.size(1)), table.size(1))
         return kept

@@ -104,16 +104,19 @@ class RotaryTable:
         self.inv_freq, self.factor = _frequencies(rotary_dim, float(base), scaling)
         # turns per position: the kernel reduces whole turns away before it goes to 32 bits
         self.turns = torch.tensor([f / (2.0 * math.pi) for f in self.inv_freq], dtype=torch.float64, device=device)
+        self.turns_ptr, self.layout_code = self.turns.data_ptr(), LAYOUTS[layout]
 
 
 def _rows(t, name, head_dim):
-    if t.dim() != 3 or t.size(2) != head_dim or t.stride(2) != 1 or (t.size(1) > 1 and t.stride(1) != head_dim):
+    """Shape of ``t`` ``[tokens, heads, head_dim]``, its heads contiguous, and the stride of its tokens."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or shape[2] != head_dim or stride[2] != 1 or (shape[1] > 1 and stride[1] != head_dim):
         raise RuntimeError(f"{name} must be [tokens, heads, {head_dim}] with contiguous heads")
-    return t
+    return shape, stride[0]
 
 
 def _positions(positions, tokens):
-    if positions.dtype != torch.int64 or positions.dim() != 1 or positions.numel() != tokens or not positions.is_contiguous():
+    if positions.dtype != torch.int64 or positions.shape != (tokens,) or not positions.is_contiguous():
         raise RuntimeError("positions must be a contiguous int64 tensor with one entry per token")
     return positions
 
@@ -124,26 +127,31 @@ def rotary(table, positions, q, k=None, q_out=None, k_out=None, inverse=False):
     In place unless ``q_out`` / ``k_out`` are given; returns ``(q_out, k_out)``.  ``inverse=True`` turns back (the
     gradient's direction).  C entry ``slora_rotary``.
     """
-    _lib.require_cuda(positions, q, k, q_out, k_out, table.turns)
-    d = table.head_dim
-    q_out = q if q_out is None else q_out
-    _rows(q, "q", d)
-    _rows(q_out, "q_out", d)
-    _positions(positions, q.size(0))
-    if q_out.shape != q.shape or q_out.dtype != q.dtype:
-        raise RuntimeError("q_out must have q's shape and dtype")
+    ctx = _lib.device_of(q, positions, table.turns, k, q_out, k_out)
+    d, dtype = table.head_dim, q.dtype
+    shape, q_stride = _rows(q, "q", d)
+    if q_out is None:
+        q_out, qo_stride = q, q_stride
+    else:
+        out_shape, qo_stride = _rows(q_out, "q_out", d)
+        if out_shape != shape or q_out.dtype != dtype:
+            raise RuntimeError("q_out must have q's shape and dtype")
+    _positions(positions, shape[0])
+    k_heads = k_stride = ko_stride = kp = kop = 0
     if k is not None:
-        k_out = k if k_out is None else k_out
-        _rows(k, "k", d)
-        _rows(k_out, "k_out", d)
-        if k.size(0) != q.size(0) or k.dtype != q.dtype or k_out.shape != k.shape or k_out.dtype != k.dtype:
-            raise RuntimeError("k and k_out must have q's tokens and dtype")
+        k_shape, k_stride = _rows(k, "k", d)
+        if k_out is None:
+            k_out, ko_stride = k, k_stride
+        else:
+            out_shape, ko_stride = _rows(k_out, "k_out", d)
+            if out_shape != k_shape or k_out.dtype != dtype:
+                raise RuntimeError("k_out must have k's shape and dtype")
+        if k_shape[0] != shape[0] or k.dtype != dtype:
+            raise RuntimeError("k must have q's tokens and dtype")
+        k_heads, kp, kop = k_shape[1], k.data_ptr(), k_out.data_ptr()
     elif k_out is not None:
         raise RuntimeError("k_out without k")
-    with _lib.on_device(q, positions, k, q_out, k_out, table.turns):
-        _lib.check(_lib.lib.slora_rotary(
-            q_out.data_ptr(), _lib.ptr(k_out), q.data_ptr(), _lib.ptr(k), q.size(0), q.size(1), 0 if k is None else k.size(1),
-            d, table.rotary_dim, q_out.stride(0), 0 if k is None else k_out.stride(0), q.stride(0),
-            0 if k is None else k.stride(0), positions.data_ptr(), table.turns.data_ptr(), table.factor,
-            LAYOUTS[table.layout], int(inverse), _lib.dtype_code(q.dtype), _lib.current_stream_ptr()))
+    _lib.call(ctx, _lib.lib.slora_rotary, q_out.data_ptr(), kop, q.data_ptr(), kp, shape[0], shape[1], k_heads, d,
+              table.rotary_dim, qo_stride, ko_stride, q_stride, k_stride, positions.data_ptr(), table.turns_ptr, table.factor,
+              table.layout_code, int(inverse), _lib.dtype_code(dtype))
     return q_out, k_out
