@@ -47,6 +47,9 @@ constexpr float kPRange = 32.f;        // p * vs / ref * 32 <= 2^8 * 2 * 2^5: in
 constexpr float kNegInf = -INFINITY;
 constexpr float kNoMax = -1e30f;       // maximum of no score: finite, so that differences of maxima are numbers
 
+// CTAs of the attention per SM, by what their registers allow (4 x 128 or 2 x 255; three of 168 spilled: 71 -> 112 us).
+__host__ __device__ constexpr int attend_ctas(int nt, int d) { return nt * d <= 128 ? 4 : 2; }
+
 struct KvAttendArgs {
   KvCache c;
   KvBatch b;
@@ -371,7 +374,7 @@ struct AttendSmem {
 };
 
 template <int D, int NT, int KIND, typename T>
-__global__ void __launch_bounds__(kAttendThreads, NT == 1 && D <= 128 ? 4 : 2) kv_attend_kernel(const __grid_constant__ KvAttendArgs a) {
+__global__ void __launch_bounds__(kAttendThreads, attend_ctas(NT, D)) kv_attend_kernel(const __grid_constant__ KvAttendArgs a) {
   using V8 = Kv8<KIND>;
   extern __shared__ __align__(16) uint8_t smem_raw[];
   AttendSmem<D, NT>& sm = *reinterpret_cast<AttendSmem<D, NT>*>(smem_raw);
@@ -870,21 +873,31 @@ __global__ void __launch_bounds__(kAttendThreads) kv_weights_kernel(const KvAtte
       const int row = rb * a.rows_per_block + lane, j = row / a.group;
       lse_l = a.lse[(static_cast<int64_t>(s.row) + j) * a.hq + head * a.group + row - j * a.group] * 1.4426950408889634f;
     }
-#pragma unroll 4
-    for (int i = max(at - kAttendPiece, 0); i < until - kAttendPiece; ++i) {
-      const int key = (range.lo + i) * kAttendTile;
-      if (key >= s.kv) break;
-      const float* src = a.scores + (base + i) * (a.part_rows * kAttendTile);
-      float sum = 0.f;
-      for (int r0 = 0; r0 < rows; r0 += 2) {
-        const float lse = __shfl_sync(0xffffffffu, lse_l, r0 + half);
-        if (r0 + half < rows && lse > kNegInf) sum += ex2(src[(r0 + half) * kAttendTile + key_in] - lse);
+    // 32 tiles at a time: lane l looks up where tile l's weights are
+    const int end = min(until - kAttendPiece, (s.kv + kAttendTile - 1) / kAttendTile - range.lo);
+    for (int i0 = max(at - kAttendPiece, 0); i0 < end; i0 += 32) {
+      int place = -1;  // token row of the cache
+      const int key_l = (range.lo + i0 + lane) * kAttendTile;
+      if (i0 + lane < end) {
+        const int64_t p = kv_page(a.c, a.b, seq, key_l);
+        if (p >= 0) place = static_cast<int>(((p * a.c.hkv + head) << a.c.shift) + (key_l & ((1 << a.c.shift) - 1)));
       }
-      sum += __shfl_down_sync(0xffffffffu, sum, 16);
-      const int64_t p = kv_page(a.c, a.b, seq, key);
-      // an atomic add only because sequences may share a page; a page of one sequence gets one add per token and row block
-      if (p >= 0 && half == 0 && key + key_in < s.kv && sum != 0.f)
-        atomicAdd(a.c.w + ((p * a.c.hkv + head) << a.c.shift) + ((key + key_in) & ((1 << a.c.shift) - 1)), sum);
+      const int n = min(32, end - i0);
+#pragma unroll 4
+      for (int i = 0; i < n; ++i) {
+        const float* src = a.scores + (base + i0 + i) * (a.part_rows * kAttendTile) + lane;
+        float sum = 0.f;
+#pragma unroll 4
+        for (int r0 = 0; r0 < rows; r0 += 2) {
+          const float lse = __shfl_sync(0xffffffffu, lse_l, r0 + half);
+          const float x = r0 + half < rows ? src[r0 * kAttendTile] : kNegInf;
+          sum += lse > kNegInf ? ex2(x - lse) : 0.f;
+        }
+        sum += __shfl_down_sync(0xffffffffu, sum, 16);
+        const int to = __shfl_sync(0xffffffffu, place, i);
+        // an atomic add only because sequences may share a page; a page of one sequence gets one add per token and row block
+        if (to >= 0 && half == 0 && (range.lo + i0 + i) * kAttendTile + key_in < s.kv && sum != 0.f) atomicAdd(a.c.w + to + key_in, sum);
+      }
     }
   }
 }

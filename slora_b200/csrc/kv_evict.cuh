@@ -69,7 +69,28 @@ __global__ void __launch_bounds__(kSelectThreads) kv_select_kernel(const EvictAr
     }
     return weight_key(a.c.w[((p * a.c.hkv + head) << a.c.shift) + (i & ((1 << a.c.shift) - 1))]);
   };
-  for (int i = c0 + tid; i < c1 && i - c0 < a.cached; i += kSelectThreads) keys[i - c0] = weight_at(i);
+  // four positions a thread and turn: their pages first, then their weights, so that the loads overlap
+  for (int i0 = c0 + tid; i0 < c1 && i0 - c0 < a.cached; i0 += 4 * kSelectThreads) {
+    int place[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = i0 + e * kSelectThreads;
+      place[e] = -1;
+      if (i < c1) {
+        const int64_t p = kv_page(a.c, a.b, seq, i);
+        place[e] = p < 0 ? -2 : static_cast<int>(((p * a.c.hkv + head) << a.c.shift) + (i & ((1 << a.c.shift) - 1)));
+      }
+    }
+    float w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = place[e] >= 0 ? a.c.w[place[e]] : 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = i0 + e * kSelectThreads;
+      if (place[e] == -2) set_status(a.b.status, SLORA_STATUS_BAD_TABLE);
+      if (place[e] != -1 && i - c0 < a.cached) keys[i - c0] = place[e] == -2 ? 0u : weight_key(w[e]);
+    }
+  }
   auto key_at = [&](int i) { return i - c0 < a.cached ? keys[i - c0] : weight_at(i); };
   if (tid == 0) {
     s_prefix = 0;

@@ -198,7 +198,7 @@ int attend_tiles(int max_q, int group, int d) {
   const int most = 256 / d;
   return rows <= 8 || most == 1 ? 1 : rows <= 16 || most == 2 ? 2 : 4;
 }
-int attend_grid(int nt, int d) { return sm_count() * (nt == 1 && d <= 128 ? 4 : 2); }
+int attend_grid(int nt, int d) { return sm_count() * attend_ctas(nt, d); }
 
 // Sequences with at least this many rows go to the tensor-memory kernel (kv_prefill.cuh), the others to kv_attend.cuh.
 constexpr int kPrefillRows = 64;

@@ -24,9 +24,9 @@
 namespace slora {
 
 constexpr int kPreSoftWarps = 8, kPreCvtWarps = 7;  // and one that issues the MMAs
-// Registers of a thread after the roles have parted: 2 x 168 + 2 x 88 for the four groups of four warps, which is what the
+// Registers of a thread after the roles have parted: 2 x 152 + 2 x 104 for the four groups of four warps, which is what the
 // launch gave them (4 x 128).
-constexpr int kPreSoftRegs = 168, kPreOtherRegs = 88;
+constexpr int kPreSoftRegs = 152, kPreOtherRegs = 104;
 constexpr int kPreThreads = (kPreSoftWarps + kPreCvtWarps + 1) * 32;
 constexpr int kPreKeys = 128;                // keys of a step
 constexpr int kPreRows = 256;                // rows of a CTA
@@ -121,12 +121,10 @@ __device__ __forceinline__ float pre_max(const PreSmem<D>& sm, int slot, uint32_
 }
 
 // p of this thread's row as f16 pairs, relative to m0, and their sum; tells whether one passes 2^14 (a score far above m0).
-// The next 32 columns are on their way from tensor memory while 32 are worked on.
 template <int D, bool MASKED>
 __device__ __forceinline__ bool pre_exp(const PreSmem<D>& sm, int slot, uint32_t t_s, float down, float m0, float* sum, int from, int to,
                                         uint32_t (&y)[64]) {
-  uint32_t w[2][32];
-  tmem_ld32(t_s, w[0]);
+  uint32_t x[32];  // (a second buffer, for the columns to come, cost the converters more registers than it saved time)
   float l = 0.f;
   uint32_t high = 0;
 #pragma unroll
@@ -134,9 +132,8 @@ __device__ __forceinline__ bool pre_exp(const PreSmem<D>& sm, int slot, uint32_t
     const float2 fk = *reinterpret_cast<const float2*>(&sm.fk[slot][2 * c]);
     const float2 lv = *reinterpret_cast<const float2*>(&sm.lv[slot][2 * c]);
     const float2 rv = *reinterpret_cast<const float2*>(&sm.rv[slot][2 * c]);
+    tmem_ld32(t_s + 32 * c, x);
     tmem_ld_wait();
-    if (c < 3) tmem_ld32(t_s + 32 * (c + 1), w[(c + 1) & 1]);
-    const uint32_t(&x)[32] = w[c & 1];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const float f = down * (h ? fk.y : fk.x), add = (h ? lv.y : lv.x) - m0;
@@ -379,18 +376,22 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_kernel(const KvAtte
     uint4 kr[kPer], vr[kPer];
     int page_l = -1;  // lane g: page * hkv + head of 16-key group g of the step that is loaded next, its scales
     float ks_l = 0.f, vs_l = 0.f;
-    auto lookup = [&](int i) {
-      page_l = -1;
+    int64_t entry_l = -1;  // the page table's entry for that group of the step after it: loaded a step ahead
+    auto look_up = [&](int i) {
       const int pos = key0 + i * kPreKeys + 16 * (l2 & (kPreGroups - 1));
+      entry_l = -1;
       if (i < steps && pos < s.kv) {
-        const int64_t p = kv_page(a.c, a.b, seq, pos);
-        if (p >= 0) {
-          page_l = static_cast<int>(p * a.c.hkv + head);
-          ks_l = a.c.ks[page_l];
-          vs_l = a.c.vs[page_l];
-        } else {
-          set_status(a.b.status, SLORA_STATUS_BAD_TABLE);
-        }
+        entry_l = a.b.table[seq * a.b.table_stride + (pos >> a.c.shift)];
+        if (entry_l < 0) entry_l = a.c.n_pages;  // told apart from "no keys" below
+      }
+    };
+    auto take_up = [&]() {  // entry_l -> page_l and its scales
+      page_l = -1;
+      if (entry_l >= a.c.n_pages) set_status(a.b.status, SLORA_STATUS_BAD_TABLE);
+      if (entry_l >= 0 && entry_l < a.c.n_pages) {
+        page_l = static_cast<int>(entry_l * a.c.hkv + head);
+        ks_l = a.c.ks[page_l];
+        vs_l = a.c.vs[page_l];
       }
     };
     auto fetch = [&](int i, const uint8_t* base, uint4 (&regs)[kPer]) {
@@ -416,7 +417,9 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_kernel(const KvAtte
         *reinterpret_cast<uint4*>(row + ((((c + 1) & 7) ^ (key & 7)) << 4)) = make_uint4(V8::lo(z), V8::hi(z), V8::lo(w), V8::hi(w));
       }
     };
-    lookup(0);
+    look_up(0);
+    take_up();
+    look_up(1);
     int page_now = page_l;
     fetch(0, a.c.k, kr);
     fetch(0, a.c.v, vr);
@@ -424,7 +427,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_kernel(const KvAtte
       const int st = i & 1, slot = i & (kPreScaleSlots - 1);
       page_now = page_l;
       const float ks_now = ks_l, vs_now = vs_l;
-      lookup(i + 1);
+      take_up();
+      look_up(i + 2);
       if (i >= 2) ok = mbar_wait(&sm.k_empty[st], ((i >> 1) - 1) & 1);
       if (!(ok = __all_sync(0xffffffffu, ok))) break;
       // lane g of each warp: scales of 16-key group g (lanes 8 and up repeat them)
