@@ -514,6 +514,7 @@ int slora_rotary(void* q_out, void* k_out, const void* q, const void* k, int64_t
  * values q become round(q * s_old / s_new); a scale below FP32's smallest normal number counts as 0.  Rounding is to nearest, ties to even, of the exact quotient.  NaN is stored as
  * 0 and infinities as the largest value (both leave the scale alone) with SLORA_STATUS_NONFINITE.  weights of new
  * tokens, where the cache has them, become 0.  Positions beyond kv_len of the last page are left as they are.
+ * A page that is appended to must belong to one sequence.
  */
 #define SLORA_STATUS_NONFINITE 16 /* a NaN or an infinity was appended to an 8-bit cache */
 int slora_kv8_append(const slora_kv8_cache* cache, const slora_kv8_batch* batch, const void* k, const void* v,
@@ -551,7 +552,7 @@ int slora_kv8_attend(const slora_kv8_cache* cache, const slora_kv8_batch* batch,
  * dest_stride entries apart; the batch's own page table: in place), their weights with them.  A destination page whose
  * tokens all keep their position is copied as it is; every other gets the scale max |value| / top of its tokens
  * and the values round(q * s_old / s_new) (as slora_kv8_append).  Destination pages must be disjoint from all source
- * pages, or the batch's own table.  The sequences' new length is min(kv_len, budget).
+ * pages, or the batch's own table; in place a page must belong to one sequence.  The sequences' new length is min(kv_len, budget).
  */
 int slora_kv8_evict(const slora_kv8_cache* cache, const slora_kv8_batch* batch, int budget, int recent, int sink,
                     int32_t* kept, const int64_t* dest_table, int64_t dest_stride, int dest_pages, void* stream);

@@ -253,7 +253,8 @@ class KvCache8:
 
         Kept are the first ``sink`` tokens, the last ``recent`` and, of the others, those with the largest ``weights``
         (ties: the lowest position); they move, in order, to the front of the sequence's own pages, or to the pages of
-        ``dest`` (a :class:`KvBatch` whose ``page_table`` names pages that no sequence of ``batch`` uses).  Returns the kept
+        ``dest`` (a :class:`KvBatch` whose ``page_table`` names pages that no sequence of ``batch`` uses).  In place a page must
+        belong to one sequence.  Returns the kept
         positions, int32 ``[n, kv_heads, budget]``, -1 behind the last.  The caller's lengths become
         ``min(kv_len, budget)`` and the pages behind them are free; all layers must be brought back alike.
         C entry ``slora_kv8_evict``.

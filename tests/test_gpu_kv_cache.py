@@ -323,6 +323,45 @@ def test_empty_batches():
     assert (idle.cache.attend(0, idle.batch, q, out=out) == 7.0).all()
 
 
+def test_sequences_that_share_a_prefix():
+    """Two sequences whose first pages are the same: both read them, and their weights gather both sequences' attention."""
+    w = World([70, 90, 40], [1, 1, 1], 2, 64, 16, "int8")
+    w.table[1, :3] = w.table[0, :3]
+    w.batch.page_table.copy_(w.table)
+    q = torch.randn(w.T, 4, 64, device=DEV).half()
+    before = w.w.clone()
+    out = w.cache.attend(0, w.batch, q, out=torch.zeros_like(q), add_weights=True)
+    _check_attend(w, q, out, None, None, None)
+    want = before.double()
+    for i, (n, r) in enumerate(zip(w.lens, w.starts)):
+        k = ref.dense(ref.values(w.k8), w.ks.double(), w.table[i], n)
+        v = ref.dense(ref.values(w.v8), w.vs.double(), w.table[i], n)
+        p = ref.attend(k, v, q[r:r + 1].double(), 0, 64 ** -0.5)[2]
+        for pos in range(n):
+            want[int(w.table[i, pos // 16]), :, pos % 16] += p[:, pos]
+    assert ((w.w.double() - want).abs() <= 2.0 ** -16 * (want + 1)).all()
+
+
+@pytest.mark.parametrize("new", [1, 130])
+def test_negative_and_zero_scale(new):
+    w = World([200, 131], [new, new], 2, 128, 32, "e4m3")
+    for scale in (-0.2, 0.0):
+        q = torch.randn(w.T, 4, 128, device=DEV).half()
+        out = w.cache.attend(0, w.batch, q, scale=scale)
+        own = w.own_rows()
+        full = torch.zeros_like(q)
+        full[own] = out[own]
+        for i, (n, m, r0) in enumerate(zip(w.lens, w.new, w.starts)):
+            k = ref.dense(ref.values(w.k8), w.ks.double(), w.table[i], n)
+            v = ref.dense(ref.values(w.v8), w.vs.double(), w.table[i], n)
+            o, _, _, mag, _ = ref.attend(k, v, q[r0:r0 + m].double(), 0, scale)
+            # as in _check_attend, with the size of the scores from |scale|
+            size = float((q[r0:r0 + m].double().abs().sum(-1).max() * k.abs().max()) * abs(scale))
+            ds = 2.0 ** -22 * 16 * size
+            tol = 2.0 ** -11 * o.abs() + (2.0 ** -11 + 4 * ds + 2.0 ** -19) * mag + 2.0 ** -25 + n * 2.0 ** -29 * float(v.abs().max())
+            assert bool(((full[r0:r0 + m].double() - o).abs() <= tol).all())
+
+
 def test_pages_beyond_four_gigabytes():
     # 2^32 bytes lie between the first and the last page
     sl = _sl()
