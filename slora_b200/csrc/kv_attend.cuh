@@ -17,7 +17,7 @@
 //                                               words by byte permutes, which the conversion to f16 needs anyway.
 // P^T is the transpose of S^T's accumulator layout: one movmatrix per 8 x 8.  q is scaled by a power of two per row into
 // f16's upper range, the 8-bit values are exact in f16 and so are their products in FP32: the only rounding before the
-// sums is p's to f16 (2^-12 relative in the mean).  p is multiplied by vs (relative to a running power of two, so its f16
+// sums is p's to f16 (2^-12 relative in the mean; for f16 outputs p goes in as two f16 numbers).  p is multiplied by vs (relative to a running power of two, so its f16
 // range holds for any scales) and the maximum is only raised when some score passes it by 2^8: no shuffles in most steps.
 //
 // Work is split over the whole batch at once: the tiles of every (sequence, row block, KV head) in one row, cut into runs
@@ -32,6 +32,8 @@
 // against the 2 d that the key cost) and kv_weights_kernel adds up their exponentials; where that would take too much
 // memory or the rows are many, kv_reweigh_kernel computes the scores again.
 #pragma once
+
+#include <type_traits>
 
 #include "kv_common.cuh"
 
@@ -376,6 +378,9 @@ struct AttendSmem {
 template <int D, int NT, int KIND, typename T>
 __global__ void __launch_bounds__(kAttendThreads, attend_ctas(NT, D)) kv_attend_kernel(const __grid_constant__ KvAttendArgs a) {
   using V8 = Kv8<KIND>;
+  // f16 outputs show p's rounding to f16 (1.4 to 1.6 times the error of their own): there p goes in as two f16 numbers.
+  // bf16 outputs, eight times coarser, do not.
+  constexpr bool kTwoParts = std::is_same<T, __half>::value;
   extern __shared__ __align__(16) uint8_t smem_raw[];
   AttendSmem<D, NT>& sm = *reinterpret_cast<AttendSmem<D, NT>*>(smem_raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -596,15 +601,21 @@ __global__ void __launch_bounds__(kAttendThreads, attend_ctas(NT, D)) kv_attend_
           }
       }
       const float pv = vs * w_scale;
-      uint32_t p[NT][2];
+      uint32_t p[NT][2], p_lo[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const float e0 = ex2(c[nt][0] - st.m[nt][0]), e1 = ex2(c[nt][1] - st.m[nt][1]);
         const float e2 = ex2(c[nt][2] - st.m[nt][0]), e3 = ex2(c[nt][3] - st.m[nt][1]);
         st.l[nt][0] += e0 + e2;
         st.l[nt][1] += e1 + e3;
-        p[nt][0] = transpose8x8(pack_f16(e0 * pv, e1 * pv));
-        p[nt][1] = transpose8x8(pack_f16(e2 * pv, e3 * pv));
+        const uint32_t h0 = pack_f16(e0 * pv, e1 * pv), h1 = pack_f16(e2 * pv, e3 * pv);
+        p[nt][0] = transpose8x8(h0);
+        p[nt][1] = transpose8x8(h1);
+        if (kTwoParts) {
+          const float2 f0 = __half22float2(reinterpret_cast<const __half2&>(h0)), f1 = __half22float2(reinterpret_cast<const __half2&>(h1));
+          p_lo[nt][0] = transpose8x8(pack_f16(__fmaf_rn(e0, pv, -f0.x), __fmaf_rn(e1, pv, -f0.y)));
+          p_lo[nt][1] = transpose8x8(pack_f16(__fmaf_rn(e2, pv, -f1.x), __fmaf_rn(e3, pv, -f1.y)));
+        }
       }
 #pragma unroll
       for (int x = 0; x < VTile<D>::N; ++x) {
@@ -618,6 +629,10 @@ __global__ void __launch_bounds__(kAttendThreads, attend_ctas(NT, D)) kv_attend_
         for (int nt = 0; nt < NT; ++nt) {
           mma_f16(st.o[nt][2 * x], a0, a1, a2, a3, p[nt][0], p[nt][1]);
           mma_f16(st.o[nt][2 * x + 1], b0, b1, b2, b3, p[nt][0], p[nt][1]);
+          if (kTwoParts) {
+            mma_f16(st.o[nt][2 * x], a0, a1, a2, a3, p_lo[nt][0], p_lo[nt][1]);
+            mma_f16(st.o[nt][2 * x + 1], b0, b1, b2, b3, p_lo[nt][0], p_lo[nt][1]);
+          }
         }
       }
       if (next >= 0) v.load(a.c.v + off, g, t);
