@@ -91,10 +91,23 @@ struct RotaryLane {
   int other;  // half layout: lane with the partners
   bool in;    // these elements turn
   __device__ __forceinline__ void load(const float2* cs, int sub, int rot, int layout) {
+    if (layout == 0)
+      load_as<0>(cs, sub, rot);
+    else
+      load_as<1>(cs, sub, rot);
+  }
+  __device__ __forceinline__ void turn(float (&x)[8], int layout) const {  // all lanes of the warp take part
+    if (layout == 0)
+      turn_as<0>(x);
+    else
+      turn_as<1>(x);
+  }
+  template <int LAYOUT>
+  __device__ __forceinline__ void load_as(const float2* cs, int sub, int rot) {
     const int lane = threadIdx.x & 31;
     other = lane;
     in = 8 * sub < rot;
-    if (layout == 0) {
+    if (LAYOUT == 0) {
       const int far = rot >> 4;  // lanes between the partners
       const bool low = sub < far;
       if (in) other = low ? lane + far : lane - far;
@@ -116,9 +129,9 @@ struct RotaryLane {
       }
     }
   }
-  // all lanes of the warp take part
-  __device__ __forceinline__ void turn(float (&x)[8], int layout) const {
-    if (layout == 0) {
+  template <int LAYOUT>
+  __device__ __forceinline__ void turn_as(float (&x)[8]) const {
+    if (LAYOUT == 0) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float y = __shfl_sync(0xffffffffu, x[e], other);
@@ -165,8 +178,8 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
 // Heads [h0, h1) of tokens [t0, t0 + n): turned rows src -> dst.  A warp takes a token and a few heads at a time: the
 // token's cosines stay in registers, and kRowUnroll loads of 512 bytes are in flight.
 constexpr int kRowUnroll = 4;
-template <int D, typename T>
-__device__ __forceinline__ void rotary_rows(const RotaryArgs& r, const T* src, T* dst, int64_t src_stride, int64_t dst_stride,
+template <int D, typename T, int LAYOUT>
+__device__ __forceinline__ void rotary_rows_as(const RotaryArgs& r, const T* src, T* dst, int64_t src_stride, int64_t dst_stride,
                                             int64_t t0, int n, int h0, int h1, const float2* cs) {
   constexpr int kLanes = D / 8, kRows = 32 / kLanes, kHeads = kRows * kRowUnroll;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % kLanes, rr = lane / kLanes;
@@ -182,15 +195,24 @@ __device__ __forceinline__ void rotary_rows(const RotaryArgs& r, const T* src, T
       if (h + u * kRows < h1) raw[u] = *reinterpret_cast<const uint4*>(from + (h + u * kRows) * D);
     }
     RotaryLane w;
-    w.load(cs + t * half, sub, r.rot, r.layout);
+    w.load_as<LAYOUT>(cs + t * half, sub, r.rot);
 #pragma unroll
     for (int u = 0; u < kRowUnroll; ++u) {
       float x[8];
       cvt8<T>(raw[u], x);
-      w.turn(x, r.layout);
+      w.turn_as<LAYOUT>(x);
       if (h + u * kRows < h1) store8<T>(to + (h + u * kRows) * D, x);
     }
   }
+}
+
+template <int D, typename T>
+__device__ __forceinline__ void rotary_rows(const RotaryArgs& r, const T* src, T* dst, int64_t src_stride, int64_t dst_stride,
+                                            int64_t t0, int n, int h0, int h1, const float2* cs) {
+  if (r.layout == 0)
+    rotary_rows_as<D, T, 0>(r, src, dst, src_stride, dst_stride, t0, n, h0, h1, cs);
+  else
+    rotary_rows_as<D, T, 1>(r, src, dst, src_stride, dst_stride, t0, n, h0, h1, cs);
 }
 
 template <int D, typename T>
