@@ -550,48 +550,75 @@ struct ReadArgs {
   void* out[2];
 };
 
-// Cached values back to 16 bits: a warp takes rows (token, head) of one sequence, k and v; eight elements a lane.
+// Cached values back to 16 bits: a warp takes kReadAhead rows a half warp (eight heads at d 128) of one token, with one look at
+// its page, eight elements a lane, and has all their k and v on their way at once. 8191 tokens of 8 heads: 17 -> 14 us against
+// a warp per token and head.
+constexpr int kReadAhead = 4;
 template <int D, int KIND, typename T>
 __global__ void __launch_bounds__(kRowThreads) kv_read_kernel(const ReadArgs a) {
-  constexpr int kLanes = D / 8, kRows = 32 / kLanes;
+  constexpr int kLanes = D / 8, kRows = 32 / kLanes, kGroup = kReadAhead * kRows;
   pdl_launch_dependents();
   pdl_wait();
-  const int lane = threadIdx.x & 31, sub = lane % kLanes;
-  const int64_t rows = a.b.n_seq * a.count * a.c.hkv;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * kRowWarps * kRows;
-  for (int64_t i = (static_cast<int64_t>(blockIdx.x) * kRowWarps + (threadIdx.x >> 5)) * kRows + lane / kLanes; i < rows; i += step) {
-    // row -> token, head; token -> sequence (32-bit divisions unless there are more rows than that)
-    const int64_t token = rows <= 0xffffffffll ? static_cast<uint32_t>(i) / static_cast<uint32_t>(a.c.hkv) : i / a.c.hkv;
-    const int h = static_cast<int>(i - token * a.c.hkv);
-    const int seq = static_cast<int>(rows <= 0xffffffffll ? static_cast<uint32_t>(token) / static_cast<uint32_t>(a.count) : token / a.count);
+  const int lane = threadIdx.x & 31, sub = lane % kLanes, rr = lane / kLanes;
+  const int groups = (a.c.hkv + kGroup - 1) / kGroup;
+  const int64_t units = a.b.n_seq * a.count * groups;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kRowWarps;
+  for (int64_t unit = static_cast<int64_t>(blockIdx.x) * kRowWarps + (threadIdx.x >> 5); unit < units; unit += step) {
+    int64_t token, seq64;
+    int group;
+    if (units <= 0xffffffffll) {
+      token = static_cast<uint32_t>(unit) / static_cast<uint32_t>(groups);
+      seq64 = static_cast<uint32_t>(token) / static_cast<uint32_t>(a.count);
+    } else {
+      token = unit / groups;
+      seq64 = token / a.count;
+    }
+    group = static_cast<int>(unit - token * groups);
+    const int seq = static_cast<int>(seq64);
     const int64_t pos = token - seq * a.count + (a.first ? a.first[seq] : 0);
     int kv = a.b.kv_len[seq];
     if (kv < 0 || kv > a.b.max_tokens) {
-      if (sub == 0) set_status(a.b.status, SLORA_STATUS_BAD_TABLE);
+      if (lane == 0) set_status(a.b.status, SLORA_STATUS_BAD_TABLE);
       kv = 0;
     }
     int64_t p = -1;
     if (pos >= 0 && pos < kv) {
       p = kv_page(a.c, a.b, seq, static_cast<int>(pos));
-      if (p < 0 && sub == 0) set_status(a.b.status, SLORA_STATUS_BAD_TABLE);
+      if (p < 0 && lane == 0) set_status(a.b.status, SLORA_STATUS_BAD_TABLE);
+    }
+    const int slot = static_cast<int>(pos & ((1 << a.c.shift) - 1));
+    T* const out[2] = {static_cast<T*>(a.out[0]) + token * a.c.hkv * D + 8 * sub, static_cast<T*>(a.out[1]) + token * a.c.hkv * D + 8 * sub};
+    const int h0 = group * kGroup + rr;
+    uint2 v[kReadAhead][2];
+    float s[kReadAhead][2];
+#pragma unroll
+    for (int u = 0; u < kReadAhead; ++u) {
+      const int h = h0 + u * kRows;
+      v[u][0] = v[u][1] = make_uint2(0, 0);
+      s[u][0] = s[u][1] = 0.f;
+      if (p >= 0 && h < a.c.hkv) {
+        const int64_t ph = p * a.c.hkv + h, at = ((ph << a.c.shift) + slot) * D + 8 * sub;
+        v[u][0] = *reinterpret_cast<const uint2*>(a.c.k + at);
+        v[u][1] = *reinterpret_cast<const uint2*>(a.c.v + at);
+        s[u][0] = a.c.ks[ph];
+        s[u][1] = a.c.vs[ph];
+      }
     }
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (p >= 0) {
-        const int64_t ph = p * a.c.hkv + h;
-        const uint8_t* src = (w ? a.c.v : a.c.k) + ((ph << a.c.shift) + (pos & ((1 << a.c.shift) - 1))) * D + 8 * sub;
-        const uint2 v = *reinterpret_cast<const uint2*>(src);
-        const float s = (w ? a.c.vs : a.c.ks)[ph];
-        float q[4];
-        Kv8<KIND>::values(v.x, q);
+    for (int u = 0; u < kReadAhead; ++u) {
+      const int h = h0 + u * kRows;
+      if (h >= a.c.hkv) break;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = q[e] * s;
-        Kv8<KIND>::values(v.y, q);
+      for (int w = 0; w < 2; ++w) {
+        float x[8], q[4];
+        Kv8<KIND>::values(v[u][w].x, q);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[4 + e] = q[e] * s;
+        for (int e = 0; e < 4; ++e) x[e] = q[e] * s[u][w];
+        Kv8<KIND>::values(v[u][w].y, q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[4 + e] = q[e] * s[u][w];
+        store8<T>(out[w] + h * D, x);
       }
-      store8<T>(static_cast<T*>(a.out[w]) + i * D + 8 * sub, x);
     }
   }
 }

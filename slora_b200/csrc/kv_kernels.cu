@@ -420,8 +420,8 @@ int slora_kv8_read(const slora_kv8_cache* cache, const slora_kv8_batch* batch, c
   a.count = count;
   a.out[0] = k_out;
   a.out[1] = v_out;
-  const int64_t rows = count * a.b.n_seq * a.c.hkv, per = kRowWarps * (256 / a.c.d);
-  const int64_t blocks = (rows + per - 1) / per, most = 8ll * sm_count();
+  const int64_t group = kReadAhead * (256 / a.c.d), units = count * a.b.n_seq * ((a.c.hkv + group - 1) / group);
+  const int64_t blocks = (units + kRowWarps - 1) / kRowWarps, most = 8ll * sm_count();
   const int grid = static_cast<int>(blocks < most ? blocks : most);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return KV_DISPATCH(a.c.d, cache->kind, dtype, (read_launch<D, KIND, T>(a, grid, s)));
