@@ -5,11 +5,16 @@
 // the remainder goes to sincospif.  Cosines and sines of a block of tokens are worked out once, in shared memory, and
 // serve all heads.  A row of a head is 8 elements a lane (16-byte loads and stores); in the half layout the partner of a
 // value sits rot / 16 lanes away (one shuffle per element), in the interleaved layout in the same lane.
-// What bounds it: q, k read and written once (16-bit), at the copy rate; one token: launch and one chain of loads.
+// What bounds it: q, k read and written once (16-bit), at the copy rate: 8191 tokens of 64 + 8 heads of 128, half of each turned: 53 us, 0.87
+// of it.  One token: 9 us, all of them the call's and the launch's.
 //
 // Append: the new tokens of one page belong to one CTA (the scale of a (page, head) is a maximum over them): all warps take
 // a (head, k or v) together when there are many tokens, one warp each when there are few (decode).  When the scale grows,
-// the page's older values are rounded to the new one in place.
+// the page's older values are rounded to the new one in place.  Pages with more than kAppendWarpTokens new tokens take two
+// launches, q by tokens and k, v by heads: one kernel for both had too many registers and instructions (236 against 152 us
+// then, 7983 tokens of 64 + 8 + 8 heads of 128; now 50 and 73 us).  What bounds it there is instructions (angles, exact
+// rounding) and the barriers of the two walks over a page; at decode a chain of loads: length, table, scale, values (77
+// sequences of 32 heads: 16 us).
 #pragma once
 
 #include "kv_common.cuh"
@@ -551,7 +556,7 @@ struct ReadArgs {
 };
 
 // Cached values back to 16 bits: a warp takes kReadAhead rows a half warp (eight heads at d 128) of one token, with one look at
-// its page, eight elements a lane, and has all their k and v on their way at once. 8191 tokens of 8 heads: 17 -> 14 us against
+// its page, eight elements a lane, and has all their k and v on their way at once. 7983 tokens of 8 heads: 17 -> 14 us against
 // a warp per token and head.
 constexpr int kReadAhead = 4;
 template <int D, int KIND, typename T>

@@ -17,8 +17,9 @@
 //                                               words by byte permutes, which the conversion to f16 needs anyway.
 // P^T is the transpose of S^T's accumulator layout: one movmatrix per 8 x 8.  q is scaled by a power of two per row into
 // f16's upper range, the 8-bit values are exact in f16 and so are their products in FP32: the only rounding before the
-// sums is p's to f16 (2^-12 relative in the mean; for f16 outputs p goes in as two f16 numbers).  p is multiplied by vs (relative to a running power of two, so its f16
-// range holds for any scales) and the maximum is only raised when some score passes it by 2^8: no shuffles in most steps.
+// sums is p's to f16 (2^-12 relative in the mean; for f16 outputs p goes in as two f16 numbers).  p is multiplied by vs
+// (relative to a running power of two, so its f16 range holds for any scales) and the maximum is only raised when some score
+// passes it by 2^8: no shuffles in most steps.
 //
 // Work is split over the whole batch at once: the tiles of every (sequence, row block, KV head) in one row, cut into runs
 // of equal cost, one per CTA (a piece costs kAttendPiece tiles before its first key: its q, its page table, its output).
@@ -27,6 +28,11 @@
 // first tiles are on their way.  Every CTA adds up the lengths itself (one round trip for a few hundred sequences), so
 // there is no plan to build or to keep.  A run that ends inside a (sequence, rows, head) leaves its part in the workspace
 // and kv_join_kernel adds the parts in order: results do not depend on timing.
+//
+// Measured (d 128): 16 sequences of 8271 to 46873 tokens, 64 q heads on 8, 681 MB of cache: 130 us with the join, 0.8 of the
+// copy rate; 64 sequences of 65 to 3955 tokens, 32 heads on 32, f16, 491 MB: 115 us, 0.65 (2048 pieces: their starts, and
+// the instructions of 16 warps per SM);
+// one short sequence: 15.5 us, two launches and some 7 us from the first load to the first product.
 //
 // Attention weights (add_weights) need the softmax's sum first: the scores go to the workspace (4 bytes per key and row,
 // against the 2 d that the key cost) and kv_weights_kernel adds up their exponentials; where that would take too much

@@ -496,7 +496,7 @@ int slora_kv8_evict(const slora_kv8_cache* cache, const slora_kv8_batch* batch, 
   a.dest = dest_table;
   a.dest_stride = dest_stride;
   a.in_place = dest_table == batch->page_table;
-  // 12288 weights in shared memory (48 KB) leave two CTAs per SM; longer rests are read again in each pass
+  // 40960 weights are what a CTA's shared memory takes (160 KB); a longer sequence's rest is read again in each pass
   a.cached = static_cast<int>(a.b.max_tokens < 40960 ? a.b.max_tokens : 40960);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (int rc = launch_pdl<kv_select_kernel>(dim3(static_cast<unsigned>(heads)), kSelectThreads,

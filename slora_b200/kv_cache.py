@@ -25,36 +25,42 @@ from .rotary import _positions, _rows
 KINDS = {"int8": (torch.int8, _lib.KV_INT8, 127.0), "e4m3": (torch.float8_e4m3fn, _lib.KV_E4M3, 448.0)}
 
 
+def _table_stride(t):
+    """Entries from one row of a page table to the next."""
+    if t.dtype != torch.int64 or t.dim() != 2 or (t.size(1) > 1 and t.stride(1) != 1):
+        raise RuntimeError("page_table must be an int64 tensor [sequences, pages] with contiguous rows")
+    if t.size(0) > 1 and t.stride(0) < t.size(1):
+        raise RuntimeError("the rows of page_table overlap (an expanded tensor?)")
+    return max(t.stride(0), t.size(1))
+
+
 class KvBatch:
     """The sequences of one step, as device tables; made once per step and used by every layer.
 
     ``page_table`` int64 ``[n, max_pages]`` (entries behind a sequence's last page are not read); ``kv_len`` int32
     ``[n]``: tokens in the cache, the step's new ones included; ``q_start`` / ``q_len`` int32 ``[n]``: the rows of q, k and
     v that are the sequence's new tokens (the reference's ``b_start_loc`` / ``b_seq_len``).  ``max_q_len`` bounds
-    ``q_len`` (as ``max_len_in_batch`` does in the reference; it sizes launches), ``max_kv_len``, when given, ``kv_len``.
+    ``q_len`` (as ``max_len_in_batch`` does in the reference; it sizes launches).
 
     The kernels check every length and page; what they had to skip is in :meth:`status`.
     """
 
-    def __init__(self, page_table, kv_len, q_start, q_len, max_q_len, max_kv_len=None):
+    def __init__(self, page_table, kv_len, q_start, q_len, max_q_len):
         _lib.require_cuda(page_table, kv_len, q_start, q_len)
-        if page_table.dtype != torch.int64 or page_table.dim() != 2 or (page_table.size(1) > 1 and page_table.stride(1) != 1):
-            raise RuntimeError("page_table must be an int64 tensor [sequences, pages] with contiguous rows")
+        stride = _table_stride(page_table)
         n = page_table.size(0)
         for name, t in (("kv_len", kv_len), ("q_start", q_start), ("q_len", q_len)):
             if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
                 raise RuntimeError(f"{name} must be a contiguous int32 tensor with one entry per sequence")
             if t.device != page_table.device:
                 raise RuntimeError(f"{name} and page_table lie on different devices")
-        if max_q_len < 0 or (max_kv_len is not None and max_kv_len < 0):
-            raise RuntimeError("max_q_len and max_kv_len must not be negative")
+        if max_q_len < 0:
+            raise RuntimeError("max_q_len must not be negative")
         self.page_table, self.kv_len, self.q_start, self.q_len = page_table, kv_len, q_start, q_len
         self.max_q_len = int(max_q_len)
-        self.max_kv_len = None if max_kv_len is None else int(max_kv_len)
         self._status = torch.zeros((1,), dtype=torch.int32, device=page_table.device)
-        self.c = _lib.Kv8Batch(page_table.data_ptr(), max(page_table.stride(0), page_table.size(1)), kv_len.data_ptr(),
-                               q_start.data_ptr(), q_len.data_ptr(), self._status.data_ptr(), n, page_table.size(1),
-                               self.max_q_len)
+        self.c = _lib.Kv8Batch(page_table.data_ptr(), stride, kv_len.data_ptr(), q_start.data_ptr(),
+                               q_len.data_ptr(), self._status.data_ptr(), n, page_table.size(1), self.max_q_len)
         self.ptr = ctypes.addressof(self.c)
         self.workspaces = {}    # bytes that attention over this batch needs, by the call's sizes
 
@@ -269,5 +275,5 @@ class KvCache8:
         ctx = _lib.device_of(self.k[layer], batch.kv_len, table)
         kept = torch.empty((batch.c.n_seq, self.kv_heads, int(budget)), dtype=torch.int32, device=self.device)
         _lib.call(ctx, _lib.lib.slora_kv8_evict, self._ptr[layer], batch.ptr, int(budget), int(recent), int(sink), kept.data_ptr(),
-                  table.data_ptr(), max(table.stride(0), table.size(1)), table.size(1))
+                  table.data_ptr(), _table_stride(table), table.size(1))
         return kept

@@ -179,3 +179,16 @@ def test_rotary_frequencies():
     for a, b in zip(base.inv_freq, l3.inv_freq):
         wave = 2 * math.pi / a
         assert math.isclose(b, a) if wave < 2048 else math.isclose(b, a / 8) if wave > 8192 else a / 8 <= b <= a
+
+
+def test_page_tables_whose_rows_overlap_are_refused():
+    from slora_b200.kv_cache import _table_stride
+    t = torch.arange(12).view(3, 4)
+    assert _table_stride(t) == 4 and _table_stride(t[:, :2]) == 4 and _table_stride(t[:1].expand(1, 4)) == 4
+    for bad in (t[:1].expand(3, 4), t.view(-1).as_strided((3, 4), (2, 1))):
+        with pytest.raises(RuntimeError, match="overlap"):
+            _table_stride(bad)
+    with pytest.raises(RuntimeError, match="contiguous rows"):
+        _table_stride(t.t())
+    with pytest.raises(RuntimeError, match="contiguous rows"):
+        _table_stride(t.int())
