@@ -15,7 +15,7 @@
 // it by 2^8; then the row's O is rescaled in tensor memory.  P(j) replaces S(j) and S(j + 1) replaces P(j): the MMAs of a
 // CTA run in order, so the commit behind S(j + 1) also says that O has P(j) V(j).
 //
-// Chunks of 4 prompts (3521 new tokens behind 2002 to 4352 cached ones, 64 q heads on 8, d 128, int8): 764 us, 515 TFLOP/s, 0.31
+// Chunks of 4 prompts (3521 new tokens behind 2002 to 4352 cached ones, 64 q heads on 8, d 128, int8): 761 us, 517 TFLOP/s, 0.31
 // of the measured rate of a large matrix product; the simple form of the same loop took 3136 us.  What bounds it is the
 // chain of one row tile (scores out of tensor memory, p back: 3600 cycles for four warps; then the product and the next
 // scores), of which two run side by side.  Without the exponentials it takes as long; without the conversion 6 % less.

@@ -40,12 +40,13 @@ class KvBatch:
     ``page_table`` int64 ``[n, max_pages]`` (entries behind a sequence's last page are not read); ``kv_len`` int32
     ``[n]``: tokens in the cache, the step's new ones included; ``q_start`` / ``q_len`` int32 ``[n]``: the rows of q, k and
     v that are the sequence's new tokens (the reference's ``b_start_loc`` / ``b_seq_len``).  ``max_q_len`` bounds
-    ``q_len`` (as ``max_len_in_batch`` does in the reference; it sizes launches).
+    ``q_len`` (as ``max_len_in_batch`` does in the reference; it sizes launches), ``max_kv_len``, when given, ``kv_len``
+    (up to the end of its page): the table's columns behind it are not looked at, and workspaces are sized by it.
 
     The kernels check every length and page; what they had to skip is in :meth:`status`.
     """
 
-    def __init__(self, page_table, kv_len, q_start, q_len, max_q_len):
+    def __init__(self, page_table, kv_len, q_start, q_len, max_q_len, max_kv_len=None):
         _lib.require_cuda(page_table, kv_len, q_start, q_len)
         stride = _table_stride(page_table)
         n = page_table.size(0)
@@ -54,15 +55,27 @@ class KvBatch:
                 raise RuntimeError(f"{name} must be a contiguous int32 tensor with one entry per sequence")
             if t.device != page_table.device:
                 raise RuntimeError(f"{name} and page_table lie on different devices")
-        if max_q_len < 0:
-            raise RuntimeError("max_q_len must not be negative")
+        if max_q_len < 0 or (max_kv_len is not None and max_kv_len < 0):
+            raise RuntimeError("max_q_len and max_kv_len must not be negative")
         self.page_table, self.kv_len, self.q_start, self.q_len = page_table, kv_len, q_start, q_len
         self.max_q_len = int(max_q_len)
+        self.max_kv_len = None if max_kv_len is None else int(max_kv_len)
         self._status = torch.zeros((1,), dtype=torch.int32, device=page_table.device)
-        self.c = _lib.Kv8Batch(page_table.data_ptr(), stride, kv_len.data_ptr(), q_start.data_ptr(),
-                               q_len.data_ptr(), self._status.data_ptr(), n, page_table.size(1), self.max_q_len)
-        self.ptr = ctypes.addressof(self.c)
+        self._fields = [page_table.data_ptr(), stride, kv_len.data_ptr(), q_start.data_ptr(), q_len.data_ptr(),
+                        self._status.data_ptr(), n, page_table.size(1), self.max_q_len]
+        self.n_seq = n
+        self._c = {}            # by the cache's page size
         self.workspaces = {}    # bytes that attention over this batch needs, by the call's sizes
+
+    def _ptr(self, page_tokens):
+        """The C struct for a cache with that page size (it counts columns of the page table)."""
+        c = self._c.get(page_tokens)
+        if c is None:
+            f = list(self._fields)
+            if self.max_kv_len is not None:
+                f[7] = min(f[7], -(-self.max_kv_len // page_tokens))
+            c = self._c[page_tokens] = _lib.Kv8Batch(*f)
+        return ctypes.addressof(c)
 
     def status(self) -> int:
         """Status bits (``_lib.STATUS_BITS``) of the calls so far -- synchronises the current stream."""
@@ -191,8 +204,8 @@ class KvCache8:
             qp, qop, q_heads = q.data_ptr(), q_out.data_ptr(), q_shape[1]
         elif q_out is not None:
             raise RuntimeError("q_out without q")
-        _lib.call(ctx, _lib.lib.slora_kv8_append, self._ptr[layer], batch.ptr, k.data_ptr(), v.data_ptr(), k_stride, v_stride,
-                  shape[0], qp, qop, q_heads, q_stride, qo_stride, pos, turns, rot, factor, layout, _lib.dtype_code(dtype))
+        _lib.call(ctx, _lib.lib.slora_kv8_append, self._ptr[layer], batch._ptr(self.page_tokens), k.data_ptr(), v.data_ptr(),
+                  k_stride, v_stride, shape[0], qp, qop, q_heads, q_stride, qo_stride, pos, turns, rot, factor, layout, _lib.dtype_code(dtype))
         return q_out
 
     def read(self, layer, batch, dtype, count, first=None):
@@ -202,12 +215,12 @@ class KvCache8:
         if count < 0:
             raise RuntimeError("count must not be negative")
         ctx = _lib.device_of(self.k[layer], batch.kv_len, first)
-        if first is not None and (first.dtype != torch.int32 or first.numel() != batch.c.n_seq or not first.is_contiguous()):
+        if first is not None and (first.dtype != torch.int32 or first.numel() != batch.n_seq or not first.is_contiguous()):
             raise RuntimeError("first must be a contiguous int32 tensor with one entry per sequence")
-        shape = (batch.c.n_seq, int(count), self.kv_heads, self.head_dim)
+        shape = (batch.n_seq, int(count), self.kv_heads, self.head_dim)
         k, v = torch.empty(shape, dtype=dtype, device=self.device), torch.empty(shape, dtype=dtype, device=self.device)
-        _lib.call(ctx, _lib.lib.slora_kv8_read, self._ptr[layer], batch.ptr, _lib.ptr(first), int(count), k.data_ptr(), v.data_ptr(),
-                  code)
+        _lib.call(ctx, _lib.lib.slora_kv8_read, self._ptr[layer], batch._ptr(self.page_tokens), _lib.ptr(first), int(count),
+                  k.data_ptr(), v.data_ptr(), code)
         return k, v
 
     def attend(self, layer, batch, q, out=None, lse=None, scale=None, window=0, add_weights=False):
@@ -240,18 +253,18 @@ class KvCache8:
                 raise RuntimeError("out must have q's shape and dtype")
         if lse is not None and (lse.dtype != torch.float32 or lse.shape != (tokens, heads) or not lse.is_contiguous()):
             raise RuntimeError("lse must be a contiguous float32 tensor [tokens, heads]")
-        if tokens == 0 or batch.c.n_seq == 0:
+        if tokens == 0 or batch.n_seq == 0:
             return out
         # the size follows from the sizes in the key (and the device, which is the cache's)
         key = (self._key, tokens, heads, bool(add_weights))
         need = batch.workspaces.get(key)
         if need is None:
             need = batch.workspaces[key] = max(_lib.lib.slora_kv8_attend_workspace_bytes(
-                self._ptr[layer], batch.ptr, tokens, heads, int(add_weights)), 16)
+                self._ptr[layer], batch._ptr(self.page_tokens), tokens, heads, int(add_weights)), 16)
         ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-        _lib.call(ctx, _lib.lib.slora_kv8_attend, self._ptr[layer], batch.ptr, q.data_ptr(), q_stride, tokens, heads, out.data_ptr(),
-                  o_stride, _lib.ptr(lse), d ** -0.5 if scale is None else float(scale), int(window), int(add_weights), ws.data_ptr(),
-                  need, code)
+        _lib.call(ctx, _lib.lib.slora_kv8_attend, self._ptr[layer], batch._ptr(self.page_tokens), q.data_ptr(), q_stride, tokens,
+                  heads, out.data_ptr(), o_stride, _lib.ptr(lse), d ** -0.5 if scale is None else float(scale), int(window),
+                  int(add_weights), ws.data_ptr(), need, code)
         return out
 
     def evict(self, layer, batch, budget, recent, sink=0, dest=None):
@@ -268,12 +281,12 @@ class KvCache8:
         if self.weights is None:
             raise RuntimeError("evict needs a cache with track_weights")
         table = batch.page_table if dest is None else dest.page_table
-        if table.size(0) != batch.c.n_seq:
+        if table.size(0) != batch.n_seq:
             raise RuntimeError("dest must have one row of pages per sequence")
         if budget < 1 or recent < 0 or sink < 0 or recent + sink > budget:
             raise RuntimeError("budget must hold the sink and the recent tokens")
         ctx = _lib.device_of(self.k[layer], batch.kv_len, table)
-        kept = torch.empty((batch.c.n_seq, self.kv_heads, int(budget)), dtype=torch.int32, device=self.device)
-        _lib.call(ctx, _lib.lib.slora_kv8_evict, self._ptr[layer], batch.ptr, int(budget), int(recent), int(sink), kept.data_ptr(),
-                  table.data_ptr(), _table_stride(table), table.size(1))
+        kept = torch.empty((batch.n_seq, self.kv_heads, int(budget)), dtype=torch.int32, device=self.device)
+        _lib.call(ctx, _lib.lib.slora_kv8_evict, self._ptr[layer], batch._ptr(self.page_tokens), int(budget), int(recent),
+                  int(sink), kept.data_ptr(), table.data_ptr(), _table_stride(table), table.size(1))
         return kept

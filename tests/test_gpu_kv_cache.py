@@ -308,6 +308,25 @@ def test_bad_tables_are_skipped_and_reported():
     assert not torch.equal(out[w.starts[0]], good[w.starts[0]])
 
 
+@pytest.mark.parametrize("bound", [80, 77, 81, 0, 10 ** 9])
+def test_bound_of_the_lengths(bound):
+    # 80 tokens are five pages of 16: a bound of 77 reaches as far, one of 81 takes a sixth page in, 0 leaves no key
+    sl = _sl()
+    w = World([100, 80, 60], [1, 1, 1], 2, 128, 16, "int8")
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    q = torch.randn(w.T, 4, 128, device=DEV).half()
+    good = w.cache.attend(0, w.batch, q, out=torch.full_like(q, 7.0))
+    b = sl.KvBatch(w.batch.page_table, i32(w.lens), i32(w.starts), i32(w.new), 1, bound)
+    out = w.cache.attend(0, b, q, out=torch.full_like(q, 7.0), add_weights=True)
+    for i, n in enumerate(w.lens):
+        inside = n <= -(-bound // 16) * 16
+        assert torch.equal(out[w.starts[i]], good[w.starts[i]] if inside else torch.full_like(q[0], 7.0)), i
+    assert b.status() == (0 if bound >= 100 else 2)
+    kept = w.cache.evict(0, b, 50, 4)
+    for i, n in enumerate(w.lens):
+        assert bool((kept[i] >= 0).all()) == (n <= -(-bound // 16) * 16), i
+
+
 def test_empty_batches():
     sl = _sl()
     w = World([30], [1], 2, 64, 16, "int8")
