@@ -39,7 +39,8 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return b >> 31 ? ~b : b | 0x80000000u;
 }
 
-// 256 (sequence, head) pairs of 3030 to 15912 weights, 2048 of them kept: 36 us; 32 pairs of 1225 to 1681: 10 us.
+// 256 (sequence, head) pairs of 3030 to 15912 weights, 2048 of them kept: 36 us; 32 pairs of 1225 to 1681: 10 us.  One CTA of
+// 1024 threads per SM; two of 512 took 42 us.
 __global__ void __launch_bounds__(kSelectThreads) kv_select_kernel(const EvictArgs a) {
   extern __shared__ uint32_t keys[];
   __shared__ int hist[kSelectCopies][256];
@@ -219,8 +220,8 @@ __device__ __forceinline__ void move_store(MoveRows<D>& m, uint8_t* dst, bool sa
   }
 }
 
-// The same 256 heads in place: 108 us for 0.27 GB.  Three CTAs per SM are what 80 registers allow; a round waits for its loads
-// and for the join of its maxima, so more rounds in flight (CTAs), not wider ones, is what the bandwidth comes from.
+// The same 256 heads to other pages: 108 us for 0.27 GB moved.  The exact rounding bounds it (17 instructions a value, issue
+// slots 63 % busy), then a round's wait for its loads and for the join of its maxima, which three CTAs per SM cover.
 template <int D, int KIND>
 __global__ void __launch_bounds__(kMoveThreads, D <= 128 ? 3 : 1) kv_move_kernel(const EvictArgs a) {
   using V8 = Kv8<KIND>;

@@ -99,6 +99,8 @@ def test_evict_is_refused():
     assert _evict(budget=0) == -4 and _evict(recent=-1) == -4 and _evict(sink=-1) == -4 and _evict(recent=20, sink=20) == -4
     assert _evict(pages=1) == -4 and _evict(stride=3) == -4
     assert _evict(b=_batch(n_seq=0)) == 0
+    # the selection counts a layer's weights in 32 bits
+    assert _evict(_cache(n_pages=2 ** 31)) == -4 and _evict(_cache(n_pages=2 ** 62)) == -4
 
 
 def test_read_is_refused():
