@@ -511,9 +511,10 @@ int slora_rotary(void* q_out, void* k_out, const void* q, const void* k, int64_t
  * and is not rounded between rotation and quantisation).
  * Per touched page and KV head: s_new = max(s_old, max |x| / top) over the new values x (top 127 or 448; s_old = 0 when
  * the page holds no older token of the sequence); new values become round(x / s_new); when s_new > s_old the page's older
- * values q become round(q * s_old / s_new); a scale below FP32's smallest normal number counts as 0.  Rounding is to nearest, ties to even, of the exact quotient.  NaN is stored as
- * 0 and infinities as the largest value (both leave the scale alone) with SLORA_STATUS_NONFINITE.  weights of new
- * tokens, where the cache has them, become 0.  Positions beyond kv_len of the last page are left as they are.
+ * values q become round(q * s_old / s_new); a scale below FP32's smallest normal number counts as 0, and the values of
+ * its page as 0.  Rounding is to nearest, ties to even, of the exact quotient.  NaN is stored as 0 and infinities as the
+ * largest value (both leave the scale alone) with SLORA_STATUS_NONFINITE.  weights of new tokens, where the cache has
+ * them, become 0.  Positions beyond kv_len of the last page are left as they are.
  * A page that is appended to must belong to one sequence.
  */
 #define SLORA_STATUS_NONFINITE 16 /* a NaN or an infinity was appended to an 8-bit cache */

@@ -294,13 +294,18 @@ __device__ __forceinline__ void kv_finite(float& x) {
   if (!(fabsf(x) <= 3.4028234663852886e38f)) x = x == x ? copysignf(3.4028234663852886e38f, x) : 0.f;
 }
 
-// Older values of a (page, head), `bytes` of them, rounded to a grown scale: 16 bytes a lane.
+// Older values of a (page, head), `bytes` of them, rounded to a grown scale: 16 bytes a lane.  s_old 0 (a scale that counts
+// as 0): they become 0, and s_new may be 0 too.
 template <int KIND>
 __device__ __forceinline__ void append_rescale(uint8_t* page, int bytes, float s_old, float s_new, int id, int step) {
   using V8 = Kv8<KIND>;
   const float mul = __fdiv_rn(s_old, s_new);
 #pragma unroll 1
   for (int i = id; i < bytes / 16; i += step) {
+    if (!(s_old > 0.f)) {
+      reinterpret_cast<uint4*>(page)[i] = make_uint4(0, 0, 0, 0);
+      continue;
+    }
     const uint4 w = reinterpret_cast<const uint4*>(page)[i];
     float q[4];
     uint4 y;
@@ -351,7 +356,7 @@ __device__ __forceinline__ void append_page_cta(const AppendArgs& a, const uint8
   __shared__ float tops[kRowWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % kLanes, half = a.r.rot >> 1;
   const int mine = warp * kRows + lane / kLanes, n = n1 - n0, passes = (n + kPass - 1) / kPass;
-  const float s_old = n0 > 0 ? *scale : 0.f;
+  const float was = n0 > 0 ? *scale : 0.f, s_old = kv_scale(was);
   auto row = [&](int p, float (&x)[8]) {
     const int i = min(mine + p * kPass, n - 1);  // lanes without a row repeat the last one
     cvt8<T>(*reinterpret_cast<const uint4*>(rows + (i * kLanes + sub) * 16), x);
@@ -386,7 +391,7 @@ __device__ __forceinline__ void append_page_cta(const AppendArgs& a, const uint8
 #pragma unroll
   for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, tops[w]);
   const float s_new = kv_scale(fmaxf(s_old, __fdiv_rn(top, V8::kTop)));
-  if (s_new != s_old && n0 > 0) append_rescale<KIND>(page, n0 * D, s_old, s_new, threadIdx.x, kRowThreads);
+  if (s_new != was && n0 > 0) append_rescale<KIND>(page, n0 * D, s_old, s_new, threadIdx.x, kRowThreads);
   const float mul = s_new > 0.f ? __fdiv_rn(1.f, s_new) : 0.f;
 #pragma unroll 1
   for (int p = 0; p < passes; ++p) {
@@ -407,7 +412,7 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, const T* src, i
   constexpr int kLanes = D / 8, kRows = 32 / kLanes;
   using V8 = Kv8<KIND>;
   const int lane = threadIdx.x & 31, sub = lane % kLanes, rr = lane / kLanes, half = a.r.rot >> 1;
-  const float s_old = n0 > 0 ? *scale : 0.f;
+  const float was = n0 > 0 ? *scale : 0.f, s_old = kv_scale(was);
   float x[8];
   auto load = [&](int base) {
     const int i = base + rr;
@@ -439,7 +444,7 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, const T* src, i
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
   const float s_new = kv_scale(fmaxf(s_old, __fdiv_rn(top, V8::kTop)));
-  if (s_new != s_old && n0 > 0) append_rescale<KIND>(page, n0 * D, s_old, s_new, lane, 32);
+  if (s_new != was && n0 > 0) append_rescale<KIND>(page, n0 * D, s_old, s_new, lane, 32);
   const float mul = s_new > 0.f ? __fdiv_rn(1.f, s_new) : 0.f;
   for (int base = n0; base < n1; base += kRows) {
     const bool real = load(base);

@@ -488,6 +488,32 @@ def test_appending_one_by_one(kind):
     assert (got[0] - x).abs().max() <= top * (0.5 / 127 * 6 if kind == "int8" else 2.0 ** -4 * 6)
 
 
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("new", [2, 9])          # a warp's page, and the whole CTA's
+@pytest.mark.parametrize("top", [0.0, 1.0])      # new values: all 0, and not
+def test_a_scale_below_the_normal_numbers_counts_as_zero(kind, new, top):
+    lens = [new + 5, 20 + new]
+    w = World(lens, [new, new], 2, 64, 16, kind)
+    firsts = [(int(w.table[i, (n - new) // 16]), (n - new) % 16) for i, n in enumerate(lens)]    # pages with older tokens
+    for p, _ in firsts:
+        w.ks[p], w.vs[p] = 2.0 ** -127, 2.0 ** -149
+    x = torch.randn(w.T, 2, 64, device=DEV).half() * top
+    w.cache.append(0, w.batch, x, x)
+    torch.cuda.synchronize()
+    assert w.batch.status() == 0
+    for (p, n0), n, r0 in zip(firsts, lens, w.starts):
+        m = min(16, n0 + new) - n0                # new tokens of that page
+        y = x[r0:r0 + m].transpose(0, 1).double()
+        s = ref.scale_of(y.abs().amax((1, 2)), kind)
+        for x8, sc in ((w.k8, w.ks), (w.v8, w.vs)):
+            assert torch.equal(sc[p].double(), s)
+            assert (ref.values(x8)[p, :, :n0] == 0).all()
+            assert torch.equal(ref.values(x8)[p, :, n0:n0 + m], ref.nearest(y / torch.where(s > 0, s, 1.0)[:, None, None], kind))
+    k, v = w.cache.read(0, w.batch, torch.float16, max(lens))
+    out = w.cache.attend(0, w.batch, torch.randn(w.T, 4, 64, device=DEV).half())
+    assert torch.isfinite(k).all() and torch.isfinite(v).all() and torch.isfinite(out[w.own_rows()]).all()
+
+
 def test_nonfinite_values_are_stored_finite_and_reported():
     w = World([20, 33], [4, 33], 2, 64, 16, "int8")
     x = torch.randn(w.T, 2, 64, device=DEV).half()
