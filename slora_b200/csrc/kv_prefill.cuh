@@ -9,16 +9,23 @@
 //   P            over S in tensor memory (f16 pairs), the A operand of the second product
 //   O += P V     V in shared memory as it lies in the cache, keys outside: the outer-major form of the same layout
 // Roles: seven warps convert 8-bit pages to f16 operands (values exact, as in kv_attend.cuh; with four of them the tensor
-// pipe waited for operands), one lane issues the MMAs, four warps per row tile do the softmax.  Scales never touch the operands: a page's k scale multiplies its 16-column groups of
-// S (the maximum of a group is taken before it), its v scale, relative to the largest one of the sequence, goes into the
-// exponent of p, and comes out of the sum of p again per group.  The running maximum is raised only when a score passes
-// it by 2^8; then the row's O is rescaled in tensor memory.  P(j) replaces S(j) and S(j + 1) replaces P(j): the MMAs of a
-// CTA run in order, so the commit behind S(j + 1) also says that O has P(j) V(j).
+// pipe waited for operands), one lane issues the MMAs, four warps per row tile do the softmax.  Scales never touch the
+// operands: a page's k scale multiplies its 16-column groups of S (the maximum of a group is taken before it), its v
+// scale, relative to the row's reference, goes into the exponent of p, and comes out of the sum of p again per group.
+// The reference is a power of two, a row's own; it follows the largest v scale that the row sees in a step of 128 keys,
+// so pages that a row does not see (later tokens, what a window has left behind) cost it nothing, and a change rescales
+// the row's O by a power of two, which rounds nothing.  p * vs is one f16 number (64 p vs / 2^ref; for f16 outputs too:
+// its 2^-11 shows as 1.4 times the error of the output's own rounding, a second number would double the product): off by
+// 2^-11 of itself or, where it is small, by 2^-31 of the reference, which is 2 to 2^9 times the step's largest scale.
+// The running maximum is raised only when a score passes it by 2^8; then the row's O is rescaled in tensor memory.  P(j)
+// replaces S(j) and S(j + 1) replaces P(j): the MMAs of a CTA run in order, so the commit behind S(j + 1) also says that
+// O has P(j) V(j).
 //
-// Chunks of 4 prompts (3521 new tokens behind 2002 to 4352 cached ones, 64 q heads on 8, d 128, int8): 761 us, 517 TFLOP/s, 0.31
-// of the measured rate of a large matrix product; the simple form of the same loop took 3136 us.  What bounds it is the
-// chain of one row tile (scores out of tensor memory, p back: 3600 cycles for four warps; then the product and the next
-// scores), of which two run side by side.  Without the exponentials it takes as long; without the conversion 6 % less.
+// Chunks of 4 prompts (3521 new tokens behind 2002 to 4352 cached ones, 64 q heads on 8, d 128, int8): 790 us, 498 TFLOP/s, 0.29
+// of the measured rate of a large matrix product (d 64: 630 us); the simple form of the same loop took 3136 us.  What bounds
+// it is the chain of one row tile (scores out of tensor memory, p back: 3700 cycles for four warps; then the product and
+// the next scores), of which two run side by side.  Without the exponentials it takes as long; without the conversion 6 %
+// less; with one reference for all rows of a CTA (which let pages that a row does not see round its p) 2 to 3 % less.
 //
 // Every wait is bounded; a CTA that gives up records SLORA_STATUS_TIMEOUT and frees its tensor memory.
 #pragma once
@@ -37,7 +44,12 @@ constexpr int kPreKeys = 128;                // keys of a step
 constexpr int kPreRows = 256;                // rows of a CTA
 constexpr int kPreGroups = kPreKeys / 16;    // 16 keys share their scales whatever the page size
 constexpr int kPreScaleSlots = 4;            // steps whose scales are kept: the softmax of a step reads them after its K is gone
-constexpr float kPreRange = 64.f;            // p * vs / vmax * 64 <= 2^8 * 2^6: inside f16
+constexpr float kPreRange = 6.f;             // log2: p * vs / reference * 2^6 <= 2^8 * 2^6: inside f16
+constexpr float kPreLower = 8.f;             // octaves that a step's largest v scale may lie below the reference
+constexpr float kPreFar = 40.f;              // octaves below the reference from which a scale's p * vs is 0 in f16 (p only counts)
+constexpr float kPreRise = 64.f;             // octaves that the reference may sink from its highest: O stays inside FP32
+constexpr float kNoScale = -1000.f;          // exponent of a scale that counts as 0, or of no page
+constexpr float kNoRef = -200.f;             // no reference yet (the smallest is above -126)
 
 template <int D>
 struct PreSmem {
@@ -47,8 +59,10 @@ struct PreSmem {
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full;
   uint32_t tmem;
   int bad;
-  unsigned vmax;
-  alignas(16) float fk[kPreScaleSlots][kPreGroups], lv[kPreScaleSlots][kPreGroups], rv[kPreScaleSlots][kPreGroups];
+  // Per 16 keys, v scale = m 2^e with m in [0.5, 1), top the largest e of the step: k scale, log2 m (-inf: a bad page), e + 6
+  // and 1 / m (part, for rows that see a part of the step), or 2^(top - e - 6) / m (whole).
+  alignas(16) float4 whole[kPreScaleSlots][kPreGroups], part[kPreScaleSlots][kPreGroups];
+  float top[kPreScaleSlots];
   KvFind find;
 };
 
@@ -98,13 +112,13 @@ __device__ __forceinline__ uint64_t umma_smem_desc_sw128_mn(uint32_t addr, uint3
 template <int D, bool MASKED>
 __device__ __forceinline__ float pre_max(const PreSmem<D>& sm, int slot, uint32_t t_s, float down, int from, int to) {
   float top = kNegInf;
-  uint32_t w[2][32];
-  tmem_ld32(t_s, w[0]);
+  uint32_t raw[2][32];
+  tmem_ld32(t_s, raw[0]);
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     tmem_ld_wait();
-    if (c < 3) tmem_ld32(t_s + 32 * (c + 1), w[(c + 1) & 1]);
-    uint32_t(&x)[32] = w[c & 1];
+    if (c < 3) tmem_ld32(t_s + 32 * (c + 1), raw[(c + 1) & 1]);
+    uint32_t(&x)[32] = raw[c & 1];
     if (MASKED) {
 #pragma unroll
       for (int e = 0; e < 32; ++e)
@@ -119,29 +133,48 @@ __device__ __forceinline__ float pre_max(const PreSmem<D>& sm, int slot, uint32_
         g1 = fmaxf(g1, __uint_as_float(x[16 * h + e + 1]));
       }
       g0 = fmaxf(g0, g1);
-      if (g0 > kNegInf && sm.lv[slot][2 * c + h] > kNegInf) top = fmaxf(top, g0 * (down * sm.fk[slot][2 * c + h]));
+      const float4 w = sm.whole[slot][2 * c + h];
+      if (g0 > kNegInf && w.y > kNegInf) top = fmaxf(top, g0 * (down * w.x));
     }
   }
   return top;
 }
 
-// p of this thread's row as f16 pairs, relative to m0, and their sum; tells whether one passes 2^14 (a score far above m0).
+// 2^e for a whole number e from -126 to 127: e + 127 in the low bits of 1.5 * 2^23 + e + 127, moved to the exponent's place.
+__device__ __forceinline__ float pre_pow2(float e) { return __uint_as_float(__float_as_uint(e + 12583039.f) << 23); }
+
+// The largest exponent of a v scale in the step among the keys [from, to).
+template <int D>
+__device__ __forceinline__ float pre_largest(const PreSmem<D>& sm, int slot, int from, int to) {
+  float e = kNoScale;
+#pragma unroll
+  for (int g = 0; g < kPreGroups; ++g)
+    if (16 * g < to && 16 * g + 16 > from) e = fmaxf(e, sm.part[slot][g].z - kPreRange);
+  return e;
+}
+
+// p of this thread's row, relative to m0, times v scale / 2^ref, as f16 pairs, and the sum of p; tells whether one passes
+// 2^14 (a score far above m0).  MASKED: groups the row does not see may have any scale.
 template <int D, bool MASKED>
-__device__ __forceinline__ bool pre_exp(const PreSmem<D>& sm, int slot, uint32_t t_s, float down, float m0, float* sum, int from, int to,
-                                        uint32_t (&y)[64]) {
+__device__ __forceinline__ bool pre_exp(const PreSmem<D>& sm, int slot, uint32_t t_s, float down, float m0, float ref, float* sum, int from,
+                                        int to, uint32_t (&y)[64]) {
   uint32_t x[32];  // (a second buffer, for the columns to come, cost the converters more registers than it saved time)
   float l = 0.f;
   uint32_t high = 0;
+  const float most = sm.top[slot];
+  if (!MASKED) ref = most > kNoScale ? fminf(ref, most + kPreFar) : kNoScale;
+  const float base = m0 + ref;  // what a score's exponent is taken relative to
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
-    const float2 fk = *reinterpret_cast<const float2*>(&sm.fk[slot][2 * c]);
-    const float2 lv = *reinterpret_cast<const float2*>(&sm.lv[slot][2 * c]);
-    const float2 rv = *reinterpret_cast<const float2*>(&sm.rv[slot][2 * c]);
+    const float4 w0 = MASKED ? sm.part[slot][2 * c] : sm.whole[slot][2 * c];
+    const float4 w1 = MASKED ? sm.part[slot][2 * c + 1] : sm.whole[slot][2 * c + 1];
     tmem_ld32(t_s + 32 * c, x);
     tmem_ld_wait();
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const float f = down * (h ? fk.y : fk.x), add = (h ? lv.y : lv.x) - m0;
+      const float4 w = h ? w1 : w0;
+      const float e2 = MASKED ? fminf(fmaxf(w.z, ref - kPreFar + kPreRange), ref + 20.f) : w.z;
+      const float f = down * w.x, add = w.y + (e2 - base), back = MASKED ? w.w * pre_pow2(ref - e2) : w.w;
       float s0 = 0.f, s1 = 0.f;
 #pragma unroll
       for (int e = 0; e < 16; e += 2) {
@@ -158,10 +191,10 @@ __device__ __forceinline__ bool pre_exp(const PreSmem<D>& sm, int slot, uint32_t
         y[16 * c + 8 * h + e / 2] = p;
         asm("max.f16x2 %0, %1, %2;" : "=r"(high) : "r"(high), "r"(p));
       }
-      l = __fmaf_rn(s0 + s1, h ? rv.y : rv.x, l);
+      l = __fmaf_rn(s0 + s1, back, l);
     }
   }
-  *sum = l;
+  *sum = MASKED ? l : l * pre_pow2(ref - most);
   const float2 top = __half22float2(reinterpret_cast<const __half2&>(high));
   return fmaxf(top.x, top.y) > 16384.f;
 }
@@ -214,27 +247,12 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_kernel(const KvAtte
     }
     mbar_init(&sm.o_full, 1);
     sm.bad = 0;
-    sm.vmax = 0;
     fence_barrier_init();
-  }
-  __syncthreads();
-  // the largest v scale of the pages in reach
-  {
-    float m = 0.f;
-    const int p1 = (key_end + (1 << a.c.shift) - 1) >> a.c.shift;
-    for (int p = (key0 >> a.c.shift) + tid; p < p1; p += kPreThreads) {
-      const int64_t id = kv_page(a.c, a.b, seq, p << a.c.shift);
-      if (id >= 0) m = fmaxf(m, a.c.vs[id * a.c.hkv + head]);
-    }
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-    if (lane == 0 && m > 0.f) atomicMax(&sm.vmax, __float_as_uint(m));
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sm.tmem;
-  const float vmax = sm.vmax > 0 ? __uint_as_float(sm.vmax) : 1.f;
   bool ok = true;
 
   if (warp < kPreSoftWarps) {
@@ -284,6 +302,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_kernel(const KvAtte
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + lane_off + tile * 128, t_o = tmem + lane_off + 256 + tile * D;
     float m = kNegInf, l = 0.f;
+    float ref = kNoRef, highest = kNoRef;  // log2 of the row's reference, and its highest so far
     for (int i = 0; i < steps && ok; ++i) {
       // the step's scales were written before k_full, which the MMAs behind this barrier waited for
       ok = __all_sync(0xffffffffu, mbar_wait(&sm.s_full[tile], i & 1));
@@ -293,19 +312,34 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_kernel(const KvAtte
       const bool masked = key < from_max || key + kPreKeys > to_min;
       uint32_t p[64];
       float sum = 0.f;
+      // the reference: above the largest scale that the row sees, and not far above
+      const float was = ref;
+      bool again = i == 0;
+      {
+        const float e = masked ? pre_largest<D>(sm, slot, from - key, to - key) : sm.top[slot];
+        if (e > kNoScale && (e > ref || (e < ref - kPreLower && ref > highest - kPreRise))) {
+          const float now = fmaxf(e + 1.f, highest - kPreRise);
+          ref = now;
+          highest = fmaxf(highest, now);
+        }
+      }
       // p relative to the maximum so far; only where a score lies far above it (and in the first step) is the maximum taken
       // anew, O and the sum so far rescaled, and p computed again (S is still there)
-      bool again = i == 0;
       if (!again)
-        again = masked ? pre_exp<D, true>(sm, slot, t_s, down, m == kNegInf ? 0.f : m, &sum, from - key, to - key, p)
-                       : pre_exp<D, false>(sm, slot, t_s, down, m == kNegInf ? 0.f : m, &sum, 0, 0, p);
+        again = masked ? pre_exp<D, true>(sm, slot, t_s, down, m == kNegInf ? 0.f : m, ref, &sum, from - key, to - key, p)
+                       : pre_exp<D, false>(sm, slot, t_s, down, m == kNegInf ? 0.f : m, ref, &sum, 0, 0, p);
       again = again || m == kNegInf;
-      if (__any_sync(0xffffffffu, again)) {
-        const float top = masked ? pre_max<D, true>(sm, slot, t_s, down, from - key, to - key) : pre_max<D, false>(sm, slot, t_s, down, 0, 0);
-        const float now = again ? fmaxf(m, top) : m;  // only rows that need it: a row's p do not depend on the others
-        const float f = now == kNegInf ? 1.f : ex2(m - now);
-        m = now;
-        l *= f;
+      if (__any_sync(0xffffffffu, again || ref != was)) {
+        float f = was > kNoRef ? pre_pow2(fmaxf(was - ref, -126.f)) : 1.f;
+        const bool anew = __any_sync(0xffffffffu, again);
+        if (anew) {
+          const float top = masked ? pre_max<D, true>(sm, slot, t_s, down, from - key, to - key) : pre_max<D, false>(sm, slot, t_s, down, 0, 0);
+          const float now = again ? fmaxf(m, top) : m;  // only rows that need it: a row's p do not depend on the others
+          const float fall = now == kNegInf ? 1.f : ex2(m - now);
+          m = now;
+          l *= fall;
+          f *= fall;
+        }
         if (i > 0) {
 #pragma unroll 1
           for (int c = 0; c < D / 32; ++c) {
@@ -321,7 +355,8 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_kernel(const KvAtte
             tmem_st16(t_o + 32 * c + 16, y);
           }
         }
-        pre_exp<D, true>(sm, slot, t_s, down, m == kNegInf ? 0.f : m, &sum, masked ? from - key : 0, masked ? to - key : kPreKeys, p);
+        if (anew)
+          pre_exp<D, true>(sm, slot, t_s, down, m == kNegInf ? 0.f : m, ref, &sum, masked ? from - key : 0, masked ? to - key : kPreKeys, p);
       }
       l += sum;
 #pragma unroll
@@ -339,7 +374,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_kernel(const KvAtte
     if (ok && steps > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sm.o_full, 0));
     if (ok) {
       tc_fence_after();
-      const float inv = l > 0.f ? vmax * (V8::kScale / kPreRange) / l : (l == 0.f ? 0.f : l);
+      const float inv = l > 0.f ? ldexpf(V8::kScale, static_cast<int>(fmaxf(ref, -140.f) - kPreRange)) / l : (l == 0.f ? 0.f : l);
       T* dst = static_cast<T*>(a.out) + (static_cast<int64_t>(s.row) + j) * a.out_stride + (head * a.group + row - j * a.group) * D;
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
@@ -437,21 +472,21 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_kernel(const KvAtte
       if (i >= 2) ok = mbar_wait(&sm.k_empty[st], ((i >> 1) - 1) & 1);
       if (!(ok = __all_sync(0xffffffffu, ok))) break;
       // lane g of each warp: scales of 16-key group g (lanes 8 and up repeat them)
-      int counts = 1;
-      {
-        float f = 0.f, lv = kNegInf, rv = 1.f;
-        if (page_now >= 0) {
-          // a scale of zero (or next to nothing beside the largest): the values count as zero, p only in the sum
-          const float rel = vs_now / vmax;
-          counts = rel > 1e-30f;
-          f = ks_now;
-          lv = (counts ? log2f(rel) : 0.f) + 6.f;
-          rv = (counts ? 1.f / rel : 1.f) * (1.f / kPreRange);
-        }
-        if (cw == 0 && l2 < kPreGroups) {
-          sm.fk[slot][l2] = f;
-          sm.lv[slot][l2] = lv;
-          sm.rv[slot][l2] = rv;
+      const bool counts = vs_now >= kLeastScale;  // a smaller scale: the values count as zero, p only in the sum
+      if (cw == 0) {
+        const uint32_t bits = __float_as_uint(vs_now);
+        const bool there = page_now >= 0;
+        const float e = there && counts ? static_cast<float>(static_cast<int>(bits >> 23) - 126) : kNoScale;
+        float top = e;
+#pragma unroll
+        for (int d = 1; d < kPreGroups; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        const float m = counts ? __uint_as_float((bits & 0x7fffffu) | 0x3f000000u) : 1.f;
+        const float e2 = fmaxf(e, top - kPreFar) + kPreRange, log2m = there ? __log2f(m) : kNegInf, ks = there ? ks_now : 0.f;
+        const float inv = __fdividef(1.f, m);  // within 2^-22, as log2m: next to nothing beside p's rounding
+        if (l2 < kPreGroups) {
+          sm.whole[slot][l2] = make_float4(ks, log2m, e2, pre_pow2(top - e2) * inv);
+          sm.part[slot][l2] = make_float4(ks, log2m, e + kPreRange, inv);
+          if (l2 == 0) sm.top[slot] = top;
         }
       }
       put(kr, sm.k[st]);
@@ -464,7 +499,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_kernel(const KvAtte
 #pragma unroll
       for (int p = 0; p < kPer; ++p) {
         const int group = min(unit_key(p * kCvtThreads + ct), kPreKeys - 1) >> 4;
-        if (__shfl_sync(0xffffffffu, counts, group) == 0) vr[p] = make_uint4(0, 0, 0, 0);
+        if (!__shfl_sync(0xffffffffu, counts, group)) vr[p] = make_uint4(0, 0, 0, 0);
       }
       put(vr, sm.v[st]);
       fence_proxy_async();

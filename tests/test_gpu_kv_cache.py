@@ -231,6 +231,63 @@ def test_extreme_scales_and_queries(kind):
     _check_attend(w, q, out, lse, None, None, 0, 2.0 ** -18)
 
 
+def _check_rows(w, q, out, window=0, without=()):
+    """As _check_attend, row by row: p vs is held to 2^-31 of a reference that is at most 2^9 times the largest v scale of the
+    keys that lie together, so a key adds at most 2^-22 |v|; |v| of the keys that the row sees, those of the pages in `without`
+    (whose p are next to 0) aside."""
+    kv, vv = ref.values(w.k8), ref.values(w.v8)
+    u = torch.finfo(q.dtype).eps / 2
+    for i, (n, m, r0) in enumerate(zip(w.lens, w.new, w.starts)):
+        k = ref.dense(kv, w.ks.double(), w.table[i], n)
+        v = ref.dense(vv, w.vs.double(), w.table[i], n)
+        o, _, _, mag, size = ref.attend(k, v, q[r0:r0 + m].double(), window, w.d ** -0.5)
+        ds = 2.0 ** -22 * (w.d / 16 + 8) * size
+        at, last = torch.arange(n, device=DEV), n - m + torch.arange(m, device=DEV)[:, None]
+        seen = (at <= last) & ((at > last - window) if window else torch.ones_like(at <= last))
+        heard = torch.tensor([int(w.table[i, pos // w.page]) not in without for pos in range(n)], device=DEV)
+        most = torch.where(seen & heard, v.abs().amax((0, 2)), 0.0).amax(1)                        # [rows]
+        tol = u * o.abs() + (2.0 ** -11 + 4 * ds + 2.0 ** -19) * mag + 2.0 ** -25 + (n * 2.0 ** -22 * most)[:, None, None]
+        off = (out[r0:r0 + m].double() - o).abs() / tol
+        assert float(off.max()) <= 1, (i, float(off.max()), off.amax((1, 2)).argmax())
+
+
+@pytest.mark.parametrize("d,page,kind", [(128, 16, "int8"), (64, 64, "e4m3"), (128, 128, "int8")])
+@pytest.mark.parametrize("more", [1e5, 2.0 ** 110])
+def test_chunks_pay_nothing_for_pages_they_do_not_see(d, page, kind, more):
+    # one page of far larger values: rows before it, and rows whose window has passed it, give the same bits without it
+    w = World([900, 640, 200], [330, 640, 70], 2, d, page, kind)
+    q = torch.randn(w.T, 8, d, device=DEV).bfloat16()
+    for window in (0, 100):
+        want = w.cache.attend(0, w.batch, q, window=window)
+        loud = [int(w.table[0, 640 // page]), int(w.table[1, 256 // page]), int(w.table[2, 128 // page])]
+        old = w.vs[loud].clone()
+        w.vs[loud] *= more
+        got = w.cache.attend(0, w.batch, q, window=window)
+        for i, first in enumerate((640, 256, 128)):
+            n, m, r0 = w.lens[i], w.new[i], w.starts[i]
+            behind = min(first + page, n) + (window if window else n) - 1
+            for j in range(m):
+                if n - m + j < first or n - m + j >= behind:
+                    assert torch.equal(got[r0 + j], want[r0 + j]), (i, j)
+        if more < 1e6:
+            _check_rows(w, q, got, window)
+        assert torch.isfinite(got[w.own_rows()].float()).all()
+        w.vs[loud] = old
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("at", [0, 3])
+def test_chunks_recover_from_large_values_of_no_weight(d, at):
+    # a page of large values (128 keys) that no query attends to: the others keep their bits
+    w = World([900], [200], 1, d, 128, "int8")
+    q = torch.randn(w.T, 4, d, device=DEV).abs().bfloat16()
+    p = int(w.table[0, at])
+    w.k8[p] = -127
+    w.ks[p] = 100.0 / 127 / d ** 0.5 / 0.7        # scores of -100 or so
+    w.vs[p] *= 1e8
+    _check_rows(w, q, w.cache.attend(0, w.batch, q), without=(p,))
+
+
 def test_strided_rows_and_scale():
     sl = _sl()
     w = World([300, 20], [1, 3], 2, 64, 16, "int8")
