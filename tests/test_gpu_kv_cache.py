@@ -288,6 +288,62 @@ def test_chunks_recover_from_large_values_of_no_weight(d, at):
     _check_rows(w, q, w.cache.attend(0, w.batch, q), without=(p,))
 
 
+@pytest.mark.parametrize("hq,hkv,d,page,kind", [(8, 2, 128, 16, "int8"), (4, 1, 64, 16, "e4m3"), (4, 2, 64, 32, "int8"),
+                                                (4, 1, 256, 16, "int8"), (2, 2, 128, 16, "e4m3")])
+@pytest.mark.parametrize("more", [1e5, 2.0 ** 110])
+def test_rows_pay_nothing_for_pages_they_do_not_see(hq, hkv, d, page, kind, more):
+    # a few tokens at once: a page of far larger values that the window of the later ones has passed, or that the earlier ones
+    # do not reach; the same bits as without it
+    w = World([900, 333], [6, 6], hkv, d, page, kind)
+    q = torch.randn(w.T, hq, d, device=DEV).bfloat16()
+    for window in (0, 98, 107):        # the first token's first key is the third from a page's end
+        want = w.cache.attend(0, w.batch, q, window=window)
+        for i, n in enumerate(w.lens):
+            begins = (n - 6 + 1 - window if window else 0) // page     # the page of the first key that the first token sees
+            for b in {max(begins, 0), (n - 1) // page}:
+                old = w.vs[int(w.table[i, b])].clone()
+                w.vs[int(w.table[i, b])] *= more
+                got = w.cache.attend(0, w.batch, q, window=window)
+                w.vs[int(w.table[i, b])] = old
+                assert torch.isfinite(got[w.own_rows()].float()).all()
+                for j in range(6):
+                    pos = n - 6 + j
+                    sees = pos >= b * page and (not window or pos - window < (b + 1) * page - 1)
+                    if not sees:
+                        assert torch.equal(got[w.starts[i] + j], want[w.starts[i] + j]), (window, i, b, j)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("new", [1, 5])
+@pytest.mark.parametrize("io", ["fp16", "bf16"])
+@pytest.mark.parametrize("at", [0, 7, 55])
+def test_rows_recover_from_large_values_of_no_weight(d, new, io, at):
+    w = World([900], [new], 1, d, 16, "int8")
+    q = torch.randn(w.T, 4, d, device=DEV).abs().to(_io(io))
+    p = int(w.table[0, at])
+    w.k8[p] = -127
+    w.ks[p] = 100.0 / 127 / d ** 0.5 / 0.7        # scores of -100 or so
+    w.vs[p] *= 1e8
+    _check_rows(w, q, w.cache.attend(0, w.batch, q), without=(p,))
+
+
+@pytest.mark.parametrize("lens,new,hq,hkv,d,page,kind,window", [
+    ([18, 505, 1517, 24, 56], [17, 5, 17, 8, 40], 18, 2, 64, 64, "e4m3", 200),
+    ([700, 333, 2000], [1, 3, 2], 8, 2, 128, 16, "int8", 100),
+    ([700, 90], [4, 7], 4, 1, 256, 16, "int8", 33),
+    ([700, 90], [1, 1], 8, 1, 128, 32, "e4m3", 0),
+    ([900, 640], [300, 70], 8, 1, 128, 16, "int8", 200),
+    ([900, 640], [300, 70], 2, 1, 64, 128, "e4m3", 0),
+])
+@pytest.mark.parametrize("span", [2, 12, 60])
+def test_scales_that_differ_from_page_to_page(lens, new, hq, hkv, d, page, kind, window, span):
+    w = World(lens, new, hkv, d, page, kind)
+    g = torch.Generator().manual_seed(span)
+    w.vs.mul_((2.0 ** torch.randint(-span, span + 1, w.vs.shape, generator=g)).to(DEV))
+    q = torch.randn(w.T, hq, d, generator=g).bfloat16().to(DEV)
+    _check_rows(w, q, w.cache.attend(0, w.batch, q, window=window), window)
+
+
 def test_strided_rows_and_scale():
     sl = _sl()
     w = World([300, 20], [1, 3], 2, 64, 16, "int8")
