@@ -535,7 +535,8 @@ int slora_kv8_read(const slora_kv8_cache* cache, const slora_kv8_batch* batch, c
  * kv_len - q_len + j, the last `window` of them when window > 0; q head h uses KV head h / (q_heads / kv_heads).
  *   p = softmax(scale * q . k), out = sum p v, lse = log sum exp (natural; may be NULL)
  * A query that sees no key gives 0 and lse -inf.  add_weights != 0: cache->weights += the p of every key, summed over
- * the step's queries and over the q heads of its KV head.
+ * the step's queries and over the q heads of its KV head.  Results do not depend on timing, with one exception: a page that
+ * several of the batch's sequences share gets their sums in no fixed order.
  * workspace: slora_kv8_attend_workspace_bytes(...) bytes of device memory, 16-byte aligned, contents irrelevant; calls
  * that may overlap on the GPU need workspaces of their own.
  */

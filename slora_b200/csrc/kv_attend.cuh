@@ -74,6 +74,7 @@ struct KvAttendArgs {
   int hq, group;
   int rows_per_block;  // 8 * NT
   int part_rows;       // rows of a block that any sequence has
+  int blocks;          // row blocks that a sequence may have
   float scale2;        // scale * log2(e)
   int window;
   int min_q, lim_q;    // sequences with min_q <= q_len <= lim_q are this launch's
@@ -883,8 +884,9 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const KvAttendArg
   }
 }
 
-// Accumulated attention weights from the stored scores: w[key] += sum over the rows of 2^(score - lse).  Runs of tiles as
-// in the attention; a lane takes a key of the tile and half of its rows.
+// Accumulated attention weights from the stored scores: w[key] += sum over the rows of 2^(score - lse).  Runs of tiles, as in
+// the attention but over (sequence, KV head) only: a warp adds up a tile's row blocks in their order and adds the sum to
+// the cache once, so that weights do not depend on timing either.  A lane takes a key of the tile and half of its rows.
 template <int D>
 __global__ void __launch_bounds__(kAttendThreads) kv_weights_kernel(const KvAttendArgs a) {
   __shared__ KvFind find;
@@ -893,8 +895,14 @@ __global__ void __launch_bounds__(kAttendThreads) kv_weights_kernel(const KvAtte
   pdl_wait();
   const int me = blockIdx.x * kAttendWarps + warp;
   const int runs = gridDim.x * kAttendWarps;
+  // units: what a sequence costs in the attention, a row block's worth of it
+  auto units = [&](const KvSeq& s) {
+    if (s.q < a.min_q || s.q > a.lim_q || s.q == 0) return 0ll;
+    const KvRange r = kv_tiles(s, a.window);
+    return static_cast<long long>(r.hi - r.lo + kAttendPiece) * a.c.hkv;
+  };
   const long long total = kv_find<kAttendWarps, kAttendWarps>(
-      a.b.n_seq, &find, [&](int i) { return kv_seq_cost(a, kv_seq(a.b, i)); },
+      a.b.n_seq, &find, [&](int i) { return units(kv_seq(a.b, i)); },
       [&](long long n, int k) { return static_cast<long long>(blockIdx.x * kAttendWarps + k) * kv_run(n, runs); });
   const long long run = kv_run(total, runs);
   long long u = me * run;
@@ -902,31 +910,40 @@ __global__ void __launch_bounds__(kAttendThreads) kv_weights_kernel(const KvAtte
   if (u >= u_end) return;
   int seq = find.seq[warp];
   long long seq_at = find.at[warp];
+  long long scores_at = seq_at;  // cost units of the attention before the sequence: where its scores start
+  if (a.blocks > 1) {
+    scores_at = 0;
+    for (int i = lane; i < seq; i += 32) scores_at += kv_seq_cost(a, kv_seq(a.b, i));
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) scores_at += __shfl_xor_sync(0xffffffffu, scores_at, d);
+  }
   KvSeq s = kv_seq(a.b, seq);
-  long long cost = kv_seq_cost(a, s);
+  long long n_units = units(s);
   const int key_in = lane & 15, half = lane >> 4;
   while (u < u_end) {
-    while (u >= seq_at + cost) {
-      seq_at += cost;
+    while (u >= seq_at + n_units) {
+      seq_at += n_units;
+      scores_at += kv_seq_cost(a, s);
       s = kv_seq(a.b, ++seq);
-      cost = kv_seq_cost(a, s);
+      n_units = units(s);
     }
     const KvRange range = kv_tiles(s, a.window);
     const int per = range.hi - range.lo, piece = per + kAttendPiece;
     const long long in = u - seq_at;
-    const int idx = in <= 0xffffffffll ? static_cast<int>(static_cast<uint32_t>(in) / static_cast<uint32_t>(piece)) : static_cast<int>(in / piece);
-    const int at = static_cast<int>(in - static_cast<long long>(idx) * piece);
+    const int head = in <= 0xffffffffll ? static_cast<int>(static_cast<uint32_t>(in) / static_cast<uint32_t>(piece)) : static_cast<int>(in / piece);
+    const int at = static_cast<int>(in - static_cast<long long>(head) * piece);
     const int until = static_cast<int>(min(static_cast<long long>(piece), at + (u_end - u)));
-    const long long base = u - at + kAttendPiece;  // unit of tile 0
     u += until - at;
-    const int rb = idx / a.c.hkv, head = idx - rb * a.c.hkv;
-    const int rows = min(a.rows_per_block, s.q * a.group - rb * a.rows_per_block);
-    // lane r holds lse of row r (32 rows at most)
-    float lse_l = kNegInf;
-    if (lane < rows) {
+    const int all_rows = s.q * a.group, blocks = (all_rows + a.rows_per_block - 1) / a.rows_per_block;
+    const float* const scores = a.scores + (scores_at + static_cast<long long>(head) * piece + kAttendPiece) * (a.part_rows * kAttendTile) + lane;
+    const long long block_step = static_cast<long long>(a.c.hkv) * piece * (a.part_rows * kAttendTile);
+    // lane r holds lse of row r of a block (32 rows at most)
+    auto lse_of = [&](int rb) {
       const int row = rb * a.rows_per_block + lane, j = row / a.group;
-      lse_l = a.lse[(static_cast<int64_t>(s.row) + j) * a.hq + head * a.group + row - j * a.group] * 1.4426950408889634f;
-    }
+      if (lane >= a.rows_per_block || row >= all_rows) return kNegInf;
+      return a.lse[(static_cast<int64_t>(s.row) + j) * a.hq + head * a.group + row - j * a.group] * 1.4426950408889634f;
+    };
+    float lse_l = lse_of(0);
     // 32 tiles at a time: lane l looks up where tile l's weights are
     const int end = min(until - kAttendPiece, (s.kv + kAttendTile - 1) / kAttendTile - range.lo);
     for (int i0 = max(at - kAttendPiece, 0); i0 < end; i0 += 32) {
@@ -937,20 +954,30 @@ __global__ void __launch_bounds__(kAttendThreads) kv_weights_kernel(const KvAtte
         if (p >= 0) place = static_cast<int>(((p * a.c.hkv + head) << a.c.shift) + (key_l & ((1 << a.c.shift) - 1)));
       }
       const int n = min(32, end - i0);
+      for (int i = 0; i < n; i += 4) {  // four tiles at a time: their loads overlap
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int rb = 0; rb < blocks; ++rb) {
+          if (blocks > 1) lse_l = lse_of(rb);
+          const int rows = min(a.rows_per_block, all_rows - rb * a.rows_per_block);
+          const float* const src = scores + rb * block_step + static_cast<int64_t>(i0 + i) * (a.part_rows * kAttendTile);
 #pragma unroll 4
-      for (int i = 0; i < n; ++i) {
-        const float* src = a.scores + (base + i0 + i) * (a.part_rows * kAttendTile) + lane;
-        float sum = 0.f;
-#pragma unroll 4
-        for (int r0 = 0; r0 < rows; r0 += 2) {
-          const float lse = __shfl_sync(0xffffffffu, lse_l, r0 + half);
-          const float x = r0 + half < rows ? src[r0 * kAttendTile] : kNegInf;
-          sum += lse > kNegInf ? ex2(x - lse) : 0.f;
+          for (int r0 = 0; r0 < rows; r0 += 2) {
+            const float lse = __shfl_sync(0xffffffffu, lse_l, r0 + half);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+              const float x = r0 + half < rows && i + t < n ? src[(t * a.part_rows + r0) * kAttendTile] : kNegInf;
+              sum[t] += lse > kNegInf ? ex2(x - lse) : 0.f;
+            }
+          }
         }
-        sum += __shfl_down_sync(0xffffffffu, sum, 16);
-        const int to = __shfl_sync(0xffffffffu, place, i);
-        // an atomic add only because sequences may share a page; a page of one sequence gets one add per token and row block
-        if (to >= 0 && half == 0 && (range.lo + i0 + i) * kAttendTile + key_in < s.kv && sum != 0.f) atomicAdd(a.c.w + to + key_in, sum);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          if (i + t >= n) break;
+          const float add = sum[t] + __shfl_down_sync(0xffffffffu, sum[t], 16);
+          const int to = __shfl_sync(0xffffffffu, place, i + t);
+          // an atomic add only because sequences may share a page (then in no fixed order); else one add per token
+          if (to >= 0 && half == 0 && (range.lo + i0 + i + t) * kAttendTile + key_in < s.kv && add != 0.f) atomicAdd(a.c.w + to + key_in, add);
+        }
       }
     }
   }
@@ -1031,7 +1058,7 @@ __global__ void __launch_bounds__(kAttendThreads, D <= 128 ? 4 : 2) kv_reweigh_k
       sum1 += __shfl_xor_sync(0xffffffffu, sum1, d);
     }
     if (t < 2) {
-      // an atomic add only because two sequences may share a page; a page of one sequence gets one add per token
+      // an atomic add only because sequences may share a page (then in no fixed order); else one add per token
       const int pos = in_page + g + 8 * t;
       const float add = t == 0 ? sum0 : sum1;
       if (key + g + 8 * t < s.kv && add != 0.f) atomicAdd(a.c.w + (ph << a.c.shift) + pos, add);

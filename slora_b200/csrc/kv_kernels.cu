@@ -208,6 +208,7 @@ constexpr int64_t kMaxScoreBytes = int64_t(1) << 29;
 
 struct AttendLayout {
   int nt, grid, part_rows;
+  int blocks;          // row blocks of a sequence, at most
   int split;           // q_len from which sequences are the prefill kernel's; above max_q: none
   int64_t pre_grid;    // its items, at most
   bool keep_scores;
@@ -233,6 +234,7 @@ AttendLayout attend_layout(const KvCache& c, const KvBatch& b, int hq, int add_w
   l.scores = l.lse + (add_weights ? up(static_cast<size_t>(b.T) * hq * sizeof(float)) : 0);
   // cost units of all pieces (see kv_attend.cuh), if every sequence were as long as the page table allows
   const int64_t blocks = (rows + 8 * l.nt - 1) / (8 * l.nt);
+  l.blocks = static_cast<int>(blocks);
   const double units = static_cast<double>(b.n_seq) * (static_cast<double>(b.max_tokens / kAttendTile) + 1 + kAttendPiece) * c.hkv * blocks;
   const double bytes = units * l.part_rows * kAttendTile * sizeof(float);
   l.keep_scores = add_weights && !pre && bytes <= static_cast<double>(kMaxScoreBytes);
@@ -465,6 +467,7 @@ int slora_kv8_attend(const slora_kv8_cache* cache, const slora_kv8_batch* batch,
   a.min_q = 0;
   a.lim_q = l.split - 1;
   a.part_rows = l.part_rows;
+  a.blocks = l.blocks;
   a.runs = l.grid;
   a.scores = l.keep_scores ? reinterpret_cast<float*>(ws + l.scores) : nullptr;
   a.part = reinterpret_cast<float*>(ws + l.part);

@@ -230,7 +230,8 @@ class KvCache8:
         of them when ``window`` > 0.  ``heads`` is a multiple of the cache's KV heads.  ``scale`` defaults to
         ``head_dim ** -0.5``; ``lse`` (FP32 ``[T, heads]``) receives the logarithm of the softmax's sum.  A query that sees
         nothing gives 0 and ``-inf``; rows that belong to no sequence are left as they are.  ``add_weights`` adds every
-        key's attention weight, summed over queries and the heads of its KV head, to ``weights[layer]``.
+        key's attention weight, summed over queries and the heads of its KV head, to ``weights[layer]`` (on pages that
+        several sequences share their sums arrive in no fixed order; all else does not depend on timing).
         C entry ``slora_kv8_attend``.
         """
         d, dtype = self.head_dim, q.dtype

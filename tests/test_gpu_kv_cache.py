@@ -373,6 +373,24 @@ def test_results_do_not_depend_on_timing():
         assert torch.equal(out, first[0]) and torch.equal(w.w, first[1])
 
 
+@pytest.mark.parametrize("lens,new,hq,hkv,d", [
+    ([3000, 2500, 700, 90] * 4, [6, 5, 7, 1] * 4, 16, 2, 128),     # up to 56 rows: four blocks of 16
+    ([3000, 2500, 700, 90] * 2, [6, 5, 7, 1] * 2, 8, 1, 256),      # seven blocks of eight
+    ([900, 300], [200, 70], 8, 1, 128),                            # scores computed again
+])
+def test_weights_do_not_depend_on_timing(lens, new, hq, hkv, d):
+    # added to what was there: with three addends or more their order would show
+    w = World(lens, new, hkv, d, 32, "int8")
+    q = torch.randn(w.T, hq, d, device=DEV, dtype=torch.bfloat16)
+    before, first = w.w.clone(), None
+    for _ in range(25):
+        w.w.copy_(before)
+        w.cache.attend(0, w.batch, q, add_weights=True)
+        first = w.w.clone() if first is None else first
+        assert torch.equal(w.w, first)
+    _run_attend(w, hq, "fp16", weights=True)
+
+
 def test_bad_tables_are_skipped_and_reported():
     sl = _sl()
     # the kernels check every entry before they use it: a bad sequence's rows stay as they are, a bad page's keys drop out
