@@ -9,6 +9,7 @@
 #include "kv_common.cuh"
 #include "kv_evict.cuh"
 #include "kv_prefill.cuh"
+#include "smem_limit.h"
 
 using namespace slora;
 
@@ -17,16 +18,24 @@ namespace {
 // `cluster`: CTAs along y that form a cluster (1: none).
 template <auto kernel, typename... A>
 int launch_cluster(int cluster, dim3 grid, int threads, size_t smem, cudaStream_t stream, const char* what, const A&... args) {
-  // more than 48 KB of shared memory (up to 16 of them static) is opted in to once per kernel, device and size
-  static std::atomic<size_t> opted[64];
-  int dev = 0;
-  if (smem > 32 * 1024 && (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64 || opted[dev].load(std::memory_order_relaxed) < smem)) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    if (e != cudaSuccess) {
-      cudaGetLastError();
-      return fail(SLORA_ERR_LAUNCH, "%s: %zu bytes of shared memory: %s", what, smem, cudaGetErrorString(e));
-    }
-    if (dev >= 0 && dev < 64) opted[dev].store(smem, std::memory_order_relaxed);
+  static SmemLimit limit;
+  int dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess) dev = -1;
+  cudaError_t refused = cudaSuccess;
+  const auto most = [&] {
+    int all = 0;
+    cudaFuncAttributes f;
+    refused = cudaFuncGetAttributes(&f, kernel);
+    if (refused == cudaSuccess) refused = cudaDeviceGetAttribute(&all, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev < 0 ? 0 : dev);
+    return refused == cudaSuccess ? static_cast<size_t>(all) - f.sharedSizeBytes : smem;
+  };
+  const auto set = [&](size_t bytes) {
+    if (refused == cudaSuccess) refused = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+    return refused == cudaSuccess;
+  };
+  if (!limit.allow(dev, smem, most, set)) {
+    cudaGetLastError();
+    return fail(SLORA_ERR_LAUNCH, "%s: %zu bytes of shared memory: %s", what, smem, cudaGetErrorString(refused));
   }
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));

@@ -2,12 +2,16 @@
 scalings, the cache's bookkeeping."""
 import ctypes
 import math
+import os
+import shutil
+import subprocess
 
 import pytest
 import torch
 
 import slora_b200 as sl
 from slora_b200 import _lib
+from tests.helpers import ROOT
 
 FAKE = 0x1000      # 16-byte aligned, never read: checks come first
 L = _lib.lib
@@ -194,3 +198,13 @@ def test_page_tables_whose_rows_overlap_are_refused():
         _table_stride(t.t())
     with pytest.raises(RuntimeError, match="contiguous rows"):
         _table_stride(t.int())
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="needs g++")
+def test_shared_memory_limit_of_two_threads(tmp_path):
+    """Launches that ask for different sizes do not lower a kernel's limit for one another (tests/smem_limit_model.cpp)."""
+    exe = str(tmp_path / "smem_limit")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-pthread", "-I", os.path.join(ROOT, "slora_b200", "csrc"),
+                    os.path.join(ROOT, "tests", "smem_limit_model.cpp"), "-o", exe], check=True)
+    res = subprocess.run([exe], capture_output=True, text=True, timeout=60)
+    assert res.returncode == 0, res.stdout
