@@ -92,7 +92,7 @@ __device__ __forceinline__ KvRange kv_tiles(const KvSeq& s, int window) {
   KvRange r;
   r.hi = s.q > 0 ? (s.kv + kAttendTile - 1) / kAttendTile : 0;
   r.lo = 0;
-  if (window > 0 && s.q > 0) r.lo = max(0, s.kv - s.q + 1 - window) / kAttendTile;
+  if (window > 0 && s.q > 0) r.lo = max(0, max(s.kv - s.q + 1, 0) - window) / kAttendTile;
   if (r.hi <= r.lo && s.q > 0) r.hi = r.lo + 1;  // no key at all: one empty tile, so that the rows are written
   return r;
 }
@@ -1043,7 +1043,7 @@ __global__ void __launch_bounds__(kAttendThreads, D <= 128 ? 4 : 2) kv_reweigh_k
         const int r = 8 * rb + 2 * t + x;
         if (r >= rows) continue;
         const int j = r / a.group;
-        const int to = s.kv - s.q + j + 1, from = a.window > 0 ? to - a.window : 0;
+        const int to = max(s.kv - s.q + j + 1, 0), from = a.window > 0 ? to - a.window : 0;
         const float lse = a.lse[(static_cast<int64_t>(s.row) + j) * a.hq + head * a.group + r - j * a.group];
         const float lse2 = lse * 1.4426950408889634f;
         const float f = q.mul[0][x] * ks;

@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_kernel(const KvAtte
   const int last_row = min(row0 + kPreRows, rows) - 1;
   const int base_to = s.kv - s.q + 1;  // keys that new token 0 sees end here
   const int key_end = max(base_to + last_row / a.group, 0);
-  const int key0 = a.window > 0 ? max(base_to + row0 / a.group - a.window, 0) / kPreKeys * kPreKeys : 0;
+  const int key0 = a.window > 0 ? max(max(base_to + row0 / a.group, 0) - a.window, 0) / kPreKeys * kPreKeys : 0;
   const int steps = key_end > key0 ? (key_end - key0 + kPreKeys - 1) / kPreKeys : 0;
 
   if (warp == kPreThreads / 32 - 1) {

@@ -34,6 +34,15 @@ def _table_stride(t):
     return max(t.stride(0), t.size(1))
 
 
+def _size(value, name):
+    """``value`` as the C interface takes it: an int from 0 to 2^31 - 1."""
+    if value < 0:
+        raise RuntimeError(f"{name} must not be negative")
+    if value > 0x7fffffff:
+        raise RuntimeError(f"{name}={value} is 2^31 or more")
+    return int(value)
+
+
 class KvBatch:
     """The sequences of one step, as device tables; made once per step and used by every layer.
 
@@ -55,11 +64,9 @@ class KvBatch:
                 raise RuntimeError(f"{name} must be a contiguous int32 tensor with one entry per sequence")
             if t.device != page_table.device:
                 raise RuntimeError(f"{name} and page_table lie on different devices")
-        if max_q_len < 0 or (max_kv_len is not None and max_kv_len < 0):
-            raise RuntimeError("max_q_len and max_kv_len must not be negative")
         self.page_table, self.kv_len, self.q_start, self.q_len = page_table, kv_len, q_start, q_len
-        self.max_q_len = int(max_q_len)
-        self.max_kv_len = None if max_kv_len is None else int(max_kv_len)
+        self.max_q_len = _size(max_q_len, "max_q_len")
+        self.max_kv_len = None if max_kv_len is None else _size(min(max_kv_len, 0x7fffffff), "max_kv_len")
         self._status = torch.zeros((1,), dtype=torch.int32, device=page_table.device)
         self._fields = [page_table.data_ptr(), stride, kv_len.data_ptr(), q_start.data_ptr(), q_len.data_ptr(),
                         self._status.data_ptr(), n, page_table.size(1), self.max_q_len]
@@ -212,14 +219,13 @@ class KvCache8:
         """Tokens ``first[b] .. first[b] + count`` of each sequence (default: from 0) as the 16-bit values they stand for:
         ``(k, v)`` ``[n, count, kv_heads, head_dim]``, zero at and beyond ``kv_len``.  C entry ``slora_kv8_read``."""
         code = _lib.dtype_code(dtype)
-        if count < 0:
-            raise RuntimeError("count must not be negative")
+        count = _size(count, "count")
         ctx = _lib.device_of(self.k[layer], batch.kv_len, first)
         if first is not None and (first.dtype != torch.int32 or first.numel() != batch.n_seq or not first.is_contiguous()):
             raise RuntimeError("first must be a contiguous int32 tensor with one entry per sequence")
-        shape = (batch.n_seq, int(count), self.kv_heads, self.head_dim)
+        shape = (batch.n_seq, count, self.kv_heads, self.head_dim)
         k, v = torch.empty(shape, dtype=dtype, device=self.device), torch.empty(shape, dtype=dtype, device=self.device)
-        _lib.call(ctx, _lib.lib.slora_kv8_read, self._ptr[layer], batch._ptr(self.page_tokens), _lib.ptr(first), int(count),
+        _lib.call(ctx, _lib.lib.slora_kv8_read, self._ptr[layer], batch._ptr(self.page_tokens), _lib.ptr(first), count,
                   k.data_ptr(), v.data_ptr(), code)
         return k, v
 
@@ -242,8 +248,7 @@ class KvCache8:
             raise RuntimeError(f"q has {heads} heads, which is no multiple of the cache's {self.kv_heads}")
         if add_weights and self.weights is None:
             raise RuntimeError("add_weights needs a cache with track_weights")
-        if window < 0:
-            raise RuntimeError("window must not be negative")
+        window = _size(window, "window")
         code = _lib.dtype_code(dtype)
         if out is None:
             out = torch.empty(shape, dtype=dtype, device=q.device)
@@ -264,7 +269,7 @@ class KvCache8:
                 self._ptr[layer], batch._ptr(self.page_tokens), tokens, heads, int(add_weights)), 16)
         ws = torch.empty(need, dtype=torch.uint8, device=q.device)
         _lib.call(ctx, _lib.lib.slora_kv8_attend, self._ptr[layer], batch._ptr(self.page_tokens), q.data_ptr(), q_stride, tokens,
-                  heads, out.data_ptr(), o_stride, _lib.ptr(lse), d ** -0.5 if scale is None else float(scale), int(window),
+                  heads, out.data_ptr(), o_stride, _lib.ptr(lse), d ** -0.5 if scale is None else float(scale), window,
                   int(add_weights), ws.data_ptr(), need, code)
         return out
 
@@ -284,10 +289,11 @@ class KvCache8:
         table = batch.page_table if dest is None else dest.page_table
         if table.size(0) != batch.n_seq:
             raise RuntimeError("dest must have one row of pages per sequence")
-        if budget < 1 or recent < 0 or sink < 0 or recent + sink > budget:
+        budget, recent, sink = _size(budget, "budget"), _size(recent, "recent"), _size(sink, "sink")
+        if budget < 1 or recent + sink > budget:
             raise RuntimeError("budget must hold the sink and the recent tokens")
         ctx = _lib.device_of(self.k[layer], batch.kv_len, table)
-        kept = torch.empty((batch.n_seq, self.kv_heads, int(budget)), dtype=torch.int32, device=self.device)
-        _lib.call(ctx, _lib.lib.slora_kv8_evict, self._ptr[layer], batch._ptr(self.page_tokens), int(budget), int(recent),
-                  int(sink), kept.data_ptr(), table.data_ptr(), _table_stride(table), table.size(1))
+        kept = torch.empty((batch.n_seq, self.kv_heads, budget), dtype=torch.int32, device=self.device)
+        _lib.call(ctx, _lib.lib.slora_kv8_evict, self._ptr[layer], batch._ptr(self.page_tokens), budget, recent,
+                  sink, kept.data_ptr(), table.data_ptr(), _table_stride(table), table.size(1))
         return kept

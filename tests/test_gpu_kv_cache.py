@@ -197,6 +197,40 @@ def test_queries_that_see_nothing():
     assert (out[r:r + 10] == 0).all() and (lse[r:r + 10] == -math.inf).all() and (lse[r + 10:r + 40] > -100).all()
 
 
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 3])
+def test_the_widest_window_is_none(window):
+    # more new tokens than cached ones: the first queries precede position 0
+    w = World([1, 3, 60, 200], [4, 90, 70, 130], 2, 128, 16, "int8")
+    q = torch.randn(w.T, 4, 128, device=DEV).half()
+    before = w.w.clone()
+    want = w.cache.attend(0, w.batch, q, out=torch.zeros_like(q), add_weights=True)
+    weights = w.w.clone()
+    w.w.copy_(before)
+    got = w.cache.attend(0, w.batch, q, out=torch.zeros_like(q), window=window, add_weights=True)
+    assert torch.equal(got, want) and torch.equal(w.w, weights) and (got != 0).any()
+    few = World([1, 3, 60], [4, 9, 2], 2, 128, 16, "int8")
+    q = torch.randn(few.T, 4, 128, device=DEV).half()
+    assert torch.equal(few.cache.attend(0, few.batch, q, out=torch.zeros_like(q)),
+                       few.cache.attend(0, few.batch, q, out=torch.zeros_like(q), window=window))
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    # the C interface takes ints: 2^32 + 5 would arrive as 5
+    sl = _sl()
+    w = World([40], [1], 2, 64, 16, "int8")
+    q = torch.randn(w.T, 4, 64, device=DEV).half()
+    b = w.batch
+    big = 2 ** 32 + 5
+    for call in (lambda: w.cache.attend(0, b, q, window=big), lambda: w.cache.attend(0, b, q, window=2 ** 31),
+                 lambda: sl.KvBatch(b.page_table, b.kv_len, b.q_start, b.q_len, big),
+                 lambda: w.cache.evict(0, b, big, 4), lambda: w.cache.read(0, b, torch.float16, big)):
+        with pytest.raises(RuntimeError, match="2.31 or more"):
+            call()
+    for call in (lambda: w.cache.attend(0, b, q, window=-1), lambda: w.cache.evict(0, b, 16, -1), lambda: w.cache.evict(0, b, 16, 1, sink=-1)):
+        with pytest.raises(RuntimeError, match="must not be negative"):
+            call()
+
+
 def test_nan_and_inf_in_q_stay_in_their_rows():
     w = World([100, 500], [1, 2], 2, 128, 16, "int8")
     g = torch.Generator().manual_seed(0)
