@@ -17,7 +17,7 @@ import torch
 
 from . import _lib
 from .kv_cache import KvCache8
-from .rotary import RotaryTable, _positions, rotary
+from .rotary import RotaryTable, _rotary_call
 
 
 class BatchPlan:
@@ -196,7 +196,8 @@ class LoraBatchOps:
         ``rope=(table, positions)`` with a :class:`~slora_b200.RotaryTable` and the tokens' positions takes any of its
         layouts and scalings; ``kv_dest=(cache, batch)`` with a :class:`~slora_b200.KvCache8` and the step's
         :class:`~slora_b200.KvBatch` puts the new k and v into the layer's 8-bit pages (turned first when ``rope`` is
-        given).  Both run as one launch behind the expand; q, k and v hold base plus delta in place (q turned).
+        given).  Both run behind the expand, in one launch (two when sequences have more than four new tokens and q is
+        turned); q, k and v hold base plus delta in place (q turned).  A call that is refused changes nothing.
         """
         kb, vb, rows, stride = self._common(layer_id)
         _lib.require_cuda(x, q, k, v)
@@ -251,16 +252,19 @@ class LoraBatchOps:
             raise RuntimeError("an 8-bit cache takes rope=(RotaryTable, positions) of its head_dim")
         if kv_dest is not None and (not isinstance(kv_dest[0], KvCache8) or kv_dest[0].head_dim != head_dim):
             raise RuntimeError("a RotaryTable goes with kv_dest=(KvCache8, KvBatch) of its head_dim, or none")
+        # every check before the deltas are added: a call that raises has changed nothing
         heads = [t.view(t.size(0), -1, head_dim) for t in (q, k, v)]
-        if rope is not None:
-            _lib.require_cuda(rope[1])
-            _positions(rope[1], x.size(0))
-        self.lora_get_qkv(layer_id, x, q, k, v)
+        if any(t.size(0) != x.size(0) for t in heads):
+            raise RuntimeError("q, k and v must have x's tokens")
+        if any(t.data_ptr() % 16 or t.stride(0) % 8 for t in (heads if kv_dest is not None else heads[:2])):
+            raise RuntimeError("rows of q, k and v are not 16-byte aligned")
         if kv_dest is None:
-            rotary(rope[0], rope[1], heads[0], heads[1])
+            call = _rotary_call(rope[0], rope[1], heads[0], heads[1])[1]
         else:
             cache, batch = kv_dest
-            cache.append(layer_id, batch, heads[1], heads[2], q=heads[0] if rope is not None else None, rope=rope)
+            call = cache._append_call(layer_id, batch, heads[1], heads[2], heads[0] if rope is not None else None, rope)[1]
+        self.lora_get_qkv(layer_id, x, q, k, v)
+        _lib.call(*call)
         return q
 
     def lora_get_o(self, layer_id, x, o):

@@ -179,6 +179,12 @@ class KvCache8:
         raises it, the page's older values are rounded to the new scale.  A page that is appended to must belong to one
         sequence only.  C entry ``slora_kv8_append``.
         """
+        q_out, call = self._append_call(layer, batch, k, v, q, rope, q_out)
+        _lib.call(*call)
+        return q_out
+
+    def _append_call(self, layer, batch, k, v, q=None, rope=None, q_out=None):
+        """The checks of :meth:`append`, and what is left to do as the arguments of ``_lib.call``."""
         d, dtype = self.head_dim, k.dtype
         table = positions = None
         if rope is not None:
@@ -211,9 +217,9 @@ class KvCache8:
             qp, qop, q_heads = q.data_ptr(), q_out.data_ptr(), q_shape[1]
         elif q_out is not None:
             raise RuntimeError("q_out without q")
-        _lib.call(ctx, _lib.lib.slora_kv8_append, self._ptr[layer], batch._ptr(self.page_tokens), k.data_ptr(), v.data_ptr(),
-                  k_stride, v_stride, shape[0], qp, qop, q_heads, q_stride, qo_stride, pos, turns, rot, factor, layout, _lib.dtype_code(dtype))
-        return q_out
+        return q_out, (ctx, _lib.lib.slora_kv8_append, self._ptr[layer], batch._ptr(self.page_tokens), k.data_ptr(), v.data_ptr(),
+                       k_stride, v_stride, shape[0], qp, qop, q_heads, q_stride, qo_stride, pos, turns, rot, factor, layout,
+                       _lib.dtype_code(dtype))
 
     def read(self, layer, batch, dtype, count, first=None):
         """Tokens ``first[b] .. first[b] + count`` of each sequence (default: from 0) as the 16-bit values they stand for:

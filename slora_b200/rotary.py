@@ -127,6 +127,13 @@ def rotary(table, positions, q, k=None, q_out=None, k_out=None, inverse=False):
     In place unless ``q_out`` / ``k_out`` are given; returns ``(q_out, k_out)``.  ``inverse=True`` turns back (the
     gradient's direction).  C entry ``slora_rotary``.
     """
+    out, call = _rotary_call(table, positions, q, k, q_out, k_out, inverse)
+    _lib.call(*call)
+    return out
+
+
+def _rotary_call(table, positions, q, k=None, q_out=None, k_out=None, inverse=False):
+    """The checks of :func:`rotary`, and what is left to do as the arguments of ``_lib.call``."""
     ctx = _lib.device_of(q, positions, table.turns, k, q_out, k_out)
     d, dtype = table.head_dim, q.dtype
     shape, q_stride = _rows(q, "q", d)
@@ -151,7 +158,6 @@ def rotary(table, positions, q, k=None, q_out=None, k_out=None, inverse=False):
         k_heads, kp, kop = k_shape[1], k.data_ptr(), k_out.data_ptr()
     elif k_out is not None:
         raise RuntimeError("k_out without k")
-    _lib.call(ctx, _lib.lib.slora_rotary, q_out.data_ptr(), kop, q.data_ptr(), kp, shape[0], shape[1], k_heads, d,
-              table.rotary_dim, qo_stride, ko_stride, q_stride, k_stride, positions.data_ptr(), table.turns_ptr, table.factor,
-              table.layout_code, int(inverse), _lib.dtype_code(dtype))
-    return q_out, k_out
+    return (q_out, k_out), (ctx, _lib.lib.slora_rotary, q_out.data_ptr(), kop, q.data_ptr(), kp, shape[0], shape[1], k_heads, d,
+                            table.rotary_dim, qo_stride, ko_stride, q_stride, k_stride, positions.data_ptr(), table.turns_ptr,
+                            table.factor, table.layout_code, int(inverse), _lib.dtype_code(dtype))

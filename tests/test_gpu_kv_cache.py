@@ -1031,3 +1031,42 @@ def test_lora_layer_with_the_cache(kv, head_dim):
     for bad in (dict(rope=(table, pos), kv_dest=(pos, k, v)), dict(rope=(table, pos[1:])), dict(rope=(sl.RotaryTable(256), pos))):
         with pytest.raises(RuntimeError):
             ops.lora_get_qkv(0, wl.x_qkv[0], q, k, v, head_dim=head_dim, **bad)
+
+
+def test_a_refused_layer_changes_nothing():
+    """``lora_get_qkv`` with a cache or a table that does not fit raises before it adds the deltas."""
+    from slora_b200.workloads import build_workload
+    sl = _sl()
+    wl = build_workload(5, pool_rows=8192, n_adapters=12, decode_tokens=50, hidden=1024, h_kv=256).to(DEV)
+    T = wl.T
+    ops = sl.LoraBatchOps(wl.a_start, wl.a_len, wl.a_loc, wl.a_scaling, wl.pools_a, wl.pools_b, wl.max_rank)
+    ops.prepare(wl.ids)
+    g = torch.Generator().manual_seed(2)
+    base = [torch.randn(T, n, generator=g).to(wl.dtype).to(DEV) for n in (1024, 256, 256)]
+    table, pos = sl.RotaryTable(128), torch.arange(T, device=DEV)
+    w = World([9] * T, [1] * T, 2, 128, 16, "int8")
+    w.batch.q_start.copy_(torch.arange(T, dtype=torch.int32))
+    other_heads = World([9] * T, [1] * T, 3, 128, 16, "int8").cache
+    wide = torch.zeros(T, 1024 + 4, dtype=wl.dtype, device=DEV)
+    cases = [dict(rope=(table, pos), kv_dest=(other_heads, w.batch)),           # the cache has other KV heads
+             dict(rope=(table, pos.cpu()), kv_dest=(w.cache, w.batch)), dict(rope=(table, pos.cpu())),
+             dict(rope=(table, pos.int())), dict(kv_dest=(other_heads, w.batch)),
+             dict(rope=(table, pos), kv_dest=(w.cache, w.batch), q=wide[:, :1024]), dict(rope=(table, pos), q=wide[:, 4:])]
+    cases.append(dict(rope=(table, pos), kv_dest=(sl.KvCache8(4, 16, 2, 128, layer_num=1), w.batch), layer=1))   # no such layer
+    for case in cases:
+        q, k, v = (b.clone() for b in base)
+        if "q" in case:
+            case["q"].copy_(q)
+            q = case.pop("q")
+        layer = case.pop("layer", 0)
+        if layer and len(ops.key_buffer) <= layer:
+            continue
+        before = w.k8.view(torch.uint8).clone()
+        with pytest.raises((RuntimeError, IndexError)):
+            ops.lora_get_qkv(layer, wl.x_qkv[0], q, k, v, **case)
+        torch.cuda.synchronize()
+        assert torch.equal(q, base[0]) and torch.equal(k, base[1]) and torch.equal(v, base[2])
+        assert torch.equal(w.k8.view(torch.uint8), before)
+    q, k, v = (b.clone() for b in base)
+    ops.lora_get_qkv(0, wl.x_qkv[0], q, k, v, rope=(table, pos), kv_dest=(w.cache, w.batch))
+    assert not torch.equal(q, base[0]) and w.batch.status() == 0
