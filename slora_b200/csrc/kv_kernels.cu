@@ -501,7 +501,6 @@ int slora_kv8_evict(const slora_kv8_cache* cache, const slora_kv8_batch* batch, 
     return fail(SLORA_ERR_SHAPE, "evict: %d destination pages cannot hold %lld tokens", dest_pages, (long long)longest);
   const int64_t heads = static_cast<int64_t>(a.b.n_seq) * a.c.hkv;
   if (heads > 0x7fffffff) return fail(SLORA_ERR_SHAPE, "evict: too many heads");
-  if (a.c.n_pages > (0x7fffffff >> a.c.shift) / a.c.hkv) return fail(SLORA_ERR_SHAPE, "evict: 2^31 weights or more");
   a.budget = budget;
   a.recent = recent;
   a.sink = sink;

@@ -107,6 +107,16 @@ def test_evict_is_refused():
     assert _evict(_cache(n_pages=2 ** 31)) == -4 and _evict(_cache(n_pages=2 ** 62)) == -4
 
 
+def test_a_layer_has_less_than_two_to_the_31_rows():
+    # rows (tokens x heads) are counted in 32 bits: the largest cache passes these checks (no sequences: nothing is launched)
+    none = _batch(n_seq=0)
+    for n, page, heads in ((2 ** 26, 16, 2), (2 ** 31 // 128 // 3 + 1, 128, 3), (2 ** 15, 128, 512)):
+        fits, over = _cache(n_pages=n - 1, page_tokens=page, kv_heads=heads), _cache(n_pages=n, page_tokens=page, kv_heads=heads)
+        assert (n - 1) * page * heads < 2 ** 31 <= n * page * heads
+        assert _append(fits, none) == 0 and _attend(fits, none, hq=heads) == 0 and _evict(fits, none) == 0
+        assert _append(over, none) == -4 and _attend(over, none, hq=heads) == -4 and _evict(over, none) == -4
+
+
 def test_read_is_refused():
     c, b = ctypes.byref(_cache()), ctypes.byref(_batch())
     assert L.slora_kv8_read(c, b, 0, 4, FAKE, FAKE, 9, 0) == -3
