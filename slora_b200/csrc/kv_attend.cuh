@@ -774,113 +774,107 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const KvAttendArg
   const int tid = threadIdx.x;
   pdl_launch_dependents();
   pdl_wait();
-  {
-    const int me = blockIdx.x;
-    const int4 rec = *reinterpret_cast<const int4*>(a.rec + 4 * static_cast<int64_t>(me));
-    if (rec.x < 0) return;
-    const KvSeq s = kv_seq(a.b, rec.x);
-    const int rb = rec.y / a.c.hkv, head = rec.y - rb * a.c.hkv;
-    const int rows = min(a.rows_per_block, s.q * a.group - rb * a.rows_per_block);
-    const int64_t words = static_cast<int64_t>(a.part_rows) * (D + 4);
-    auto part_of = [&](int p) { return a.part + (p == 0 ? rec.z : 2 * (me + p)) * words; };
-    const int e = tid % kLanes, team = tid / kLanes;
-    const int groups = max(kTeams / rows, 1);  // teams that share a row's parts
-    const int r_me = team % rows, grp = team / rows;
-    // rows <= 32 and teams >= 8: with more rows than teams a team takes several rows in turn
-    for (int r0 = 0; r0 < rows; r0 += kTeams) {
-      const int r = groups > 1 || kTeams >= rows ? r_me : r0 + team;
-      const bool on = groups > 1 || kTeams >= rows ? grp < groups : r < rows;
-      float4 o[kVec];
+  const int me = blockIdx.x;
+  const int4 rec = *reinterpret_cast<const int4*>(a.rec + 4 * static_cast<int64_t>(me));
+  if (rec.x < 0) return;
+  const KvSeq s = kv_seq(a.b, rec.x);
+  const int rb = rec.y / a.c.hkv, head = rec.y - rb * a.c.hkv;
+  const int rows = min(a.rows_per_block, s.q * a.group - rb * a.rows_per_block);
+  const int64_t words = static_cast<int64_t>(a.part_rows) * (D + 4);
+  auto part_of = [&](int p) { return a.part + (p == 0 ? rec.z : 2 * (me + p)) * words; };
+  const int e = tid % kLanes, team = tid / kLanes;
+  static_assert(8 * (256 / D) <= kTeams, "a team has one row of the block at most (attend_tiles)");
+  const int groups = kTeams / rows;  // teams that share a row's parts
+  const int r = team % rows, grp = team / rows;
+  const bool on = grp < groups;
+  float4 o[kVec];
 #pragma unroll
-      for (int v = 0; v < kVec; ++v) o[v] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (tid < 32) {
-        sh_m[tid] = kNoMax;
-        sh_l[tid] = 0.f;
+  for (int v = 0; v < kVec; ++v) o[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (tid < 32) {
+    sh_m[tid] = kNoMax;
+    sh_l[tid] = 0.f;
+  }
+  for (int p0 = 0; p0 < rec.w; p0 += kJoinParts) {
+    const int np = min(kJoinParts, rec.w - p0);
+    __syncthreads();
+    // one warp per row: the weights of this stretch of parts relative to the maximum so far
+    for (int rr = tid >> 5; rr < rows; rr += kJoinThreads / 32) {
+      float m = kNoMax;
+      float2 ml[kJoinParts / 32];
+#pragma unroll
+      for (int k = 0; k < kJoinParts / 32; ++k) {
+        const int p = k * 32 + (tid & 31);
+        ml[k] = make_float2(kNoMax, 0.f);
+        if (p < np) ml[k] = *reinterpret_cast<const float2*>(part_of(p0 + p) + static_cast<int64_t>(a.part_rows) * D + 2 * rr);
+        m = fmaxf(m, ml[k].x);
       }
-      for (int p0 = 0; p0 < rec.w; p0 += kJoinParts) {
-        const int np = min(kJoinParts, rec.w - p0);
-        __syncthreads();
-        // one warp per row: the weights of this stretch of parts relative to the maximum so far
-        for (int rr = tid >> 5; rr < rows; rr += kJoinThreads / 32) {
-          float m = kNoMax;
-          float2 ml[kJoinParts / 32];
 #pragma unroll
-          for (int k = 0; k < kJoinParts / 32; ++k) {
-            const int p = k * 32 + (tid & 31);
-            ml[k] = make_float2(kNoMax, 0.f);
-            if (p < np) ml[k] = *reinterpret_cast<const float2*>(part_of(p0 + p) + static_cast<int64_t>(a.part_rows) * D + 2 * rr);
-            m = fmaxf(m, ml[k].x);
-          }
+      for (int d = 1; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+      const float was = sh_m[rr], now = fmaxf(was, m);
+      float l = 0.f;
 #pragma unroll
-          for (int d = 1; d < 32; d <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-          const float was = sh_m[rr], now = fmaxf(was, m);
-          float l = 0.f;
+      for (int k = 0; k < kJoinParts / 32; ++k) {
+        const float f = ex2(ml[k].x - now);
+        sh_f[rr][k * 32 + (tid & 31)] = f;
+        l += f * ml[k].y;
+      }
 #pragma unroll
-          for (int k = 0; k < kJoinParts / 32; ++k) {
-            const float f = ex2(ml[k].x - now);
-            sh_f[rr][k * 32 + (tid & 31)] = f;
-            l += f * ml[k].y;
-          }
+      for (int d = 1; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+      if ((tid & 31) == 0) {
+        const float keep = ex2(was - now);
+        sh_keep[rr] = keep;
+        sh_l[rr] = sh_l[rr] * keep + l;
+        sh_m[rr] = now;
+      }
+      __syncwarp();
+    }
+    __syncthreads();
+    if (on) {
+      const float keep = sh_keep[r];
 #pragma unroll
-          for (int d = 1; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
-          if ((tid & 31) == 0) {
-            const float keep = ex2(was - now);
-            sh_keep[rr] = keep;
-            sh_l[rr] = sh_l[rr] * keep + l;
-            sh_m[rr] = now;
-          }
-          __syncwarp();
-        }
-        __syncthreads();
-        if (on) {
-          const float keep = sh_keep[r];
-#pragma unroll
-          for (int v = 0; v < kVec; ++v) o[v].x *= keep, o[v].y *= keep, o[v].z *= keep, o[v].w *= keep;
+      for (int v = 0; v < kVec; ++v) o[v].x *= keep, o[v].y *= keep, o[v].z *= keep, o[v].w *= keep;
 #pragma unroll 8
-          for (int p = grp; p < np; p += groups) {
-            const float f = sh_f[r][p];
-            const float* part = part_of(p0 + p) + r * D;
-#pragma unroll
-            for (int v = 0; v < kVec; ++v) {
-              const float4 y = *reinterpret_cast<const float4*>(part + 4 * (v * kLanes + e));
-              if (f != 0.f) {
-                o[v].x += y.x * f;
-                o[v].y += y.y * f;
-                o[v].z += y.z * f;
-                o[v].w += y.w * f;
-              }
-            }
-          }
-        }
-      }
-#pragma unroll
-      for (int v = 0; v < kVec; ++v) sh_o[v * kJoinThreads + tid] = o[v];
-      __syncthreads();
-      if (on && grp == 0) {
-        const float l = sh_l[r];
-        const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-        const int row = rb * a.rows_per_block + r, j = row / a.group, h = head * a.group + row - j * a.group;
-        const int64_t token = static_cast<int64_t>(s.row) + j;
+      for (int p = grp; p < np; p += groups) {
+        const float f = sh_f[r][p];
+        const float* part = part_of(p0 + p) + r * D;
 #pragma unroll
         for (int v = 0; v < kVec; ++v) {
-          for (int k = 1; k < groups; ++k) {
-            const float4 y = sh_o[v * kJoinThreads + tid + k * rows * kLanes];
-            o[v].x += y.x, o[v].y += y.y, o[v].z += y.z, o[v].w += y.w;
+          const float4 y = *reinterpret_cast<const float4*>(part + 4 * (v * kLanes + e));
+          if (f != 0.f) {
+            o[v].x += y.x * f;
+            o[v].y += y.y * f;
+            o[v].z += y.z * f;
+            o[v].w += y.w * f;
           }
-          union {
-            uint2 u;
-            T e[4];
-          } p;
-          p.e[0] = from_f32<T>(o[v].x * inv);
-          p.e[1] = from_f32<T>(o[v].y * inv);
-          p.e[2] = from_f32<T>(o[v].z * inv);
-          p.e[3] = from_f32<T>(o[v].w * inv);
-          *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + token * a.out_stride + h * D + 4 * (v * kLanes + e)) = p.u;
         }
-        if (a.lse && e == 0) a.lse[token * a.hq + h] = l == 0.f ? kNegInf : (sh_m[r] + log2f(l)) * 0.69314718055994531f;
       }
-      __syncthreads();
     }
+  }
+#pragma unroll
+  for (int v = 0; v < kVec; ++v) sh_o[v * kJoinThreads + tid] = o[v];
+  __syncthreads();
+  if (on && grp == 0) {
+    const float l = sh_l[r];
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+    const int row = rb * a.rows_per_block + r, j = row / a.group, h = head * a.group + row - j * a.group;
+    const int64_t token = static_cast<int64_t>(s.row) + j;
+#pragma unroll
+    for (int v = 0; v < kVec; ++v) {
+      for (int k = 1; k < groups; ++k) {
+        const float4 y = sh_o[v * kJoinThreads + tid + k * rows * kLanes];
+        o[v].x += y.x, o[v].y += y.y, o[v].z += y.z, o[v].w += y.w;
+      }
+      union {
+        uint2 u;
+        T e[4];
+      } p;
+      p.e[0] = from_f32<T>(o[v].x * inv);
+      p.e[1] = from_f32<T>(o[v].y * inv);
+      p.e[2] = from_f32<T>(o[v].z * inv);
+      p.e[3] = from_f32<T>(o[v].w * inv);
+      *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + token * a.out_stride + h * D + 4 * (v * kLanes + e)) = p.u;
+    }
+    if (a.lse && e == 0) a.lse[token * a.hq + h] = l == 0.f ? kNegInf : (sh_m[r] + log2f(l)) * 0.69314718055994531f;
   }
 }
 
