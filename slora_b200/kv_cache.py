@@ -14,6 +14,7 @@ One layer of a step, between ``LoraBatchOps.lora_get_qkv`` and ``lora_get_o``::
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 import torch
@@ -271,8 +272,9 @@ class KvCache8:
         key = (self._key, tokens, heads, bool(add_weights))
         need = batch.workspaces.get(key)
         if need is None:
-            need = batch.workspaces[key] = max(_lib.lib.slora_kv8_attend_workspace_bytes(
-                self._ptr[layer], batch._ptr(self.page_tokens), tokens, heads, int(add_weights)), 16)
+            with ctx or contextlib.nullcontext():    # it goes by the device's SMs
+                need = batch.workspaces[key] = max(_lib.lib.slora_kv8_attend_workspace_bytes(
+                    self._ptr[layer], batch._ptr(self.page_tokens), tokens, heads, int(add_weights)), 16)
         ws = torch.empty(need, dtype=torch.uint8, device=q.device)
         _lib.call(ctx, _lib.lib.slora_kv8_attend, self._ptr[layer], batch._ptr(self.page_tokens), q.data_ptr(), q_stride, tokens,
                   heads, out.data_ptr(), o_stride, _lib.ptr(lse), d ** -0.5 if scale is None else float(scale), window,

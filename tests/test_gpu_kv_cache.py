@@ -920,6 +920,44 @@ def test_streams_and_graphs():
     _check_attend(w, q_out, out, None, None, None)
 
 
+def test_calls_run_on_the_device_of_their_tensors(monkeypatch):
+    # as on a machine with several GPUs: whatever goes by the current device happens with the tensors' one made current
+    from slora_b200 import _lib
+    sl = _sl()
+    w = World([300, 45], [1, 1], 2, 128, 16, "int8")
+    table, pos = sl.RotaryTable(128), torch.zeros(w.T, dtype=torch.int64, device=DEV)
+    q, x = torch.randn(w.T, 8, 128, device=DEV).half(), torch.randn(w.T, 2, 128, device=DEV).half()
+    inside, called = [0], []
+
+    class Current:
+        def __enter__(self):
+            inside[0] += 1
+
+        def __exit__(self, *args):
+            inside[0] -= 1
+
+    class Library:
+        def __getattr__(self, name):
+            called.append(name)
+            fn = getattr(library, name)
+
+            def call(*args):
+                assert inside[0] == 1, name
+                return fn(*args)
+            return call
+
+    library = _lib.lib
+    monkeypatch.setattr(_lib, "lib", Library())
+    monkeypatch.setattr(_lib, "device_of", lambda *tensors: Current())
+    w.cache.append(0, w.batch, x, x, q=q, rope=(table, pos))
+    w.cache.attend(0, w.batch, q, add_weights=True)
+    w.cache.read(0, w.batch, torch.float16, 4)
+    w.cache.evict(0, w.batch, 32, 4)
+    sl.rotary(table, pos, q)
+    assert set(called) == {"slora_kv8_append", "slora_kv8_attend_workspace_bytes", "slora_kv8_attend", "slora_kv8_read", "slora_kv8_evict",
+                           "slora_rotary"}
+
+
 def test_two_calls_at_once():
     w = World([2000, 45, 800], [1, 1, 1], 2, 128, 16, "int8")
     qs = [torch.randn(w.T, 8, 128, device=DEV).half() for _ in range(4)]
