@@ -491,7 +491,7 @@ typedef struct slora_kv8_batch { /* the sequences of a step; every table is devi
 
 /*
  * Rotary embedding of q [T][q_heads][head_dim] and k [T][k_heads][head_dim] (either may be NULL with 0 heads; rows
- * *_stride elements apart, heads contiguous) into q_out / k_out (which may be q / k).  The first `rot` elements of a head
+ * *_stride elements apart, heads contiguous) into q_out / k_out (which may be q / k, but not overlap them otherwise).  The first `rot` elements of a head
  * are turned, the others copied.  Pair i: elements (i, i + rot / 2) with layout 0 ("half", the reference's
  * rotary_emb_fwd, slora/models/llama/triton_kernel/rotary_emb.py:8-71), (2i, 2i + 1) with layout 1 ("interleaved").
  *   angle = 2 pi positions[t] turns[i] (turns: rot / 2 doubles, device), (c, s) = factor * (cos, sin) of the angle,
@@ -537,6 +537,7 @@ int slora_kv8_read(const slora_kv8_cache* cache, const slora_kv8_batch* batch, c
  * A query that sees no key gives 0 and lse -inf.  add_weights != 0: cache->weights += the p of every key, summed over
  * the step's queries and over the q heads of its KV head.  Results do not depend on timing, with one exception: a page that
  * several of the batch's sequences share gets their sums in no fixed order.
+ * out may be q unless add_weights is set, which reads q again.
  * workspace: slora_kv8_attend_workspace_bytes(...) bytes of device memory, 16-byte aligned, contents irrelevant; calls
  * that may overlap on the GPU need workspaces of their own.
  */

@@ -149,6 +149,23 @@ int check_rows(const void* p, int64_t stride, int64_t width, int64_t T, const ch
   return SLORA_OK;
 }
 
+// Do two sets of T rows of `width` 16-bit elements share memory?  (Rows side by side in one wider buffer do not.)
+bool rows_overlap(const void* a, int64_t a_stride, const void* b, int64_t b_stride, int64_t width, int64_t T) {
+  const int64_t d = (static_cast<const char*>(b) - static_cast<const char*>(a)) / 2;  // rows start on 16 bytes
+  if (d >= (T - 1) * a_stride + width || -d >= (T - 1) * b_stride + width) return false;
+  if (T > 1 && a_stride == b_stride) {
+    const int64_t r = (d % a_stride + a_stride) % a_stride;
+    return r < width || a_stride - r < width;
+  }
+  return true;
+}
+// Rows that are written while others are still read: the same ones, or none of them.
+int check_in_place(const void* from, int64_t from_stride, const void* to, int64_t to_stride, int64_t width, int64_t T, const char* name) {
+  if (from == to && (T <= 1 || from_stride == to_stride)) return SLORA_OK;
+  return rows_overlap(from, from_stride, to, to_stride, width, T) ? fail(SLORA_ERR_SHAPE, "%s_out overlaps %s and is not the same rows", name, name)
+                                                                  : SLORA_OK;
+}
+
 int check_rotary(int head_dim, int rot, int layout, const void* positions, const void* turns, RotaryArgs* out, float factor,
                  int inverse) {
   if (rot < 16 || rot > head_dim || rot % 16 != 0)
@@ -354,6 +371,7 @@ int slora_rotary(void* q_out, void* k_out, const void* q, const void* k, int64_t
     if (heads[i] == 0) continue;
     if (int rc = check_rows(src[i], ss[i], static_cast<int64_t>(heads[i]) * head_dim, T, names[i][0])) return rc;
     if (int rc = check_rows(dst[i], ds[i], static_cast<int64_t>(heads[i]) * head_dim, T, names[i][1])) return rc;
+    if (int rc = check_in_place(src[i], ss[i], dst[i], ds[i], static_cast<int64_t>(heads[i]) * head_dim, T, names[i][0])) return rc;
     a.src[i] = src[i];
     a.dst[i] = dst[i];
     a.src_stride[i] = ss[i];
@@ -395,6 +413,7 @@ int slora_kv8_append(const slora_kv8_cache* cache, const slora_kv8_batch* batch,
     if (q_heads < 1 || q_heads > 65535) return fail(SLORA_ERR_SHAPE, "append: q_heads=%d", q_heads);
     if (int rc = check_rows(q, q_stride, static_cast<int64_t>(q_heads) * a.c.d, T, "q")) return rc;
     if (int rc = check_rows(q_out, q_out_stride, static_cast<int64_t>(q_heads) * a.c.d, T, "q_out")) return rc;
+    if (int rc = check_in_place(q, q_stride, q_out, q_out_stride, static_cast<int64_t>(q_heads) * a.c.d, T, "q")) return rc;
   }
   a.q = q;
   a.q_out = q_out;
@@ -458,6 +477,8 @@ int slora_kv8_attend(const slora_kv8_cache* cache, const slora_kv8_batch* batch,
   const int64_t width = static_cast<int64_t>(q_heads) * a.c.d;
   if (int rc = check_rows(q, q_stride, width, T, "q")) return rc;
   if (int rc = check_rows(out, out_stride, width, T, "out")) return rc;
+  if (add_weights && rows_overlap(q, q_stride, out, out_stride, width, T))
+    return fail(SLORA_ERR_SHAPE, "attend: out overlaps q, which add_weights reads again");
   const AttendLayout l = attend_layout(a.c, a.b, q_heads, add_weights);
   if (!workspace || workspace_bytes < l.total)
     return fail(SLORA_ERR_WORKSPACE, "attend: workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : 0, l.total);

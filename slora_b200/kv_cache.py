@@ -242,7 +242,8 @@ class KvCache8:
         A sequence's new tokens are its last: query ``j`` sees positions up to ``kv_len - q_len + j``, the last ``window``
         of them when ``window`` > 0.  ``heads`` is a multiple of the cache's KV heads.  ``scale`` defaults to
         ``head_dim ** -0.5``; ``lse`` (FP32 ``[T, heads]``) receives the logarithm of the softmax's sum.  A query that sees
-        nothing gives 0 and ``-inf``; rows that belong to no sequence are left as they are.  ``add_weights`` adds every
+        nothing gives 0 and ``-inf``; rows that belong to no sequence are left as they are.  ``out`` may be ``q`` unless
+        ``add_weights`` is set, which reads q again.  ``add_weights`` adds every
         key's attention weight, summed over queries and the heads of its KV head, to ``weights[layer]`` (on pages that
         several sequences share their sums arrive in no fixed order; all else does not depend on timing).
         C entry ``slora_kv8_attend``.

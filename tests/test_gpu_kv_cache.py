@@ -1108,3 +1108,12 @@ def test_a_refused_layer_changes_nothing():
     q, k, v = (b.clone() for b in base)
     ops.lora_get_qkv(0, wl.x_qkv[0], q, k, v, rope=(table, pos), kv_dest=(w.cache, w.batch))
     assert not torch.equal(q, base[0]) and w.batch.status() == 0
+
+
+def test_out_may_be_q_without_weights():
+    w = World([700, 300, 40, 2000], [300, 5, 1, 1], 2, 128, 16, "int8")
+    q = torch.randn(w.T, 8, 128, device=DEV).half()
+    want = w.cache.attend(0, w.batch, q, out=q.clone())
+    with pytest.raises(RuntimeError, match="overlaps"):
+        w.cache.attend(0, w.batch, q, out=q, add_weights=True)
+    assert w.cache.attend(0, w.batch, q, out=q) is q and torch.equal(q, want)

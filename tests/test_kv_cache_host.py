@@ -98,6 +98,23 @@ def test_attend_is_refused():
     assert plain > 0 and more >= plain + 2 * 4 * 4
 
 
+def test_rows_that_overlap_are_refused():
+    # two tokens of four heads of 128.  What passes is stopped by the next check (no workspace, no k), so that nothing is launched
+    rope = dict(pos=FAKE, turns=FAKE, rot=128, q=FAKE, hq=4, qs=512)
+
+    def rotary(q_out, stride, q_stride):
+        return L.slora_rotary(q_out, FAKE, FAKE, 0, 2, 4, 2, 128, 128, stride, 256, q_stride, 256, FAKE, FAKE, 1.0, 0, 0, 0, 0)
+
+    for out, stride in ((FAKE + 16, 512), (FAKE + 512 * 2 - 16, 512), (FAKE, 520), (FAKE + 1024, 1024), (FAKE - 16, 512)):
+        for rc in (_append(**rope, q_out=out, qos=stride), rotary(out, stride, 512), _attend(out=out, os=stride, add=1, ws=0)):
+            assert rc == -4 and b"overlaps" in L.slora_last_error()
+    assert _attend(add=1, out=FAKE, ws=0) == -4 and b"overlaps" in L.slora_last_error()     # the weights read q again
+    assert _attend(out=FAKE, ws=0) == -6 and rotary(FAKE, 512, 512) == -1                   # in place
+    for out in (FAKE + 1024, FAKE + 2048, FAKE - 1024, FAKE + 3 * 1024):                    # side by side in a wider buffer
+        assert rotary(out, 2048, 2048) == -1 and _attend(qs=2048, out=out, os=2048, add=1, ws=0) == -6
+    assert rotary(FAKE + 2 * 1024, 512, 512) == -1 and _attend(out=FAKE + 2 * 1024, add=1, ws=0) == -6   # one behind the other
+
+
 def test_evict_is_refused():
     assert _evict(_cache(weights=0)) == -1 and _evict(kept=0) == -1 and _evict(dest=0) == -1
     assert _evict(budget=0) == -4 and _evict(recent=-1) == -4 and _evict(sink=-1) == -4 and _evict(recent=20, sink=20) == -4
