@@ -1117,3 +1117,63 @@ def test_out_may_be_q_without_weights():
     with pytest.raises(RuntimeError, match="overlaps"):
         w.cache.attend(0, w.batch, q, out=q, add_weights=True)
     assert w.cache.attend(0, w.batch, q, out=q) is q and torch.equal(q, want)
+
+
+@pytest.mark.parametrize("new,io", [(1, "fp16"), (2, "bf16")])
+def test_a_sequence_in_more_parts_than_the_join_holds_at_once(new, io):
+    # 60000 keys of one KV head: every CTA has a part of them
+    w = World([60000], [new], 1, 128, 128, "int8", track=False)
+    _run_attend(w, 8, io)
+    _run_attend(w, 8, io, window=50000)
+
+
+@pytest.mark.parametrize("lens,new,hq,hkv,d,kind", [
+    ([700, 5, 130], [1, 1, 1], 8, 2, 128, "int8"),
+    ([700, 5, 130], [3, 2, 17], 8, 2, 64, "e4m3"),
+    ([700, 5, 130], [1, 1, 1], 8, 2, 256, "int8"),
+    ([700, 5, 130], [40, 2, 9], 8, 2, 256, "e4m3"),
+])
+@pytest.mark.parametrize("window", [0, 90])
+def test_weights_with_scores_computed_again(lens, new, hq, hkv, d, kind, window):
+    # a table for 2^24 tokens a sequence: scores of that many keys are not kept
+    w = World(lens, new, hkv, d, 128, kind, max_pages=1 << 17)
+    _run_attend(w, hq, "fp16", window=window, weights=True)
+
+
+def test_calls_from_several_threads():
+    import threading
+    sl = _sl()
+    page, results = [16, 32, 64, 128], {}
+
+    def work(i):
+        try:
+            w = World([300 + 7 * i, 90], [1 + 60 * (i % 3), 5], 2, 64 * (1 + i % 2), page[i % 4], "int8", seed=i)
+            d = w.d
+            table, pos = sl.RotaryTable(d), torch.arange(w.T, device=DEV)
+            g = torch.Generator().manual_seed(i)
+            stream = torch.cuda.Stream()
+            torch.cuda.synchronize()
+            with torch.cuda.stream(stream):
+                for _ in range(10):
+                    q, x = (torch.randn(w.T, h, d, generator=g).half().to(DEV) for h in (8, 2))
+                    q = w.cache.append(0, w.batch, x, x, q=q, rope=(table, pos))
+                    out = w.cache.attend(0, w.batch, q, out=torch.zeros_like(q), add_weights=True)
+                w.cache.evict(0, w.batch, 64, 8)
+                stream.synchronize()
+            results[i] = (w, q, out)
+        except BaseException as e:      # shown by the main thread
+            results[i] = e
+
+    for run in range(2):
+        threads = [threading.Thread(target=work, args=(i,)) for i in range(8)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        for i in range(8):
+            assert not isinstance(results[i], BaseException), results[i]
+            assert results[i][0].batch.status() == 0
+        if run == 0:
+            first = {i: results[i][2].clone() for i in range(8)}
+        else:
+            assert all(torch.equal(first[i], results[i][2]) for i in range(8))
