@@ -21,11 +21,11 @@
 // replaces S(j) and S(j + 1) replaces P(j): the MMAs of a CTA run in order, so the commit behind S(j + 1) also says that
 // O has P(j) V(j).
 //
-// Chunks of 4 prompts (3521 new tokens behind 2002 to 4352 cached ones, 64 q heads on 8, d 128, int8): 790 us, 498 TFLOP/s, 0.29
-// of the measured rate of a large matrix product (d 64: 630 us); the simple form of the same loop took 3136 us.  What bounds
+// Chunks of 4 prompts (3521 new tokens behind 2002 to 4352 cached ones, 64 q heads on 8, d 128, int8): 735 us, 536 TFLOP/s, 0.32
+// of the measured rate of a large matrix product (d 64: 566 us); the simple form of the same loop took 3136 us.  What bounds
 // it is the chain of one row tile (scores out of tensor memory, p back: 3700 cycles for four warps; then the product and
 // the next scores), of which two run side by side.  Without the exponentials it takes as long; without the conversion 6 %
-// less; with one reference for all rows of a CTA (which let pages that a row does not see round its p) 2 to 3 % less.
+// less; with one reference for all rows of a CTA (which let pages that a row does not see round its p) 3 to 4 % less.
 //
 // Every wait is bounded; a CTA that gives up records SLORA_STATUS_TIMEOUT and frees its tensor memory.
 #pragma once
@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(kPreThreads, 1) kv_prefill_kernel(const KvAtte
       if (!again)
         again = masked ? pre_exp<D, true>(sm, slot, t_s, down, m == kNegInf ? 0.f : m, ref, &sum, from - key, to - key, p)
                        : pre_exp<D, false>(sm, slot, t_s, down, m == kNegInf ? 0.f : m, ref, &sum, 0, 0, p);
-      again = again || m == kNegInf;
+      again = again || (m == kNegInf && to > key && from < key + kPreKeys);  // a row's first keys (a row without any waits for none)
       if (__any_sync(0xffffffffu, again || ref != was)) {
         float f = was > kNoRef ? pre_pow2(fmaxf(was - ref, -126.f)) : 1.f;
         const bool anew = __any_sync(0xffffffffu, again);

@@ -378,6 +378,24 @@ def test_scales_that_differ_from_page_to_page(lens, new, hq, hkv, d, page, kind,
     _check_rows(w, q, w.cache.attend(0, w.batch, q, window=window), window)
 
 
+def test_rows_that_are_not_there_cost_no_time():
+    # 64 rows of a 256-row tile: those that see no key must not send their warps the long way (it took twice the time of 256)
+    def took(new):
+        w = World([4096], [new], 1, 128, 128, "int8", track=False)
+        q = torch.randn(w.T, 8, 128, device=DEV).bfloat16()
+        times = []
+        for _ in range(12):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            w.cache.attend(0, w.batch, q)
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b))
+        return sorted(times)[len(times) // 2]
+
+    assert took(8) < 1.5 * took(32)
+
+
 def test_strided_rows_and_scale():
     sl = _sl()
     w = World([300, 20], [1, 3], 2, 64, 16, "int8")
