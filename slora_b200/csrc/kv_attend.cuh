@@ -879,31 +879,36 @@ __global__ void __launch_bounds__(kJoinThreads) kv_join_kernel(const KvAttendArg
 }
 
 // Accumulated attention weights from the stored scores: w[key] += sum over the rows of 2^(score - lse).  Runs of tiles, as in
-// the attention but over (sequence, KV head) only: a warp adds up a tile's row blocks in their order and adds the sum to
-// the cache once, so that weights do not depend on timing either.  A lane takes a key of the tile and half of its rows.
-template <int D>
-__global__ void __launch_bounds__(kAttendThreads) kv_weights_kernel(const KvAttendArgs a) {
+// the attention but over (sequence, KV head) only.  A lane takes a key of a tile and half of a block's rows.  A warp has a run
+// of its own and goes through a tile's row blocks in their order; with many of them (SPLIT) a CTA has the run, and teams of 2
+// to 16 warps share a tile's row blocks and add up their sums in a fixed order.  Either way one addition per token to the
+// cache, so that weights do not depend on timing.
+template <int D, bool SPLIT>
+__global__ void __launch_bounds__(SPLIT ? 512 : kAttendThreads) kv_weights_kernel(const KvAttendArgs a) {
+  constexpr int kWarps = SPLIT ? 16 : kAttendWarps, kRuns = SPLIT ? 1 : kWarps;  // runs of a CTA
   __shared__ KvFind find;
+  __shared__ float part[SPLIT ? 2 : 1][SPLIT ? kWarps : 1][4 * kAttendTile];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_launch_dependents();
   pdl_wait();
-  const int me = blockIdx.x * kAttendWarps + warp;
-  const int runs = gridDim.x * kAttendWarps;
+  const int me = blockIdx.x * kRuns + (SPLIT ? 0 : warp);
+  const int runs = gridDim.x * kRuns;
   // units: what a sequence costs in the attention, a row block's worth of it
   auto units = [&](const KvSeq& s) {
     if (s.q < a.min_q || s.q > a.lim_q || s.q == 0) return 0ll;
     const KvRange r = kv_tiles(s, a.window);
     return static_cast<long long>(r.hi - r.lo + kAttendPiece) * a.c.hkv;
   };
-  const long long total = kv_find<kAttendWarps, kAttendWarps>(
+  auto run_of = [&](long long n) { return SPLIT ? (n + runs - 1) / runs : kv_run(n, runs); };
+  const long long total = kv_find<kWarps, kRuns>(
       a.b.n_seq, &find, [&](int i) { return units(kv_seq(a.b, i)); },
-      [&](long long n, int k) { return static_cast<long long>(blockIdx.x * kAttendWarps + k) * kv_run(n, runs); });
-  const long long run = kv_run(total, runs);
+      [&](long long n, int k) { return static_cast<long long>(blockIdx.x * kRuns + k) * run_of(n); });
+  const long long run = run_of(total);
   long long u = me * run;
   const long long u_end = min(u + run, total);
   if (u >= u_end) return;
-  int seq = find.seq[warp];
-  long long seq_at = find.at[warp];
+  int seq = find.seq[SPLIT ? 0 : warp];
+  long long seq_at = find.at[SPLIT ? 0 : warp];
   long long scores_at = seq_at;  // cost units of the attention before the sequence: where its scores start
   if (a.blocks > 1) {
     scores_at = 0;
@@ -914,6 +919,7 @@ __global__ void __launch_bounds__(kAttendThreads) kv_weights_kernel(const KvAtte
   KvSeq s = kv_seq(a.b, seq);
   long long n_units = units(s);
   const int key_in = lane & 15, half = lane >> 4;
+  int buf = 0;
   while (u < u_end) {
     while (u >= seq_at + n_units) {
       seq_at += n_units;
@@ -929,6 +935,8 @@ __global__ void __launch_bounds__(kAttendThreads) kv_weights_kernel(const KvAtte
     const int until = static_cast<int>(min(static_cast<long long>(piece), at + (u_end - u)));
     u += until - at;
     const int all_rows = s.q * a.group, blocks = (all_rows + a.rows_per_block - 1) / a.rows_per_block;
+    const int team = SPLIT ? (blocks > 8 ? 16 : blocks > 4 ? 8 : blocks > 2 ? 4 : 2) : 1;  // warps that share a tile's blocks
+    const int mate = SPLIT ? warp % team : 0, first = SPLIT ? 4 * (warp / team) : 0, step = SPLIT ? 4 * (kWarps / team) : 4;
     const float* const scores = a.scores + (scores_at + static_cast<long long>(head) * piece + kAttendPiece) * (a.part_rows * kAttendTile) + lane;
     const long long block_step = static_cast<long long>(a.c.hkv) * piece * (a.part_rows * kAttendTile);
     // lane r holds lse of row r of a block (32 rows at most)
@@ -948,29 +956,50 @@ __global__ void __launch_bounds__(kAttendThreads) kv_weights_kernel(const KvAtte
         if (p >= 0) place = static_cast<int>(((p * a.c.hkv + head) << a.c.shift) + (key_l & ((1 << a.c.shift) - 1)));
       }
       const int n = min(32, end - i0);
-      for (int i = 0; i < n; i += 4) {  // four tiles at a time: their loads overlap
+      // an atomic add only because sequences may share a page (then in no fixed order); else one add per token
+      auto add = [&](int tile, int key, int to, float sum) {
+        if (to >= 0 && (range.lo + i0 + tile) * kAttendTile + key < s.kv && sum != 0.f) atomicAdd(a.c.w + to + key, sum);
+      };
+      for (int i = 0; i < n; i += step) {  // four tiles a warp: their loads overlap
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int rb = 0; rb < blocks; ++rb) {
+        for (int rb = mate; rb < blocks; rb += team) {
           if (blocks > 1) lse_l = lse_of(rb);
           const int rows = min(a.rows_per_block, all_rows - rb * a.rows_per_block);
-          const float* const src = scores + rb * block_step + static_cast<int64_t>(i0 + i) * (a.part_rows * kAttendTile);
+          const float* const src = scores + rb * block_step + static_cast<int64_t>(i0 + i + first) * (a.part_rows * kAttendTile);
 #pragma unroll 4
           for (int r0 = 0; r0 < rows; r0 += 2) {
             const float lse = __shfl_sync(0xffffffffu, lse_l, r0 + half);
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
-              const float x = r0 + half < rows && i + t < n ? src[(t * a.part_rows + r0) * kAttendTile] : kNegInf;
+              const float x = r0 + half < rows && i + first + t < n ? src[(t * a.part_rows + r0) * kAttendTile] : kNegInf;
               sum[t] += lse > kNegInf ? ex2(x - lse) : 0.f;
             }
           }
         }
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          if (i + t >= n) break;
-          const float add = sum[t] + __shfl_down_sync(0xffffffffu, sum[t], 16);
-          const int to = __shfl_sync(0xffffffffu, place, i + t);
-          // an atomic add only because sequences may share a page (then in no fixed order); else one add per token
-          if (to >= 0 && half == 0 && (range.lo + i0 + i + t) * kAttendTile + key_in < s.kv && add != 0.f) atomicAdd(a.c.w + to + key_in, add);
+        for (int t = 0; t < 4; ++t) sum[t] += __shfl_down_sync(0xffffffffu, sum[t], 16);
+        if (!SPLIT) {
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            if (i + t >= n) break;
+            const int to = __shfl_sync(0xffffffffu, place, i + t);
+            if (half == 0) add(i + t, key_in, to, sum[t]);
+          }
+        } else {
+          if (half == 0) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t) part[buf][warp][t * kAttendTile + key_in] = sum[t];
+          }
+          __syncthreads();
+          // two warps per team: a thread adds up its team's sums of one key
+          if (tid < 64 * (kWarps / team)) {
+            const int of = tid >> 6, tile = i + 4 * of + (tid >> 4 & 3);
+            const int to = __shfl_sync(0xffffffffu, place, tile & 31);
+            float all = 0.f;
+            for (int x = 0; x < team; ++x) all += part[buf][of * team + x][tid & 63];
+            if (tile < n) add(tile, key_in, to, all);
+          }
+          buf ^= 1;
         }
       }
     }

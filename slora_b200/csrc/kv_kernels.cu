@@ -226,11 +226,28 @@ int attend_tiles(int max_q, int group, int d) {
 }
 int attend_grid(int nt, int d) { return sm_count() * attend_ctas(nt, d); }
 
-// Sequences with at least this many rows go to the tensor-memory kernel (kv_prefill.cuh), the others to kv_attend.cuh.
+// Which sequences go to the tensor-memory kernel (kv_prefill.cuh): those with at least kPrefillRows rows, or, where a batch
+// has few (sequence, KV head) pairs, with kPrefillShare / pairs.  That kernel does not split keys: an item of 256 rows takes
+// 3 to 4 us per 128 keys on an SM of its own, however many SMs are idle, while the row kernel spreads any work over all
+// of them at 8.6 ns per 128 keys and 16 rows.  Measured (d 128, us, row kernel / tensor-memory kernel):
+//   24 sequences x 8 heads, 4096 keys:  56 rows 209 / -, 64 rows 211 / 333, 128 rows 398 / 323, 256 rows 774 / 271
+//   4 sequences x 8 heads, 8192 keys:   64 rows 82 / 292, 128 rows 141 / 253, 256 rows 254 / 230
+//   1 sequence, one KV head, 32768 keys: 64 rows 39 / 945, 256 rows 51 / 767
+// head_dim 256 has no tensor-memory kernel: its operands do not fit.
 constexpr int kPrefillRows = 64;
+constexpr int64_t kPrefillShare = 6144;
 
-// The scores that add_weights keeps take 4 bytes per key and row; beyond this many bytes they are computed again.
+// The scores that add_weights keeps take 4 bytes per key and row.  With them the row kernel takes all rows (128 keys and 16
+// rows: 8.6 ns and 1.5 for the weights; the tensor-memory kernel 1.3, but 15 for the scores again).  Beyond this many bytes,
+// if every sequence were as long as the table allows, they are computed again (32 sequences of 4096 keys, 32 heads on 8,
+// one token each: weights kept 88 us, computed again 123): it bounds the workspace.
 constexpr int64_t kMaxScoreBytes = int64_t(1) << 29;
+
+// When the weights are added up, the warps of a CTA share a tile's row blocks where there are more than kSplitBlocks, or more
+// than one and fewer (sequence, KV head) pairs than SMs.  Weights alone, us, a warp all blocks / shared (d 128):
+//   24 sequences x 8 heads, 3 blocks, 4000 keys: 90 / 115;  5 blocks, 2000 keys: 141 / 145
+//   4 x 8 heads, 8 blocks, 2000 keys: 185 / 34;  1 x 1 head, 400 blocks, 1000 keys: 6900 / 86
+constexpr int kSplitBlocks = 4;
 
 struct AttendLayout {
   int nt, grid, part_rows;
@@ -238,18 +255,36 @@ struct AttendLayout {
   int split;           // q_len from which sequences are the prefill kernel's; above max_q: none
   int64_t pre_grid;    // its items, at most
   bool keep_scores;
+  bool split_weights;
   size_t part, rec, lse, scores, total;
 };
 AttendLayout attend_layout(const KvCache& c, const KvBatch& b, int hq, int add_weights) {
   AttendLayout l;
   const int group = hq / c.hkv;
-  l.split = c.d <= 128 ? (kPrefillRows + group - 1) / group : 0x7fffffff;
-  const bool pre = b.max_q >= l.split;
-  const int most_q = pre ? l.split - 1 : b.max_q;
-  l.nt = attend_tiles(most_q, group, c.d);
-  const int64_t rows = static_cast<int64_t>(most_q) * group;
-  l.part_rows = static_cast<int>(rows < 1 ? 1 : rows < 8 * l.nt ? rows : 8 * l.nt);
   const int64_t seqs = b.n_seq < b.T ? b.n_seq : b.T;
+  double bytes = 0;  // of the scores
+  // the row kernel's part, for sequences of up to most_q new tokens
+  const auto rows_up_to = [&](int most_q) {
+    l.nt = attend_tiles(most_q, group, c.d);
+    const int64_t rows = static_cast<int64_t>(most_q) * group;
+    l.part_rows = static_cast<int>(rows < 1 ? 1 : rows < 8 * l.nt ? rows : 8 * l.nt);
+    l.blocks = static_cast<int>((rows + 8 * l.nt - 1) / (8 * l.nt));
+    // cost units of all pieces (see kv_attend.cuh), if every sequence were as long as the page table allows
+    const double units =
+        static_cast<double>(b.n_seq) * (static_cast<double>(b.max_tokens / kAttendTile) + 1 + kAttendPiece) * c.hkv * l.blocks;
+    bytes = units * l.part_rows * kAttendTile * sizeof(float);
+  };
+  l.split = 0x7fffffff;
+  rows_up_to(b.max_q);
+  l.keep_scores = add_weights && bytes <= static_cast<double>(kMaxScoreBytes);
+  const int64_t pairs = seqs * c.hkv > 0 ? seqs * c.hkv : 1;
+  l.split_weights = l.blocks > kSplitBlocks || (l.blocks > 1 && pairs < sm_count());
+  if (!l.keep_scores && c.d <= 128) {
+    const int64_t rows = kPrefillShare / pairs > kPrefillRows ? kPrefillShare / pairs : kPrefillRows;
+    l.split = static_cast<int>((rows + group - 1) / group);
+  }
+  const bool pre = b.max_q >= l.split;
+  if (pre) rows_up_to(l.split - 1);
   l.pre_grid = pre ? (b.T * group / kPreRows + seqs) * c.hkv : 0;
   l.grid = attend_grid(l.nt, c.d);
   const auto up = [](size_t x) { return (x + 15) & ~static_cast<size_t>(15); };
@@ -258,12 +293,6 @@ AttendLayout attend_layout(const KvCache& c, const KvBatch& b, int hq, int add_w
   l.rec = up(2u * runs * l.part_rows * (c.d + 4) * sizeof(float));
   l.lse = l.rec + up(runs * 16);
   l.scores = l.lse + (add_weights ? up(static_cast<size_t>(b.T) * hq * sizeof(float)) : 0);
-  // cost units of all pieces (see kv_attend.cuh), if every sequence were as long as the page table allows
-  const int64_t blocks = (rows + 8 * l.nt - 1) / (8 * l.nt);
-  l.blocks = static_cast<int>(blocks);
-  const double units = static_cast<double>(b.n_seq) * (static_cast<double>(b.max_tokens / kAttendTile) + 1 + kAttendPiece) * c.hkv * blocks;
-  const double bytes = units * l.part_rows * kAttendTile * sizeof(float);
-  l.keep_scores = add_weights && !pre && bytes <= static_cast<double>(kMaxScoreBytes);
   l.total = l.scores + (l.keep_scores ? up(static_cast<size_t>(bytes)) : 0);
   return l;
 }
@@ -294,7 +323,9 @@ int attend_launch(KvAttendArgs a, const AttendLayout& l, int add_weights, cudaSt
   }
   rc = launch_pdl<kv_join_kernel<D, T>>(dim3(l.grid), kJoinThreads, 0, s, "kv8_attend join", a);
   if (rc || !add_weights) return rc;
-  if (l.keep_scores) return launch_pdl<kv_weights_kernel<D>>(dim3(8 * sm_count()), kAttendThreads, 0, s, "kv8_attend weights", a);
+  if (l.keep_scores)
+    return l.split_weights ? launch_pdl<kv_weights_kernel<D, true>>(dim3(2 * sm_count()), 512, 0, s, "kv8_attend weights", a)
+                           : launch_pdl<kv_weights_kernel<D, false>>(dim3(8 * sm_count()), kAttendThreads, 0, s, "kv8_attend weights", a);
   a.rows_per_block = 8;
   return launch_pdl<kv_reweigh_kernel<D, KIND, T>>(dim3(attend_grid(1, D)), kAttendThreads, 0, s, "kv8_attend weights", a);
 }

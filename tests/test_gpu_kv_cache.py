@@ -1195,3 +1195,64 @@ def test_calls_from_several_threads():
             first = {i: results[i][2].clone() for i in range(8)}
         else:
             assert all(torch.equal(first[i], results[i][2]) for i in range(8))
+
+
+@pytest.mark.parametrize("hq,hkv,d,page,kind,io", [(32, 16, 128, 16, "int8", "bf16"), (64, 16, 64, 64, "e4m3", "fp16"),
+                                                   (48, 16, 128, 128, "e4m3", "fp16"), (16, 16, 64, 32, "int8", "bf16")])
+@pytest.mark.parametrize("window", [0, 100])
+def test_chunks_of_a_batch_with_many_heads(hq, hkv, d, page, kind, io, window):
+    # with this many (sequence, KV head) pairs the tensor-memory kernel takes sequences of 64 rows and more
+    new = [64, 70, 1, 0, 130, 200, 33, 22, 300]
+    lens = [64, 470, 300, 20, 129, 333, 900, 22, 1000]
+    w = World(lens, new, hkv, d, page, kind)
+    _run_attend(w, hq, io, window=window)
+    # capacity for 2^24 tokens: the scores are not kept
+    w = World(lens, new, hkv, d, page, kind, max_pages=(1 << 24) // page)
+    _run_attend(w, hq, io, window=window, weights=True)
+
+
+@pytest.mark.parametrize("lens,new,hq,hkv", [([1000], [400], 16, 1), ([2000, 700, 30], [100, 40, 30], 8, 2), ([9000], [1], 64, 1)])
+def test_many_rows_of_few_heads(lens, new, hq, hkv):
+    # few (sequence, KV head) pairs: the row kernel, its keys split over the GPU; the weights from kept scores
+    for d in (64, 128):
+        w = World(lens, new, hkv, d, 32, "int8")
+        _run_attend(w, hq, "bf16")
+        _run_attend(w, hq, "fp16", window=200, weights=True)
+
+
+@pytest.mark.parametrize("lens,new,hq,hkv,max_pages", [
+    ([300 + 11 * i for i in range(20)], [5] * 20, 64, 8, None),        # many heads: a warp goes through all row blocks
+    ([1000], [400], 16, 1, None),                                      # many row blocks: shared by the warps of a CTA
+    ([900, 300], [60, 9], 16, 2, 1 << 17),                             # scores computed again
+])
+def test_weights_repeat_whichever_way_they_are_added_up(lens, new, hq, hkv, max_pages):
+    w = World(lens, new, hkv, 128, 128 if max_pages else 32, "int8", max_pages=max_pages)
+    q = torch.randn(w.T, hq, 128, device=DEV, dtype=torch.bfloat16)
+    before, first = w.w.clone(), None
+    for _ in range(15):
+        w.w.copy_(before)
+        w.cache.attend(0, w.batch, q, add_weights=True)
+        first = w.w.clone() if first is None else first
+        assert torch.equal(w.w, first)
+    w.w.copy_(before)
+    _run_attend(w, hq, "bf16", weights=True)
+
+
+def test_few_heads_have_the_whole_gpu():
+    # one KV head: 64 rows took 25 times the time of 56 (one CTA walked the whole context), the weights of a chunk 15 times the
+    # attention's
+    def took(n, new, hq, weights):
+        w = World([n], [new], 1, 128, 128, "int8")
+        q = torch.randn(w.T, hq, 128, device=DEV).bfloat16()
+        times = []
+        for _ in range(12):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            w.cache.attend(0, w.batch, q, add_weights=weights)
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b))
+        return sorted(times)[len(times) // 2]
+
+    assert took(32768, 1, 64, False) < 3 * took(32768, 1, 56, False)
+    assert took(1000, 400, 16, True) < 6 * took(1000, 400, 16, False)
