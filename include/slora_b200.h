@@ -515,7 +515,8 @@ int slora_rotary(void* q_out, void* k_out, const void* q, const void* k, int64_t
  * its page as 0.  Rounding is to nearest, ties to even, of the exact quotient.  NaN is stored as 0 and infinities as the
  * largest value (both leave the scale alone) with SLORA_STATUS_NONFINITE.  weights of new tokens, where the cache has
  * them, become 0.  Positions beyond kv_len of the last page are left as they are.
- * A page that is appended to must belong to one sequence.
+ * A page that is appended to must belong to one sequence.  Of a sequence with q_len > kv_len the last kv_len rows are
+ * appended and BAD_TABLE is set; its first rows have no position, and their q is not turned.
  */
 #define SLORA_STATUS_NONFINITE 16 /* a NaN or an infinity was appended to an 8-bit cache */
 int slora_kv8_append(const slora_kv8_cache* cache, const slora_kv8_batch* batch, const void* k, const void* v,
@@ -537,7 +538,11 @@ int slora_kv8_read(const slora_kv8_cache* cache, const slora_kv8_batch* batch, c
  * A query that sees no key gives 0 and lse -inf.  add_weights != 0: cache->weights += the p of every key, summed over
  * the step's queries and over the q heads of its KV head.  Results do not depend on timing, with one exception: a page that
  * several of the batch's sequences share gets their sums in no fixed order.
- * out may be q unless add_weights is set, which reads q again.
+ * out may be q unless add_weights is set, which reads q again.  q_len > kv_len is no error here: the first queries see no key.
+ * Scores and sums are FP32; p times the v scale goes into its product as f16, off by 2^-11 of itself or, where it is small,
+ * by 2^-21 of the largest such product among the keys that lie together (16, or 128 in long chunks) and that the row sees.
+ * add_weights keeps scores in the workspace, 4 bytes per key and row for max_pages * page_tokens keys of every sequence,
+ * up to 512 MB, and computes them again beyond that.
  * workspace: slora_kv8_attend_workspace_bytes(...) bytes of device memory, 16-byte aligned, contents irrelevant; calls
  * that may overlap on the GPU need workspaces of their own.
  */

@@ -196,7 +196,7 @@ class LoraBatchOps:
         ``rope=(table, positions)`` with a :class:`~slora_b200.RotaryTable` and the tokens' positions takes any of its
         layouts and scalings; ``kv_dest=(cache, batch)`` with a :class:`~slora_b200.KvCache8` and the step's
         :class:`~slora_b200.KvBatch` puts the new k and v into the layer's 8-bit pages (turned first when ``rope`` is
-        given).  Both run behind the expand, in one launch (two when sequences have more than four new tokens and q is
+        given).  Both run behind the expand, in one launch (two when `max_q_len` is above four and q is
         turned); q, k and v hold base plus delta in place (q turned).  A call that is refused changes nothing.
         """
         kb, vb, rows, stride = self._common(layer_id)

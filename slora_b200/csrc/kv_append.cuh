@@ -5,16 +5,16 @@
 // the remainder goes to sincospif.  Cosines and sines of a block of tokens are worked out once, in shared memory, and
 // serve all heads.  A row of a head is 8 elements a lane (16-byte loads and stores); in the half layout the partner of a
 // value sits rot / 16 lanes away (one shuffle per element), in the interleaved layout in the same lane.
-// What bounds it: q, k read and written once (16-bit), at the copy rate: 8191 tokens of 64 + 8 heads of 128, half of each turned: 53 us, 0.87
-// of it.  One token: 9 us, all of them the call's and the launch's.
+// What bounds it: q, k read and written once (16-bit), at the copy rate: 8191 tokens of 64 + 8 heads of 128, half of each
+// turned: 53 us, 0.86 of it.  One token: 10 us, all of them the call's and the launch's.
 //
 // Append: the new tokens of one page belong to one CTA (the scale of a (page, head) is a maximum over them): all warps take
 // a (head, k or v) together when there are many tokens, one warp each when there are few (decode).  When the scale grows,
-// the page's older values are rounded to the new one in place.  Pages with more than kAppendWarpTokens new tokens take two
-// launches, q by tokens and k, v by heads: one kernel for both had too many registers and instructions (236 against 152 us
+// the page's older values are rounded to the new one in place.  Batches with more than kAppendWarpTokens new tokens of a
+// sequence (max_q_len) take two launches, q by tokens and k, v by heads: one kernel for both had too many registers and instructions (236 against 152 us
 // then, 7983 tokens of 64 + 8 + 8 heads of 128; now 50 and 73 us).  What bounds it there is instructions (angles, exact
-// rounding) and the barriers of the two walks over a page; at decode a chain of loads: length, table, scale, values (77
-// sequences of 32 heads: 16 us).
+// rounding) and the barriers of the two walks over a page; at decode every CTA's scan over the lengths, with two barriers, and
+// then a chain of loads: table, scale, values (77 sequences of 32 heads: 16 us).
 #pragma once
 
 #include "kv_common.cuh"

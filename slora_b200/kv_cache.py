@@ -3,7 +3,7 @@
 The reference keeps KV rows in the pool's 16-bit type (``slora/common/mem_allocator.py:229-234``), one row per token, and
 its attention kernels read them there (``slora/models/llama/triton_kernel/token_attention_nopad_att1.py``).  Here a page
 holds ``page_tokens`` tokens of every KV head in 8 bits with one scale per (page, KV head): half the bytes that a decode
-step reads, and half the memory that the cache takes from the adapters.  Pages are rows of a
+step reads and half the memory, in buffers of the cache's own.  Pages are rows of a
 :class:`~slora_b200.MemoryAllocator` that owns no buffers.
 
 One layer of a step, between ``LoraBatchOps.lora_get_qkv`` and ``lora_get_o``::
@@ -178,7 +178,8 @@ class KvCache8:
         ``rope=(table, positions)`` turns k (which itself is not written) and, when given, q: in place, or into ``q_out``.
         Returns the turned q.  The scale of a (page, head) is the largest value over all its tokens; when a new token
         raises it, the page's older values are rounded to the new scale.  A page that is appended to must belong to one
-        sequence only.  C entry ``slora_kv8_append``.
+        sequence only.  Rows of no sequence are left as they are; of a sequence with more new tokens than ``kv_len`` the last
+        ``kv_len`` are appended, the others' q is not turned, and the status says so.  C entry ``slora_kv8_append``.
         """
         q_out, call = self._append_call(layer, batch, k, v, q, rope, q_out)
         _lib.call(*call)
@@ -243,7 +244,8 @@ class KvCache8:
         of them when ``window`` > 0.  ``heads`` is a multiple of the cache's KV heads.  ``scale`` defaults to
         ``head_dim ** -0.5``; ``lse`` (FP32 ``[T, heads]``) receives the logarithm of the softmax's sum.  A query that sees
         nothing gives 0 and ``-inf``; rows that belong to no sequence are left as they are.  ``out`` may be ``q`` unless
-        ``add_weights`` is set, which reads q again.  ``add_weights`` adds every
+        ``add_weights`` is set, which reads q again.  Up to 512 MB of scores are kept for the weights (by the capacity of the
+        page table, or ``max_kv_len``); beyond that they are computed again.  ``add_weights`` adds every
         key's attention weight, summed over queries and the heads of its KV head, to ``weights[layer]`` (on pages that
         several sequences share their sums arrive in no fixed order; all else does not depend on timing).
         C entry ``slora_kv8_attend``.
