@@ -491,8 +491,8 @@ typedef struct slora_kv8_batch { /* the sequences of a step; every table is devi
 
 /*
  * Rotary embedding of q [T][q_heads][head_dim] and k [T][k_heads][head_dim] (either may be NULL with 0 heads; rows
- * *_stride elements apart, heads contiguous) into q_out / k_out (which may be q / k, but not overlap them otherwise).  The first `rot` elements of a head
- * are turned, the others copied.  Pair i: elements (i, i + rot / 2) with layout 0 ("half", the reference's
+ * *_stride elements apart, heads contiguous) into q_out / k_out (which may be q / k, but not overlap them otherwise).
+ * The first `rot` elements of a head are turned, the others copied.  Pair i: elements (i, i + rot / 2) with layout 0 ("half", the reference's
  * rotary_emb_fwd, slora/models/llama/triton_kernel/rotary_emb.py:8-71), (2i, 2i + 1) with layout 1 ("interleaved").
  *   angle = 2 pi positions[t] turns[i] (turns: rot / 2 doubles, device), (c, s) = factor * (cos, sin) of the angle,
  *   y0 = x0 c - x1 s, y1 = x0 s + x1 c; inverse != 0 turns the other way, which is also the gradient's direction.

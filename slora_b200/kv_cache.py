@@ -244,10 +244,13 @@ class KvCache8:
         of them when ``window`` > 0.  ``heads`` is a multiple of the cache's KV heads.  ``scale`` defaults to
         ``head_dim ** -0.5``; ``lse`` (FP32 ``[T, heads]``) receives the logarithm of the softmax's sum.  A query that sees
         nothing gives 0 and ``-inf``; rows that belong to no sequence are left as they are.  ``out`` may be ``q`` unless
-        ``add_weights`` is set, which reads q again.  Up to 512 MB of scores are kept for the weights (by the capacity of the
-        page table, or ``max_kv_len``); beyond that they are computed again.  ``add_weights`` adds every
-        key's attention weight, summed over queries and the heads of its KV head, to ``weights[layer]`` (on pages that
-        several sequences share their sums arrive in no fixed order; all else does not depend on timing).
+        ``add_weights`` is set, which reads q again.  At head_dim 256 long chunks of prompts are slow: the cache is read once
+        per eight rows.
+
+        ``add_weights`` adds every key's attention weight, summed over queries and the heads of its KV head, to
+        ``weights[layer]``.  Up to 512 MB of scores are kept for that (by the capacity of the page table, or
+        ``max_kv_len``); beyond they are computed again.  On pages that several sequences share their sums arrive in no
+        fixed order; all else does not depend on timing.
         C entry ``slora_kv8_attend``.
         """
         d, dtype = self.head_dim, q.dtype
